@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define AQ_ABI_VERSION 13
+#define AQ_ABI_VERSION 14
 #define AQ_MAX_LEVELS 128     /* largest supported number of quantisation levels L */
 #define AQ_MAX_ABS_BETA 64.0f /* |beta| above this is rejected (exp() range of the kernels) */
 /* flags of aq_synth_fwd / aq_synth_bwd */
@@ -452,6 +452,69 @@ int aq_pkt_loss(const float *student, const float *teacher, int N, int Ds, int D
                 float *dstudent, void *workspace, size_t workspace_bytes, void *stream);
 /* K = (xh xh^T + 1) / 2 alone.  workspace: ceil256(N * D * 4) + ceil256(N * 4) bytes. */
 int aq_pkt_kernel_matrix(const float *feat, int N, int D, float eps, float *K, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- 8-bit floating point with a scale per block of 128 ------------------------------------------------------------
+ * No counterpart in the reference (parity unpinned).  A matrix [rows, cols] of e4m3 codes (1 sign, 4 exponent, 3 mantissa
+ * bits; finite up to 448; 0x7f / 0xff are NaN), row i at byte i * ld, with one scale per block: block_rows = 1: blocks of
+ * 1 x 128 along a row; block_rows = 128: tiles of 128 x 128 (the last blocks of odd sizes are smaller).  Scales
+ * [ceil(rows / block_rows), ceil(cols / 128)], row i at element i * lds, either one byte b standing for 2^(b - 127)
+ * (AQ_SCALE_POW2; 255 is NaN) or fp32 (AQ_SCALE_F32).  value = code * scale.  Element types of plain matrices: AQ_F32,
+ * AQ_BF16, AQ_F16; leading dimensions count elements; columns are contiguous. */
+#define AQ_F32 0
+#define AQ_BF16 1
+#define AQ_F16 2
+#define AQ_SCALE_POW2 0
+#define AQ_SCALE_F32 1
+/* Codes of x [rows, cols] and / or of its transpose.  Per block: amax over the finite |x|, scale = 2^ceil(log2(amax / 448))
+ * (at least 2^-126; 1 for a block of zeros), code = x / scale rounded to nearest even; a NaN or infinite x becomes NaN.
+ *   q, qs:   codes and scales of x (NULL: not wanted);  qt, qts: codes [cols, rows] and scales of x^T, blocks along ITS rows
+ *   colsum:  [cols] fp32 sum over the rows of x, in double (NULL: not wanted; needs qt, and the workspace of
+ *            aq_fp8_quantize_workspace_bytes(rows, cols), 8-byte aligned). */
+size_t aq_fp8_quantize_workspace_bytes(long long rows, long long cols);
+int aq_fp8_quantize(const void *x, int xtype, long long rows, long long cols, long long ldx, uint8_t *q, long long ldq, void *qs,
+                    long long ldqs, uint8_t *qt, long long ldqt, void *qts, long long ldqts, int block_rows, int scale_type,
+                    float *colsum, void *workspace, size_t workspace_bytes, void *stream);
+/* Codes and scales of the transpose of a matrix that is in the format already.  block_rows = 128: the same codes; block_rows =
+ * 1: the values are quantised again in blocks along the other axis (exact but for values that fall below the new block's
+ * smallest subnormal step). */
+int aq_fp8_transpose(const uint8_t *a, long long lda, const void *as, long long ldas, long long rows, long long cols, uint8_t *at,
+                     long long ldat, void *ats, long long ldats, int block_rows, int scale_type, void *stream);
+/* y[i, j] = code * scale, rounded to y's type. */
+int aq_fp8_dequantize(const uint8_t *q, long long ldq, const void *qs, long long ldqs, long long rows, long long cols, int block_rows,
+                      int scale_type, void *y, int ytype, long long ldy, void *stream);
+/* y [M, N] = A [M, K] . B [N, K]^T + bias[N] (NULL: none).  A, B and their pitches 16-byte aligned, every row readable up to
+ * the next multiple of 16 bytes (what lies behind K does not matter).  Sums in fp32.  bf16 / fp16 outputs: the 8-bit matrix
+ * instructions, which align the products of a group of 8 to the largest of them and drop what lies 2^-14 below it; fp32
+ * output: the codes as fp16 through the 16-bit instructions, whose sums keep fp32.  workspace:
+ * aq_fp8_matmul_workspace_bytes(M, N, K) bytes, 16-byte aligned (partial sums of products with few rows). */
+size_t aq_fp8_matmul_workspace_bytes(long long M, long long N, long long K);
+int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long ldas, int a_block_rows, const uint8_t *b, long long ldb,
+                  const void *bs, long long ldbs, int b_block_rows, long long M, long long N, long long K, int scale_type,
+                  const float *bias, void *y, int ytype, long long ldy, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- root-mean-square norm over rows, with the residual's addition ---------------------------------------------------
+ * h = round(x + res) (h = x without res), rstd = 1 / sqrt(mean(h^2) + eps), y = (h * rstd) * w; x, res, h, y of one type, w and
+ * rstd fp32.  Outputs that are not wanted are NULL.  q / qs: y in blocks of 1 x 128 as aq_fp8_quantize makes them, instead
+ * of or beside y.  h may be x or res itself (in place). */
+int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldres, int type, const float *w, long long rows,
+                    long long cols, double eps, void *y, long long ldy, uint8_t *q, long long ldq, void *qs, long long ldqs, int scale_type,
+                    void *h, long long ldh, float *rstd, void *stream);
+/* dx = rstd * (dy * w - h * rstd^2 * mean(dy * w * h)) + dh (dh: the gradient that arrives at h, NULL: none), dw = sum over rows of
+ * dy * h * rstd (dx or dw may be NULL).  dx is the gradient of x and of res alike.  workspace:
+ * aq_rms_norm_bwd_workspace_bytes(rows, cols) bytes, 16-byte aligned. */
+size_t aq_rms_norm_bwd_workspace_bytes(long long rows, long long cols);
+int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long lddh, const void *h, long long ldh, int type, const float *w,
+                    const float *rstd, long long rows, long long cols, void *dx, long long lddx, float *dw, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+/* ---- global gradient norm and clipping ---------------------------------------------------------------------------------
+ * norm[0] = sqrt(sum of g^2 over all tensors), summed in double.  outs != NULL: outs[i] = g[i] * min(1, max_norm / (norm + 1e-6))
+ * (outs[i] may be tensors[i]: in place, and then nothing is written when nothing is clipped).  A NaN in any tensor makes the
+ * norm and all outs NaN; an infinity makes the norm infinite and the finite elements zero.  types[i]: AQ_F32, AQ_BF16 or AQ_F16.
+ * workspace: aq_clip_grad_norm_workspace_bytes(sizes, n) bytes, 8-byte aligned. */
+size_t aq_clip_grad_norm_workspace_bytes(const long long *sizes, int n);
+int aq_clip_grad_norm(const void *const *tensors, void *const *outs, const long long *sizes, const int *types, int n, double max_norm,
+                      float *norm, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("AQ_HIP_LIB", os.path.join(_HERE, "lib", "libaq_hip.so"))  # override: development builds
-ABI_VERSION = 13
+ABI_VERSION = 14
 FLAG_EXACT = 1
 BN_RELU, BN_EVAL = 1, 2
 MAX_LEVELS = 128
@@ -29,8 +29,12 @@ EXPORTS = (
     "aq_bn_relu_bwd_shortcut", "aq_bn_relu_fwd_shortcut", "aq_conv_dgrad_add", "aq_synth_fwd_static",
     "aq_tern_workspace_bytes", "aq_tern_fwd", "aq_tern_bwd", "aq_inq_partition", "aq_tern_bwd_adam", "aq_inq_effective", "aq_inq_effective_sumsq", "aq_bn_add_relu_fwd", "aq_bn_add_relu_bwd",
     "aq_pkt_workspace_bytes", "aq_pkt_loss", "aq_pkt_kernel_matrix", "aq_maxpool3s2_fwd", "aq_maxpool3s2_bwd",
+    "aq_fp8_quantize_workspace_bytes", "aq_fp8_quantize", "aq_fp8_transpose", "aq_fp8_dequantize", "aq_fp8_matmul_workspace_bytes", "aq_fp8_matmul",
+    "aq_rms_norm_fwd", "aq_rms_norm_bwd_workspace_bytes", "aq_rms_norm_bwd", "aq_clip_grad_norm_workspace_bytes", "aq_clip_grad_norm",
 )
 TERN_TWN, TERN_TTQ, TERN_INQ = 0, 1, 2
+SCALE_POW2, SCALE_F32 = 0, 1
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class AqSeg(C.Structure):
@@ -172,6 +176,24 @@ def lib():
         L.aq_bn_add_relu_fwd.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, f, f, vp, vp, vp, vp, vp, sz, vp, vp]
         L.aq_bn_add_relu_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, i, vp, vp, vp, vp, vp, sz, vp]
         L.aq_bn_add_relu_fwd.restype = L.aq_bn_add_relu_bwd.restype = i
+        ll = C.c_longlong
+        L.aq_fp8_quantize_workspace_bytes.argtypes = [ll, ll]
+        L.aq_fp8_quantize.argtypes = [vp, i, ll, ll, ll, vp, ll, vp, ll, vp, ll, vp, ll, i, i, vp, vp, sz, vp]
+        L.aq_fp8_transpose.argtypes = [vp, ll, vp, ll, ll, ll, vp, ll, vp, ll, i, i, vp]
+        L.aq_fp8_dequantize.argtypes = [vp, ll, vp, ll, ll, ll, i, i, vp, i, ll, vp]
+        L.aq_fp8_matmul_workspace_bytes.argtypes = [ll, ll, ll]
+        L.aq_fp8_matmul.argtypes = [vp, ll, vp, ll, i, vp, ll, vp, ll, i, ll, ll, ll, i, vp, vp, i, ll, vp, sz, vp]
+        L.aq_rms_norm_fwd.argtypes = [vp, ll, vp, ll, i, vp, ll, ll, C.c_double, vp, ll, vp, ll, vp, ll, i, vp, ll, vp, vp]
+        L.aq_rms_norm_bwd_workspace_bytes.argtypes = [ll, ll]
+        L.aq_rms_norm_bwd.argtypes = [vp, ll, vp, ll, vp, ll, i, vp, vp, ll, ll, vp, ll, vp, vp, sz, vp]
+        L.aq_clip_grad_norm_workspace_bytes.argtypes = [C.POINTER(ll), i]
+        L.aq_clip_grad_norm.argtypes = [C.POINTER(vp), C.POINTER(vp), C.POINTER(ll), C.POINTER(i), i, C.c_double, vp, vp, sz, vp]
+        for name in ("aq_fp8_quantize_workspace_bytes", "aq_fp8_matmul_workspace_bytes", "aq_rms_norm_bwd_workspace_bytes",
+                     "aq_clip_grad_norm_workspace_bytes"):
+            getattr(L, name).restype = sz
+        for name in ("aq_fp8_quantize", "aq_fp8_transpose", "aq_fp8_dequantize", "aq_fp8_matmul", "aq_rms_norm_fwd", "aq_rms_norm_bwd",
+                     "aq_clip_grad_norm"):
+            getattr(L, name).restype = i
         if L.aq_abi_version() != ABI_VERSION:
             raise ImportError("libaq_hip.so ABI %d != binding ABI %d: rebuild" % (L.aq_abi_version(), ABI_VERSION))
         _lib = L

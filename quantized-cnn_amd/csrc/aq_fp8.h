@@ -1,0 +1,170 @@
+// Shared pieces of the 8-bit floating point kernels: element types, vector access, the power-of-two block scale.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/aq_hip.h"
+#include "aq_common.h"
+
+namespace aq {
+
+constexpr int FP8_BLK = 128;  // elements along a row that share a scale
+
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+
+struct bf16_el { uint16_t b; };
+struct f16_el { uint16_t b; };
+struct e4m3_el { uint8_t b; };
+
+__device__ inline float to_f32(float v) { return v; }
+__device__ inline float to_f32(bf16_el v) { return __uint_as_float((uint32_t)v.b << 16); }
+__device__ inline float to_f32(f16_el v) { return (float)__builtin_bit_cast(_Float16, v.b); }
+__device__ inline float to_f32(e4m3_el v) { return __builtin_amdgcn_cvt_f32_fp8((int)v.b, 0); }
+template <typename T> __device__ inline T from_f32(float v);
+template <> __device__ inline float from_f32<float>(float v) { return v; }
+template <> __device__ inline bf16_el from_f32<bf16_el>(float v) { return bf16_el{__builtin_bit_cast(uint16_t, (__bf16)v)}; }
+template <> __device__ inline f16_el from_f32<f16_el>(float v) { return f16_el{__builtin_bit_cast(uint16_t, (_Float16)v)}; }
+
+// Eight neighbouring elements, at any address that is a multiple of the element's size: the global memory path takes 16-byte
+// accesses at any address, so rows of odd lengths need no variant of their own.
+typedef f4_t f4_any __attribute__((aligned(4)));
+typedef u4_t u4_any __attribute__((aligned(2)));
+typedef u2_t u2_any __attribute__((aligned(1)));
+__device__ inline void load8(const float *p, float (&v)[8])
+{
+    const f4_t a = *reinterpret_cast<const f4_any *>(p), b = *reinterpret_cast<const f4_any *>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+}
+__device__ inline void load8(const bf16_el *p, float (&v)[8])
+{
+    const u4_t a = *reinterpret_cast<const u4_any *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(a[i] << 16), v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+}
+__device__ inline void load8(const f16_el *p, float (&v)[8])
+{
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    const h8 a = __builtin_bit_cast(h8, (u4_t) * reinterpret_cast<const u4_any *>(p));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+}
+__device__ inline void load8(const e4m3_el *p, float (&v)[8])
+{
+    const u2_t a = *reinterpret_cast<const u2_any *>(p);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)a[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)a[i], true);
+        v[4 * i] = lo[0], v[4 * i + 1] = lo[1], v[4 * i + 2] = hi[0], v[4 * i + 3] = hi[1];
+    }
+}
+__device__ inline void store8(float *p, const float (&v)[8])
+{
+    f4_t a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = v[i], b[i] = v[4 + i];
+    *reinterpret_cast<f4_any *>(p) = a;
+    *reinterpret_cast<f4_any *>(p + 4) = b;
+}
+template <typename T> __device__ inline uint32_t pack2(float a, float b) { return (uint32_t)from_f32<T>(a).b | (uint32_t)from_f32<T>(b).b << 16; }
+template <typename T> __device__ inline void store8(T *p, const float (&v)[8])
+{
+    u4_t a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<u4_any *>(p) = a;
+}
+// the first n (0..8) of eight elements; the others read as zero and are not written
+template <typename T> __device__ inline void load_n(const T *p, int n, float (&v)[8])
+{
+    if (n >= 8) {
+        load8(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) v[i] = to_f32(p[i]);
+}
+template <typename T> __device__ inline void store_n(T *p, int n, const float (&v)[8])
+{
+    if (n >= 8) {
+        store8(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) p[i] = from_f32<T>(v[i]);
+}
+
+// |v| where v is finite, 0 elsewhere
+__device__ inline float finite_abs(float v)
+{
+    const float a = fabsf(v);
+    return a < __builtin_inff() ? a : 0.0f;
+}
+// Exponent e of the block scale 2^e, the smallest with amax <= 448 * 2^e: amax = (1 + f) 2^E, 448 = 1.75 * 2^8, so
+// e = E - 8, one more where 1 + f > 1.75.  At least -126, the smallest whose scale and reciprocal are normal fp32 numbers.
+__device__ inline int scale_exponent(float amax)
+{
+    const uint32_t b = __float_as_uint(amax);
+    if (b == 0) return 0;
+    const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -126 ? -126 : e;
+}
+__device__ inline float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+// four codes from four values that lie within +-448 (or are not finite: NaN)
+__device__ inline uint32_t e4m3x4(float a, float b, float c, float d)
+{
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+__device__ inline u2_t e4m3x8(const float (&v)[8], float inv)
+{
+    u2_t r;
+    r[0] = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    r[1] = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+    return r;
+}
+__device__ inline void store_codes(uint8_t *p, int n, u2_t c)  // the first n (0..8) of eight codes
+{
+    if (n >= 8) {
+        *reinterpret_cast<u2_any *>(p) = c;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) p[i] = (uint8_t)(c[i >> 2] >> 8 * (i & 3));
+}
+__device__ inline void store_scale(void *s, long long i, int e, int scale_f32)
+{
+    if (scale_f32) static_cast<float *>(s)[i] = exp2_int(e);
+    else static_cast<uint8_t *>(s)[i] = (uint8_t)(e + 127);
+}
+// byte b of a power-of-two scale: 2^(b - 127); b = 0 is the subnormal 2^-127, 255 NaN
+__device__ inline float pow2_scale(uint32_t b) { return b == 0 ? 0x1p-127f : b == 255 ? __builtin_nanf("") : __uint_as_float(b << 23); }
+__device__ inline float load_scale(const void *s, long long i, int scale_f32)
+{
+    return scale_f32 ? static_cast<const float *>(s)[i] : pow2_scale(static_cast<const uint8_t *>(s)[i]);
+}
+// max over the 16 lanes of an aligned group of 16
+__device__ inline float max16(float v)
+{
+#pragma unroll
+    for (int m = 8; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
+    return v;
+}
+
+template <typename F> inline int by_type(int type, F f)
+{
+    return type == AQ_F32 ? f((float *)nullptr) : type == AQ_BF16 ? f((bf16_el *)nullptr) : f((f16_el *)nullptr);
+}
+inline bool is_type(int t) { return t == AQ_F32 || t == AQ_BF16 || t == AQ_F16; }
+inline int type_size(int t) { return t == AQ_F32 ? 4 : 2; }
+
+} // namespace aq

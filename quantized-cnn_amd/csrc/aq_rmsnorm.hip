@@ -1,0 +1,380 @@
+// Root-mean-square norm over the rows of a matrix, with the residual's addition in front and, where it is wanted, e4m3 codes
+// with a scale per 1 x 128 block behind; and its gradients.
+//   h = round(x + res);  rstd = 1 / sqrt(mean(h^2) + eps);  y = (h * rstd) * w
+//   n = h * rstd, g = dy * w:  dx = rstd * (g - n * mean(g * n)) + dh,  dw = sum over rows of dy * n
+// The squares are summed in double: rstd is then the correctly rounded one whatever the order of the sum, and codes next to
+// a rounding border do not depend on the launch's shape.  One pass: a row stays in the registers of its workgroup between the
+// statistics and the outputs, so the traffic is what the operands hold and the kernels are bound by memory bandwidth.
+#include <algorithm>
+
+#include "aq_fp8.h"
+
+namespace aq {
+
+template <typename S> __device__ inline S wave_sum(S v)
+{
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+// sum over the workgroup, the same value in every thread; sh: one element per wavefront, free to be used again on return
+template <int THREADS, typename S> __device__ inline S group_sum(S v, S *sh)
+{
+    v = wave_sum(v);
+    if (THREADS == 64) return v;
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    S s = sh[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; ++i) s += sh[i];
+    __syncthreads();
+    return s;
+}
+
+struct NormArgs {
+    const void *x, *res;
+    const float *w;
+    void *y, *h, *qs;
+    uint8_t *q;
+    float *rstd;
+    long long ldx, ldres, ldy, ldh, ldq, ldqs, rows, cols;
+    double eps;
+    int scale_f32;
+};
+
+template <typename T> __device__ inline void norm_outputs(const NormArgs &a, long long r, long long c, int n, const float (&hv)[8], float rs)
+{
+    float wv[8], o[8];
+    load_n(a.w + c, n, wv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (hv[j] * rs) * wv[j];
+    if (a.y) store_n(static_cast<T *>(a.y) + r * a.ldy + c, n, o);
+    if (a.q) {
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(o[j]));
+        const int e = scale_exponent(max16(m));  // 16 lanes with 8 elements each: one block
+        store_codes(a.q + r * a.ldq + c, n, e4m3x8(o, exp2_int(-e)));
+        if ((threadIdx.x & 15) == 0 && n > 0) store_scale(a.qs, r * a.ldqs + c / FP8_BLK, e, a.scale_f32);
+    }
+}
+
+// one workgroup per row; a thread holds V chunks of 8 columns
+template <typename T, int THREADS, int V>
+__global__ __launch_bounds__(THREADS) void rms_norm_fwd_kernel(const NormArgs a)
+{
+    __shared__ double sh[THREADS / 64];
+    const long long r = blockIdx.x;
+    const T *x = static_cast<const T *>(a.x) + r * a.ldx, *res = static_cast<const T *>(a.res) + r * a.ldres;
+    float hv[V][8];
+    double s = 0.0;
+    const bool whole = a.cols == THREADS * V * 8;  // the same in all lanes: all loads in flight at once
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) load8(x + (i * THREADS + threadIdx.x) * 8, hv[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (i * THREADS + threadIdx.x) * 8;
+            load_n(x + c, (int)min(8LL, a.cols - c), hv[i]);
+        }
+    }
+    if (a.res) {
+        float rv[V][8];
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) load8(res + (i * THREADS + threadIdx.x) * 8, rv[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = (i * THREADS + threadIdx.x) * 8;
+                load_n(res + c, (int)min(8LL, a.cols - c), rv[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) hv[i][j] = to_f32(from_f32<T>(hv[i][j] + rv[i][j]));
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = (i * THREADS + threadIdx.x) * 8;
+        if (a.h) store_n(static_cast<T *>(a.h) + r * a.ldh + c, (int)min(8LL, a.cols - c), hv[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = __builtin_fma((double)hv[i][j], (double)hv[i][j], s);
+    }
+    const float rs = (float)(1.0 / sqrt(group_sum<THREADS>(s, sh) / (double)a.cols + a.eps));
+    if (a.rstd && threadIdx.x == 0) a.rstd[r] = rs;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = (i * THREADS + threadIdx.x) * 8;
+        norm_outputs<T>(a, r, c, (int)max(0LL, min(8LL, a.cols - c)), hv[i], rs);
+    }
+}
+
+// rows too long for the registers: read twice
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_fwd_long_kernel(const NormArgs a)
+{
+    __shared__ double sh[16];
+    const long long r = blockIdx.x;
+    const T *x = static_cast<const T *>(a.x) + r * a.ldx, *res = static_cast<const T *>(a.res) + r * a.ldres;
+    T *h = static_cast<T *>(a.h) + r * a.ldh;
+    const long long chunks = (a.cols + 1023 * 8 + 7) / (1024 * 8);
+    double s = 0.0;
+    auto row_chunk = [&](long long c, int n, float(&hv)[8]) {
+        load_n(x + c, n, hv);
+        if (!a.res) return;
+        float rv[8];
+        load_n(res + c, n, rv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) hv[j] = to_f32(from_f32<T>(hv[j] + rv[j]));
+    };
+    for (long long i = 0; i < chunks; ++i) {
+        const long long c = (i * 1024 + threadIdx.x) * 8;
+        const int n = (int)max(0LL, min(8LL, a.cols - c));
+        float hv[8];
+        row_chunk(c, n, hv);
+        if (a.h) store_n(h + c, n, hv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = __builtin_fma((double)hv[j], (double)hv[j], s);
+    }
+    const float rs = (float)(1.0 / sqrt(group_sum<1024>(s, sh) / (double)a.cols + a.eps));
+    if (a.rstd && threadIdx.x == 0) a.rstd[r] = rs;
+    for (long long i = 0; i < chunks; ++i) {
+        const long long c = (i * 1024 + threadIdx.x) * 8;
+        const int n = (int)max(0LL, min(8LL, a.cols - c));
+        float hv[8];
+        if (a.h) load_n(static_cast<const T *>(h) + c, n, hv);  // (its own store: h may be x or res itself)
+        else row_chunk(c, n, hv);
+        norm_outputs<T>(a, r, c, n, hv, rs);
+    }
+}
+
+struct NormBwdArgs {
+    const void *dy, *dh, *h;
+    const float *w, *rstd;
+    void *dx;
+    float *part;  // [grid, cols] partial dw (NULL: not wanted)
+    long long lddy, lddh, ldh, lddx, rows, cols;
+};
+
+// A fixed number of workgroups, each over every gridDim.x-th row: the columns' partial dw stay in registers from row to row.
+template <typename T, int THREADS, int V>
+__global__ __launch_bounds__(THREADS) void rms_norm_bwd_kernel(const NormBwdArgs a)
+{
+    __shared__ float sh[THREADS / 64];
+    const bool whole = a.cols == THREADS * V * 8;
+    float wv[V][8], acc[V][8];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = (i * THREADS + threadIdx.x) * 8;
+        load_n(a.w + c, (int)max(0LL, min(8LL, a.cols - c)), wv[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
+    }
+    const float inv = 1.0f / (float)a.cols;
+    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *dy = static_cast<const T *>(a.dy) + r * a.lddy, *h = static_cast<const T *>(a.h) + r * a.ldh;
+        const T *dh = static_cast<const T *>(a.dh) + r * a.lddh;
+        const float rs = a.rstd[r];
+        float g[V][8], n[V][8];
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) load8(dy + (i * THREADS + threadIdx.x) * 8, g[i]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) load8(h + (i * THREADS + threadIdx.x) * 8, n[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = (i * THREADS + threadIdx.x) * 8, k = (int)max(0LL, min(8LL, a.cols - c));
+                load_n(dy + c, k, g[i]);
+                load_n(h + c, k, n[i]);
+            }
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                n[i][j] *= rs;
+                acc[i][j] = __builtin_fmaf(g[i][j], n[i][j], acc[i][j]);
+                g[i][j] *= wv[i][j];
+                s = __builtin_fmaf(g[i][j], n[i][j], s);
+            }
+        if (!a.dx) continue;
+        const float m = group_sum<THREADS>(s, sh) * inv;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (i * THREADS + threadIdx.x) * 8, k = (int)max(0LL, min(8LL, a.cols - c));
+            float o[8];
+            if (a.dh) load_n(dh + c, k, o);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = rs * __builtin_fmaf(-n[i][j], m, g[i][j]);
+                o[j] = a.dh ? d + o[j] : d;
+            }
+            store_n(static_cast<T *>(a.dx) + r * a.lddx + c, k, o);
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int c = (i * THREADS + threadIdx.x) * 8;
+        store_n(a.part + (long long)blockIdx.x * a.cols + c, (int)max(0LL, min(8LL, a.cols - c)), acc[i]);
+    }
+}
+
+// rows too long for the registers: dx reads its row twice, dw is a sum over a slice of rows for 256 columns a workgroup
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_dx_long_kernel(const NormBwdArgs a)
+{
+    __shared__ float sh[16];
+    const long long r = blockIdx.x;
+    const T *dy = static_cast<const T *>(a.dy) + r * a.lddy, *h = static_cast<const T *>(a.h) + r * a.ldh;
+    const T *dh = static_cast<const T *>(a.dh) + r * a.lddh;
+    const float rs = a.rstd[r];
+    float s = 0.0f;
+    for (long long c = threadIdx.x; c < a.cols; c += 1024) s = __builtin_fmaf(to_f32(dy[c]) * a.w[c], to_f32(h[c]) * rs, s);
+    const float m = group_sum<1024>(s, sh) / (float)a.cols;
+    for (long long c = threadIdx.x; c < a.cols; c += 1024) {
+        const float d = rs * __builtin_fmaf(-to_f32(h[c]) * rs, m, to_f32(dy[c]) * a.w[c]);
+        static_cast<T *>(a.dx)[r * a.lddx + c] = from_f32<T>(a.dh ? d + to_f32(dh[c]) : d);
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void rms_norm_dw_long_kernel(const NormBwdArgs a, int slices)
+{
+    const long long c = (long long)(blockIdx.x / slices) * 256 + threadIdx.x;
+    const int slice = blockIdx.x % slices;
+    if (c >= a.cols) return;
+    float s = 0.0f;
+    for (long long r = slice; r < a.rows; r += slices)
+        s = __builtin_fmaf(to_f32(static_cast<const T *>(a.dy)[r * a.lddy + c]), to_f32(static_cast<const T *>(a.h)[r * a.ldh + c]) * a.rstd[r], s);
+    a.part[(long long)slice * a.cols + c] = s;
+}
+
+// dw: 64 columns and 16 runs of the partial rows a workgroup, summed in double in a fixed order
+__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float *__restrict__ part, int n, long long cols, float *__restrict__ dw)
+{
+    __shared__ double sh[16][64];
+    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
+    const long long c = (long long)blockIdx.x * 64 + lane;
+    double s = 0.0;
+    if (c < cols) {
+#pragma unroll 4
+        for (int i = run; i < n; i += 16) s += (double)part[i * cols + c];
+    }
+    sh[run][lane] = s;
+    __syncthreads();
+    if (run || c >= cols) return;
+    for (int i = 1; i < 16; ++i) s += sh[i][lane];
+    dw[c] = (float)s;
+}
+
+constexpr long long NORM_LONG = 1024 * 4 * 8;  // columns that fit the registers of a workgroup
+// calls f(threads, chunks per thread) with the smallest shape that holds a row
+template <typename F> inline void norm_shape(long long cols, F f)
+{
+    using std::integral_constant;
+    if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    else if (cols <= 1024) f(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+    else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    else if (cols <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    else if (cols <= 16384) f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+    else f(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+}
+constexpr long long NORM_BWD_LONG = 1024 * 2 * 8;
+// the backward kernel holds four arrays of a row, so more threads with fewer chunks each
+template <typename F> inline void norm_bwd_shape(long long cols, F f)
+{
+    using std::integral_constant;
+    if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    else if (cols <= 1024) f(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+    else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    else if (cols <= 4096) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+    else if (cols <= 8192) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+    else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+}
+// workgroups of the backward kernel (= rows of partial dw)
+static int norm_parts(long long rows, long long cols) { return (int)std::min<long long>(rows, cols > NORM_BWD_LONG ? 64 : cols <= 1024 ? 2048 : 512); }
+
+} // namespace aq
+
+extern "C" {
+
+int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldres, int type, const float *w, long long rows,
+                    long long cols, double eps, void *y, long long ldy, uint8_t *q, long long ldq, void *qs, long long ldqs, int scale_type,
+                    void *h, long long ldh, float *rstd, void *stream)
+{
+    using namespace aq;
+    AQ_REQUIRE(type == AQ_F32 || type == AQ_BF16 || type == AQ_F16, -EINVAL, "aq_rms_norm_fwd: unknown element type %d", type);
+    AQ_REQUIRE(scale_type == AQ_SCALE_POW2 || scale_type == AQ_SCALE_F32, -EINVAL, "aq_rms_norm_fwd: unknown scale type %d", scale_type);
+    AQ_REQUIRE(rows >= 0 && rows < (1LL << 22) && cols >= 1 && cols < (1LL << 31) - 16384, -EINVAL, "aq_rms_norm_fwd: bad sizes %lld x %lld", rows, cols);
+    AQ_REQUIRE(eps >= 0, -EDOM, "aq_rms_norm_fwd: eps=%g is negative", eps);
+    if (rows == 0) return 0;
+    AQ_REQUIRE(x && w && (y || q || h || rstd) && (!q || qs), -EFAULT, "aq_rms_norm_fwd: NULL pointer");
+    AQ_REQUIRE(ldx >= cols && (!res || ldres >= cols) && (!y || ldy >= cols) && (!q || (ldq >= cols && ldqs >= (cols + FP8_BLK - 1) / FP8_BLK)) &&
+                   (!h || ldh >= cols), -EINVAL, "aq_rms_norm_fwd: a pitch is smaller than its row");
+    const NormArgs a = {x, res, w, y, h, qs, q, rstd, ldx, ldres, ldy, ldh, ldq, ldqs, rows, cols, eps, scale_type == AQ_SCALE_F32};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    by_type(type, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (cols > NORM_LONG) {
+            hipLaunchKernelGGL((rms_norm_fwd_long_kernel<T>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+            return 0;
+        }
+        norm_shape(cols, [&](auto threads, auto v) {
+            hipLaunchKernelGGL((rms_norm_fwd_kernel<T, decltype(threads)::value, decltype(v)::value>), dim3((unsigned)rows), dim3(decltype(threads)::value), 0, st, a);
+        });
+        return 0;
+    });
+    return check_launch("aq_rms_norm_fwd");
+}
+
+size_t aq_rms_norm_bwd_workspace_bytes(long long rows, long long cols)
+{
+    return rows > 0 && cols > 0 ? (size_t)aq::norm_parts(rows, cols) * (size_t)cols * sizeof(float) : 0;
+}
+
+int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long lddh, const void *h, long long ldh, int type, const float *w,
+                    const float *rstd, long long rows, long long cols, void *dx, long long lddx, float *dw, void *workspace,
+                    size_t workspace_bytes, void *stream)
+{
+    using namespace aq;
+    AQ_REQUIRE(type == AQ_F32 || type == AQ_BF16 || type == AQ_F16, -EINVAL, "aq_rms_norm_bwd: unknown element type %d", type);
+    AQ_REQUIRE(rows >= 0 && rows < (1LL << 22) && cols >= 1 && cols < (1LL << 31) - 16384, -EINVAL, "aq_rms_norm_bwd: bad sizes %lld x %lld", rows, cols);
+    AQ_REQUIRE(dx || dw, -EINVAL, "aq_rms_norm_bwd: no output is wanted");
+    AQ_REQUIRE(rows == 0 || (dy && h && w && rstd), -EFAULT, "aq_rms_norm_bwd: NULL pointer");
+    AQ_REQUIRE(rows == 0 || (lddy >= cols && ldh >= cols && (!dh || lddh >= cols) && (!dx || lddx >= cols)), -EINVAL,
+               "aq_rms_norm_bwd: a pitch is smaller than its row");
+    const int parts = norm_parts(rows, cols);
+    if (dw && rows) {
+        const size_t need = aq_rms_norm_bwd_workspace_bytes(rows, cols);
+        AQ_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, -ENOSPC,
+                   "aq_rms_norm_bwd: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
+    }
+    const NormBwdArgs a = {dy, dh, h, w, rstd, dx, dw ? static_cast<float *>(workspace) : nullptr, lddy, lddh, ldh, lddx, rows, cols};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (rows > 0) {
+        by_type(type, [&](auto *t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            if (cols > NORM_BWD_LONG) {
+                if (dx) hipLaunchKernelGGL((rms_norm_dx_long_kernel<T>), dim3((unsigned)rows), dim3(1024), 0, st, a);
+                if (dw) hipLaunchKernelGGL((rms_norm_dw_long_kernel<T>), dim3((unsigned)((cols + 255) / 256 * parts)), dim3(256), 0, st, a, parts);
+                return 0;
+            }
+            norm_bwd_shape(cols, [&](auto threads, auto v) {
+                hipLaunchKernelGGL((rms_norm_bwd_kernel<T, decltype(threads)::value, decltype(v)::value>), dim3((unsigned)parts),
+                                   dim3(decltype(threads)::value), 0, st, a);
+            });
+            return 0;
+        });
+        if (int rc = check_launch("aq_rms_norm_bwd")) return rc;
+    }
+    if (dw) hipLaunchKernelGGL(rms_norm_dw_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, a.part, parts, cols, dw);
+    return check_launch("aq_rms_norm_bwd");
+}
+
+} // extern "C"

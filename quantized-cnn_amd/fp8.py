@@ -1,0 +1,197 @@
+"""Linear layers and row norms in 8-bit floating point: e4m3 codes with a power-of-two scale per block of 128.
+
+    y = fp8.linear(x, weight, bias)                              # weight (in, out) as in MyLinear, fp32 / bf16 / fp16
+    y, h = fp8.norm_linear(x, norm_weight, weight, bias, residual=r)   # RMS norm of x + r, its codes straight into the product
+    layer = fp8.Fp8Linear(512, 1000); norm = fp8.RMSNorm(512)
+    layer.pack()                                                 # serving: the codes of the weights are kept
+
+Forward and both gradients are products of codes (ops.fp8_matmul): activations and gradients in 1 x 128 blocks along the
+product's contraction, weights in 128 x 128 tiles.  The weight gradient of fp32 weights is an fp32 product.  Gradients pass the
+roundings unchanged (straight through).  The reference has no such layer: parity unpinned.
+"""
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+def _flat(t):
+    """(..., n) -> (rows, n), a view where the strides allow it."""
+    return t if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1) else t.reshape(-1, t.shape[-1]).contiguous()
+
+
+def _weight_forms(weight, need_dx):
+    """-> (codes of weight^T for the forward product, codes of weight for the input gradient or None)."""
+    if need_dx:
+        rows, cols = ops.fp8_quantize(weight, forms="both", block_rows=ops.FP8_BLOCK)
+        return cols, rows
+    return ops.fp8_quantize(weight, forms="cols", block_rows=ops.FP8_BLOCK), None
+
+
+def _grad_forms(dy, need_dx, need_dw, need_db):
+    """Codes of dy along its rows and along its columns, and its column sums, from one read; None where not needed."""
+    if need_dw or need_db:
+        got = ops.fp8_quantize(dy, forms="both" if need_dx else "cols", colsum=need_db)
+        got = got if isinstance(got, tuple) else (got,)
+        return got[0] if need_dx else None, got[1 if need_dx else 0], got[-1] if need_db else None
+    return ops.fp8_quantize(dy) if need_dx else None, None, None
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, out_dtype):
+        need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        xq, ctx.xt = ops.fp8_quantize(x, forms="both") if need_dw else (ops.fp8_quantize(x), None)
+        wt, ctx.w = _weight_forms(weight, need_dx)
+        ctx.types = x.dtype, weight.dtype, bias.dtype if bias is not None else None
+        return ops.fp8_matmul(xq, wt, bias=bias.float() if bias is not None else None, out_dtype=out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        xtype, wtype, btype = ctx.types
+        dq, dt, db = _grad_forms(_flat(dy), need_dx, need_dw, need_db)
+        dx = ops.fp8_matmul(dq, ctx.w, out_dtype=xtype) if need_dx else None
+        dw = ops.fp8_matmul(ctx.xt, dt, out_dtype=wtype) if need_dw else None
+        return dx, dw, db.to(btype) if need_db else None, None
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h, rstd = ops.rms_norm_forward(x, weight, residual=residual, eps=eps)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.both = residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, h) if ctx.both else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        if dy is None:  # only h was used
+            return dh, None, dh, None
+        dx, dw = ops.rms_norm_backward(_flat(dy), h, weight, rstd, dh=_flat(dh) if dh is not None else None,
+                                       need_dx=ctx.needs_input_grad[0] or ctx.needs_input_grad[2], need_dweight=ctx.needs_input_grad[1])
+        return dx, dw, dx if ctx.both else None, None
+
+
+class _NormLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, norm_weight, weight, bias, residual, eps, out_dtype):
+        need_dn = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[4]
+        xq, h, rstd = ops.rms_norm_forward(x, norm_weight, residual=residual, eps=eps, quantize=True)
+        wt, ctx.w = _weight_forms(weight, need_dn)
+        ctx.xq = xq if ctx.needs_input_grad[2] else None
+        ctx.types = x.dtype, weight.dtype, bias.dtype if bias is not None else None
+        ctx.both = residual is not None
+        ctx.save_for_backward(h, norm_weight, rstd)
+        ctx.set_materialize_grads(False)
+        y = ops.fp8_matmul(xq, wt, bias=bias.float() if bias is not None else None, out_dtype=out_dtype)
+        return (y, h) if ctx.both else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, norm_weight, rstd = ctx.saved_tensors
+        need_x, need_nw, need_dw, need_db, need_r = ctx.needs_input_grad[:5]
+        if dy is None:
+            return dh, None, None, None, dh if ctx.both else None, None, None
+        need_dn = need_x or need_nw or need_r
+        xtype, wtype, btype = ctx.types
+        dq, dt, db = _grad_forms(_flat(dy), need_dn, need_dw, need_db)
+        dw = ops.fp8_matmul(ops.fp8_transpose(ctx.xq), dt, out_dtype=wtype) if need_dw else None
+        dx = dnw = None
+        if need_dn:
+            dn = ops.fp8_matmul(dq, ctx.w, out_dtype=xtype)
+            dx, dnw = ops.rms_norm_backward(dn, h, norm_weight, rstd, dh=_flat(dh) if dh is not None else None, need_dx=need_x or need_r,
+                                            need_dweight=need_nw)
+        return dx, dnw, dw, db.to(btype) if need_db else None, dx if ctx.both else None, None, None
+
+
+def linear(x, weight, bias=None, out_dtype=None):
+    """x (..., in) @ weight + bias in 8-bit floating point; out_dtype defaults to x's.  weight: (in, out) tensor, quantised in
+    this call, or Fp8Blocks (out, in) made before (no gradient of the weight then, and none of x)."""
+    out_dtype = out_dtype or x.dtype
+    x2 = _flat(x)
+    if isinstance(weight, ops.Fp8Blocks):
+        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+            raise RuntimeError("fp8.linear: packed weights serve without gradients: call it under torch.no_grad(), or with the weight tensor")
+        y = ops.fp8_matmul(ops.fp8_quantize(x2), weight, bias=bias.detach().float() if bias is not None else None, out_dtype=out_dtype)
+    else:
+        if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
+            raise ValueError("fp8.linear: x %s / weight %s: need (..., in) and (in, out)" % (tuple(x.shape), tuple(weight.shape)))
+        y = _Linear.apply(x2, weight, bias, out_dtype)
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (y.shape[1],))
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight over the last axis -> (y, h), or y alone without residual."""
+    out = _RmsNorm.apply(_flat(x), weight, _flat(residual) if residual is not None else None, eps)
+    if residual is None:
+        return out.view(x.shape)
+    return out[0].view(x.shape), out[1].view(x.shape)
+
+
+def norm_linear(x, norm_weight, weight, bias=None, residual=None, eps=1e-6, out_dtype=None):
+    """linear(rms_norm(x, norm_weight, residual), weight, bias) with the norm's output kept as codes only -> (y, h), or y alone
+    without residual."""
+    if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
+        raise ValueError("fp8.norm_linear: x %s / weight %s: need (..., in) and (in, out)" % (tuple(x.shape), tuple(weight.shape)))
+    out = _NormLinear.apply(_flat(x), norm_weight, weight, bias, _flat(residual) if residual is not None else None, eps, out_dtype or x.dtype)
+    y, h = out if residual is not None else (out, None)
+    y = y.view(x.shape[:-1] + (y.shape[1],))
+    return y if residual is None else (y, h.view(x.shape))
+
+
+class Fp8Linear(nn.Module):
+    """Linear layer with weight (in_feature, out_feature) like MyLinear's, computed in 8-bit floating point."""
+
+    def __init__(self, in_feature, out_feature, bias=True):
+        super().__init__()
+        self.weight = nn.Parameter(torch.empty(in_feature, out_feature))
+        bound = 1 / math.sqrt(in_feature)
+        nn.init.uniform_(self.weight, -bound, bound)
+        self.bias = nn.Parameter(torch.empty(out_feature).uniform_(-bound, bound)) if bias else None
+        self._packed = None
+
+    def pack(self):
+        """Quantises the weight once, for serving: forward() under no_grad in eval mode then reads the codes.  They are of the weight as
+        it is now; train(), load_state_dict() and moving the module drop them."""
+        with torch.no_grad():
+            self._packed = ops.fp8_quantize(self.weight, forms="cols", block_rows=ops.FP8_BLOCK)
+        return self
+
+    def train(self, mode=True):
+        if mode:
+            self._packed = None
+        return super().train(mode)
+
+    def _apply(self, fn, *args, **kw):
+        self._packed = None
+        return super()._apply(fn, *args, **kw)
+
+    def _load_from_state_dict(self, *args, **kw):
+        self._packed = None
+        return super()._load_from_state_dict(*args, **kw)
+
+    def forward(self, x):
+        if self._packed is not None and not self.training and not torch.is_grad_enabled():
+            return linear(x, self._packed, self.bias)
+        return linear(x, self.weight, self.bias)
+
+
+class RMSNorm(nn.Module):
+    """y = x / sqrt(mean(x^2) + eps) * weight over the last axis; forward(x, residual) -> (y, x + residual)."""
+
+    def __init__(self, features, eps=1e-6):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(features))
+        self.eps = eps
+
+    def forward(self, x, residual=None):
+        return rms_norm(x, self.weight, residual, self.eps)

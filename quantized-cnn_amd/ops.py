@@ -4,6 +4,7 @@ Every function launches on torch's current HIP stream, allocates its outputs and
 torch's caching allocator (so calls are capturable in a HIP graph), and never synchronises.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -899,3 +900,331 @@ def pkt_kernel_matrix(feat, eps=1e-7):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=feat.device)
     _lib.check(_lib.lib().aq_pkt_kernel_matrix(_lib.ptr(feat, name="feat"), N, D, float(eps), _lib.ptr(K), ws.data_ptr(), nbytes, _lib.stream()))
     return K
+
+
+# ------------------------------------------------------- 8-bit floating point, a scale per block of 128
+
+FP8_BLOCK = 128
+_SCALE_TYPES = {torch.float8_e8m0fnu: _lib.SCALE_POW2, torch.float32: _lib.SCALE_F32}
+
+
+def _on_device(f):
+    """Runs f on the device of its first argument (a tensor, Fp8Blocks, or a list of tensors), whichever is current."""
+    @functools.wraps(f)
+    def call(first, *args, **kw):
+        d = first.device if isinstance(first, (torch.Tensor, Fp8Blocks)) else first[0].device if len(first) else None
+        if d is None or d.type != "cuda" or d.index == torch.cuda.current_device():
+            return f(first, *args, **kw)
+        with torch.cuda.device(d):
+            return f(first, *args, **kw)
+    return call
+
+
+def _hip(t, name, device=None):
+    if not t.is_cuda:
+        raise RuntimeError("%s lives on %s: the quantized layers run on the HIP device only "
+                           "(no CPU path); move the model and its inputs to cuda" % (name, t.device))
+    if device is not None and t.device != device:
+        raise ValueError("%s lives on %s, the first argument on %s" % (name, t.device, device))
+
+
+def _matrix(t, name, device=None, dtype=None, shape=None):
+    """Checks of a 2-D operand whose rows may lie apart; returns its pitch in elements."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError("%s: expected a 2-D tensor" % name)
+    _hip(t, name, device)
+    if t.dtype not in _lib.ELEMENT_TYPES or (dtype is not None and t.dtype != dtype):
+        raise ValueError("%s: dtype %s, expected %s" % (name, t.dtype, dtype or "float32, bfloat16 or float16"))
+    if shape is not None and t.shape != shape:
+        raise ValueError("%s: shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    return _pitch(t, name)
+
+
+def _pitch(t, name):
+    rows, cols = t.shape
+    ld = t.stride(0) if rows > 1 else cols
+    if (cols > 1 and t.stride(1) != 1) or (ld < cols and rows and cols):
+        raise ValueError("%s: strides %s: the elements of a row have to be neighbours, and rows must not overlap" % (name, t.stride()))
+    return max(ld, cols)
+
+
+class Fp8Blocks:
+    """A matrix (rows, cols) of e4m3 codes with a scale per block: value = data * scale.
+
+    data   torch.float8_e4m3fn (rows, cols), the codes of a row neighbours in memory
+    scale  (ceil(rows / block_rows), ceil(cols / 128)): torch.float8_e8m0fnu (powers of two) or torch.float32 (any value)
+    block_rows  1: blocks of 1 x 128; 128: tiles of 128 x 128
+    Made by `fp8_quantize`, or from codes and scales of other origin.  `fp8_matmul` reads 16 bytes at a time: where the rows do not
+    start at multiples of 16 bytes, or the last one ends within such a piece at the end of its storage, it first copies the
+    codes (those of `fp8_quantize` never need it)."""
+
+    __slots__ = ("data", "scale", "block_rows", "shape", "device", "_ld", "_lds", "_scale_type")
+
+    def __init__(self, data, scale, block_rows=1):
+        if not isinstance(data, torch.Tensor) or not isinstance(scale, torch.Tensor) or data.dim() != 2 or scale.dim() != 2:
+            raise ValueError("Fp8Blocks: data and scale have to be 2-D tensors")
+        _hip(data, "data")
+        _hip(scale, "scale", data.device)
+        if data.dtype != torch.float8_e4m3fn or scale.dtype not in _SCALE_TYPES:
+            raise ValueError("Fp8Blocks: data %s / scale %s, expected float8_e4m3fn and float8_e8m0fnu or float32" % (data.dtype, scale.dtype))
+        if block_rows not in (1, FP8_BLOCK):
+            raise ValueError("Fp8Blocks: block_rows %r, expected 1 or %d" % (block_rows, FP8_BLOCK))
+        rows, cols = data.shape
+        if scale.shape != (-(-rows // block_rows), -(-cols // FP8_BLOCK)):
+            raise ValueError("Fp8Blocks: scale %s does not belong to data %s in blocks of %d x %d" % (
+                tuple(scale.shape), (rows, cols), block_rows, FP8_BLOCK))
+        self.data, self.scale, self.block_rows, self.shape, self.device = data, scale, block_rows, (rows, cols), data.device
+        self._ld, self._lds = _pitch(data, "data"), _pitch(scale, "scale")
+        self._scale_type = _SCALE_TYPES[scale.dtype]
+
+    def _by16(self):
+        """Codes whose rows can be read 16 bytes at a time up to their last: (tensor to keep alive, address, pitch)."""
+        d, cols = self.data, self.shape[1]
+        p = d.data_ptr()
+        if self._ld % 16 == 0 and p % 16 == 0 and (cols % 16 == 0 or d.storage_offset() + (self.shape[0] - 1) * self._ld + _up(cols, 16)
+                                                   <= d.untyped_storage().nbytes()):
+            return d, p, self._ld
+        c = torch.empty((self.shape[0], _up(cols, 16)), dtype=torch.float8_e4m3fn, device=self.device)
+        c[:, :cols].copy_(d)
+        return c, c.data_ptr(), c.shape[1]
+
+
+def _up(n, m):
+    return (n + m - 1) // m * m
+
+
+def _new_blocks(rows, cols, block_rows, scale_dtype, device):
+    """Uninitialised storage: rows of codes start at multiples of 16 bytes, rows of scales at multiples of 4 elements."""
+    b = Fp8Blocks.__new__(Fp8Blocks)
+    ld, nb = _up(cols, 16), -(-cols // FP8_BLOCK)
+    lds = _up(nb, 4)
+    b.data = torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)
+    if ld != cols:
+        b.data = b.data[:, :cols]
+    b.scale = torch.empty((rows if block_rows == 1 else -(-rows // block_rows), lds), dtype=scale_dtype, device=device)
+    if lds != nb:
+        b.scale = b.scale[:, :nb]
+    b.block_rows, b.shape, b.device, b._ld, b._lds, b._scale_type = block_rows, (rows, cols), device, ld, lds, _SCALE_TYPES[scale_dtype]
+    return b
+
+
+def _stream_of(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _scale_dtype(scale_dtype):
+    if scale_dtype not in _SCALE_TYPES:
+        raise ValueError("scale_dtype %s, expected float8_e8m0fnu or float32" % (scale_dtype,))
+    return _SCALE_TYPES[scale_dtype]
+
+
+@_on_device
+def fp8_quantize(x, forms="rows", block_rows=1, scale_dtype=torch.float8_e8m0fnu, colsum=False):
+    """x (rows, cols), fp32 / bf16 / fp16 -> Fp8Blocks: per block the smallest power of two that brings its largest finite
+    magnitude to 448 or less, codes rounded to nearest even; NaN and infinities become NaN codes.
+    forms: "rows" x itself, "cols" its transpose (cols, rows) in blocks along the transpose's rows, "both" the pair, from one
+    read of x.  colsum=True ("cols" or "both", block_rows=1) appends the fp32 sums of x over its rows (a bias gradient)."""
+    ldx = _matrix(x, "x")
+    st = _scale_dtype(scale_dtype)
+    if forms not in ("rows", "cols", "both"):
+        raise ValueError("fp8_quantize: forms %r, expected rows, cols or both" % (forms,))
+    if block_rows not in (1, FP8_BLOCK):
+        raise ValueError("fp8_quantize: block_rows %r, expected 1 or %d" % (block_rows, FP8_BLOCK))
+    if colsum and (forms == "rows" or block_rows != 1):
+        raise ValueError("fp8_quantize: column sums come with the transposed form in 1 x 128 blocks only")
+    rows, cols = x.shape
+    dev = x.device
+    q = _new_blocks(rows, cols, block_rows, scale_dtype, dev) if forms != "cols" else None
+    qt = _new_blocks(cols, rows, block_rows, scale_dtype, dev) if forms != "rows" else None
+    sums = ws = None
+    nbytes = 0
+    if colsum:
+        sums = torch.empty(cols, dtype=torch.float32, device=dev)
+        nbytes = _lib.lib().aq_fp8_quantize_workspace_bytes(rows, cols)
+        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    if cols and (rows or colsum):
+        _lib.check(_lib.lib().aq_fp8_quantize(
+            x.data_ptr(), _lib.ELEMENT_TYPES[x.dtype], rows, cols, ldx,
+            q.data.data_ptr() if q else None, q._ld if q else 0, q.scale.data_ptr() if q else None, q._lds if q else 0,
+            qt.data.data_ptr() if qt else None, qt._ld if qt else 0, qt.scale.data_ptr() if qt else None, qt._lds if qt else 0,
+            block_rows, st, sums.data_ptr() if colsum else None, ws.data_ptr() if colsum else None, nbytes, _stream_of(dev)))
+    out = (q,) if forms == "rows" else (qt,) if forms == "cols" else (q, qt)
+    if colsum:
+        out += (sums,)
+    return out[0] if len(out) == 1 else out
+
+
+@_on_device
+def fp8_transpose(q):
+    """Fp8Blocks of the transposed matrix.  Tiles of 128 x 128 keep their codes; 1 x 128 blocks are formed anew along the other axis
+    (exact but for values below the new block's smallest subnormal step)."""
+    rows, cols = q.shape
+    t = _new_blocks(cols, rows, q.block_rows, q.scale.dtype, q.device)
+    if rows and cols:
+        _lib.check(_lib.lib().aq_fp8_transpose(q.data.data_ptr(), q._ld, q.scale.data_ptr(), q._lds, rows, cols, t.data.data_ptr(), t._ld,
+                                               t.scale.data_ptr(), t._lds, q.block_rows, q._scale_type, _stream_of(q.device)))
+    return t
+
+
+@_on_device
+def fp8_dequantize(q, dtype=torch.bfloat16):
+    """The values of Fp8Blocks as a plain tensor (in bf16 and fp32 exact where the scales are powers of two and the values in range)."""
+    if dtype not in _lib.ELEMENT_TYPES:
+        raise ValueError("fp8_dequantize: dtype %s, expected float32, bfloat16 or float16" % (dtype,))
+    rows, cols = q.shape
+    y = torch.empty((rows, cols), dtype=dtype, device=q.device)
+    if rows and cols:
+        _lib.check(_lib.lib().aq_fp8_dequantize(q.data.data_ptr(), q._ld, q.scale.data_ptr(), q._lds, rows, cols, q.block_rows, q._scale_type,
+                                                y.data_ptr(), _lib.ELEMENT_TYPES[dtype], cols, _stream_of(q.device)))
+    return y
+
+
+@_on_device
+def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
+    """a (M, K) @ b (N, K)^T + bias (N,) of two Fp8Blocks with scales of one type -> (M, N).  fp32 outputs keep fp32 sums; bf16 and
+    fp16 outputs run on the 8-bit matrix instructions (error of a sum up to 2^-13 of the sum of its terms' magnitudes)."""
+    if not isinstance(a, Fp8Blocks) or not isinstance(b, Fp8Blocks):
+        raise ValueError("fp8_matmul: both operands have to be Fp8Blocks")
+    M, K = a.shape
+    N = b.shape[0]
+    dev = a.device
+    if b.shape[1] != K or b.device != dev or a._scale_type != b._scale_type:
+        raise ValueError("fp8_matmul: a %s with %s scales on %s, b %s with %s scales on %s" % (
+            a.shape, a.scale.dtype, dev, b.shape, b.scale.dtype, b.device))
+    if out_dtype not in _lib.ELEMENT_TYPES:
+        raise ValueError("fp8_matmul: out_dtype %s, expected float32, bfloat16 or float16" % (out_dtype,))
+    if bias is not None:
+        _hip(bias, "bias", dev)
+        if bias.dtype != torch.float32 or bias.shape != (N,) or not bias.is_contiguous():
+            raise ValueError("fp8_matmul: bias has to be a contiguous fp32 vector of %d elements" % N)
+    if K == 0:
+        y = torch.zeros((M, N), dtype=out_dtype, device=dev)
+        return y if bias is None else y + bias.to(out_dtype)
+    y = torch.empty((M, N), dtype=out_dtype, device=dev)
+    if M == 0 or N == 0:
+        return y
+    L = _lib.lib()
+    da, pa, lda = a._by16()
+    db, pb, ldb = b._by16()
+    nbytes = L.aq_fp8_matmul_workspace_bytes(M, N, K)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _lib.check(L.aq_fp8_matmul(pa, lda, a.scale.data_ptr(), a._lds, a.block_rows, pb, ldb, b.scale.data_ptr(), b._lds, b.block_rows, M, N, K,
+                               a._scale_type, bias.data_ptr() if bias is not None else None, y.data_ptr(), _lib.ELEMENT_TYPES[out_dtype], N,
+                               ws.data_ptr() if nbytes else None, nbytes, _stream_of(dev)))
+    return y
+
+
+# --------------------------------------------------------------------------- root-mean-square norm
+
+def _norm_vector(t, n, name, dev):
+    _hip(t, name, dev)
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError("%s has to be a contiguous fp32 vector of %d elements" % (name, n))
+    return t.data_ptr()
+
+
+@_on_device
+def rms_norm_forward(x, weight, residual=None, eps=1e-6, quantize=False, scale_dtype=torch.float8_e8m0fnu):
+    """h = x + residual (rounded to x's type; x itself without residual); y = h / sqrt(mean(h^2) + eps) * weight over the rows of
+    x (rows, cols) -> (y, h, rstd): y of x's type, or Fp8Blocks of it (1 x 128 blocks) with quantize=True; rstd fp32 (rows,)."""
+    ldx = _matrix(x, "x")
+    rows, cols = x.shape
+    dev = x.device
+    if cols == 0:
+        raise ValueError("rms_norm_forward: x %s has no columns" % (tuple(x.shape),))
+    ldr = _matrix(residual, "residual", dev, x.dtype, x.shape) if residual is not None else 0
+    w = _norm_vector(weight, cols, "weight", dev)
+    st = _scale_dtype(scale_dtype)
+    y = _new_blocks(rows, cols, 1, scale_dtype, dev) if quantize else torch.empty((rows, cols), dtype=x.dtype, device=dev)
+    h = torch.empty((rows, cols), dtype=x.dtype, device=dev) if residual is not None else x
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+    if rows:
+        _lib.check(_lib.lib().aq_rms_norm_fwd(
+            x.data_ptr(), ldx, residual.data_ptr() if residual is not None else None, ldr, _lib.ELEMENT_TYPES[x.dtype], w, rows, cols, eps,
+            None if quantize else y.data_ptr(), cols, y.data.data_ptr() if quantize else None, y._ld if quantize else 0,
+            y.scale.data_ptr() if quantize else None, y._lds if quantize else 0, st, h.data_ptr() if residual is not None else None, cols,
+            rstd.data_ptr(), _stream_of(dev)))
+    return y, h, rstd
+
+
+@_on_device
+def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dx=True, need_dweight=True):
+    """Gradients of rms_norm_forward from h and rstd as it returned them: -> (dx, dweight), dx (of h's type) for x and residual
+    alike, dweight fp32; None where not needed.  dh: the gradient that arrives at h by itself (the residual path), added to dx."""
+    ldd = _matrix(dy, "dy")
+    dev = dy.device
+    rows, cols = dy.shape
+    ldh = _matrix(h, "h", dev, dy.dtype, dy.shape)
+    lddh = _matrix(dh, "dh", dev, dy.dtype, dy.shape) if dh is not None else 0
+    if cols == 0:
+        raise ValueError("rms_norm_backward: dy %s has no columns" % (tuple(dy.shape),))
+    w = _norm_vector(weight, cols, "weight", dev)
+    r = _norm_vector(rstd, rows, "rstd", dev)
+    dx = torch.empty((rows, cols), dtype=dy.dtype, device=dev) if need_dx else None
+    dw = torch.empty(cols, dtype=torch.float32, device=dev) if need_dweight else None
+    if not need_dx and not need_dweight:
+        return None, None
+    L = _lib.lib()
+    nbytes = L.aq_rms_norm_bwd_workspace_bytes(rows, cols) if need_dweight else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _lib.check(L.aq_rms_norm_bwd(dy.data_ptr(), ldd, dh.data_ptr() if dh is not None else None, lddh, h.data_ptr(), ldh, _lib.ELEMENT_TYPES[dy.dtype],
+                                 w, r, rows, cols, dx.data_ptr() if need_dx else None, cols, dw.data_ptr() if need_dweight else None,
+                                 ws.data_ptr() if nbytes else None, nbytes, _stream_of(dev)))
+    return dx, dw
+
+
+# ------------------------------------------------------------------- gradient norm over all tensors
+
+def _grad_lists(tensors):
+    dev = tensors[0].device if tensors else None
+    for i, t in enumerate(tensors):
+        if not t.is_cuda:
+            _hip(t, "tensor[%d]" % i)
+        if t.device != dev or t.dtype not in _lib.ELEMENT_TYPES or not t.is_contiguous():
+            raise ValueError("tensor[%d]: %s on %s, strides %s: contiguous float32, bfloat16 or float16 tensors of one device are expected" % (
+                i, t.dtype, t.device, t.stride()))
+    n = len(tensors)
+    return (C.c_void_p * n)(*[t.data_ptr() for t in tensors]), (C.c_longlong * n)(*[t.numel() for t in tensors]), \
+        (C.c_int * n)(*[_lib.ELEMENT_TYPES[t.dtype] for t in tensors]), dev
+
+
+def _grad_norm(tensors, outs, max_norm):
+    ptrs, sizes, types, dev = _grad_lists(tensors)
+    n = len(tensors)
+    L = _lib.lib()
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    nbytes = L.aq_clip_grad_norm_workspace_bytes(sizes, n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _lib.check(L.aq_clip_grad_norm(ptrs, outs, sizes, types, n, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes, _stream_of(dev)))
+    return norm
+
+
+@_on_device
+def grad_norm(tensors):
+    """sqrt(sum of squares of all elements of all tensors), fp32 0-dim device tensor (sums in double)."""
+    if len(tensors) == 0:
+        raise ValueError("grad_norm: the list of tensors is empty")
+    return _grad_norm(tensors, None, 0.0)
+
+
+@_on_device
+def clip_grad_norm(tensors, max_norm, out=None):
+    """Scales all tensors by min(1, max_norm / (norm + 1e-6)), norm = sqrt(sum of squares of all their elements): in place, or into
+    the tensors of `out` (same shapes and types).  -> norm, fp32 0-dim device tensor.  The host does not wait; a NaN makes
+    everything NaN, an infinity makes the finite elements 0.  Two launches per 64 tensors."""
+    if len(tensors) == 0:
+        raise ValueError("clip_grad_norm: the list of tensors is empty")
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError("clip_grad_norm: max_norm %r" % max_norm)
+    seen = {t.data_ptr() for t in tensors if t.numel()}
+    if len(seen) != sum(1 for t in tensors if t.numel()):
+        raise ValueError("clip_grad_norm: a tensor is in the list twice")
+    if out is None:
+        return _grad_norm(tensors, (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors]), max_norm)
+    if len(out) != len(tensors):
+        raise ValueError("clip_grad_norm: %d outputs for %d tensors" % (len(out), len(tensors)))
+    for i, (o, t) in enumerate(zip(out, tensors)):
+        if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or not o.is_contiguous():
+            raise ValueError("clip_grad_norm: out[%d] does not match its tensor" % i)
+    return _grad_norm(tensors, (C.c_void_p * len(out))(*[o.data_ptr() for o in out]), max_norm)

@@ -138,12 +138,27 @@ class DataParallel:
         layers.set_dW_reduce_hook(None)
 
 
+def _clip(opts, max_norm):
+    """Clips the gradients of all parameters of the optimizers by their common norm, on the device -> the norm."""
+    from . import ops
+    return ops.clip_grad_norm([p.grad for o in opts for g in o.param_groups for p in g["params"] if p.grad is not None], max_norm)
+
+
+def _checked_max_norm(max_norm):
+    if max_norm is not None and not max_norm > 0:
+        raise ValueError("max_norm %r: a positive number, or None for no clipping" % (max_norm,))
+    return max_norm
+
+
 class TrainStep:
     """One optimisation step with the reference's order of operations: forward, CrossEntropy +
-    model_loss, backward, optimizer_prim / optimizer_q / optimizer .step(), three zero_grad()."""
+    model_loss, backward, optimizer_prim / optimizer_q / optimizer .step(), three zero_grad().
+    max_norm: the gradients of all parameters together are clipped to this norm before the optimizers' steps (behind the
+    data-parallel exchange, so all ranks scale alike); the norm before clipping is left in `grad_norm`, a device scalar."""
 
-    def __init__(self, model, config, module, dp=None, use_graph=False):
+    def __init__(self, model, config, module, dp=None, use_graph=False, max_norm=None):
         self.model, self.config, self.module, self.dp = model, config, module, dp
+        self.max_norm, self.grad_norm = _checked_max_norm(max_norm), None
         self.criterion = nn.CrossEntropyLoss()
         self.use_graph = use_graph
         self.opts = make_optimizers(model, config, capturable=use_graph)
@@ -157,6 +172,8 @@ class TrainStep:
         loss.backward()
         if self.dp is not None:
             self.dp.reduce_dense()
+        if self.max_norm is not None:
+            self.grad_norm = _clip(self.opts, self.max_norm)
         for o in self.opts:
             o.step()
         return loss, logits
@@ -222,20 +239,25 @@ class CapturedStep:
     (ternary.ResNet, resnet18.ResNet18, single layers); the reference's own step order is TrainStep / FusedTrainStep.
     `warmup` (>= 1) eager steps on the first batch run first (they are real steps: optimizer state is created there), then
     the capture; every call
-    copies (x, y) into the graph's input buffers and replays.  Shapes must stay fixed; SyncBatchNorm is refused."""
+    copies (x, y) into the graph's input buffers and replays.  Shapes must stay fixed; SyncBatchNorm is refused.
+    max_norm: the gradients of all parameters of the optimizers together are clipped to this norm before their steps; the norm
+    before clipping is left in `grad_norm`, a device scalar."""
 
-    def __init__(self, model, optimizers, loss_fn, warmup=2):
+    def __init__(self, model, optimizers, loss_fn, warmup=2, max_norm=None):
         if warmup < 1:  # optimizers create their state (momentum, Adam's averages) in their first step: a capture of THAT
             # step would replay the state's creation, not its update
             raise ValueError("CapturedStep: at least one eager warm-up step is needed before the capture")
         self.model, self.loss_fn, self.warmup = model, loss_fn, warmup
         self.opts = list(optimizers) if isinstance(optimizers, (list, tuple)) else [optimizers]
+        self.max_norm, self.grad_norm = _checked_max_norm(max_norm), None
         self._graph = None
 
     def _body(self):
         out = self.model(self._sx)
         loss = self.loss_fn(out, self._sy)
         loss.backward()
+        if self.max_norm is not None:
+            self.grad_norm = _clip(self.opts, self.max_norm)
         for o in self.opts:
             o.step()
         self.loss, self.output = loss.detach(), out.detach()

@@ -1,0 +1,112 @@
+"""Host side of the 8-bit floating point operators, the row norm and gradient clipping: the checker's own format against
+torch's e4m3 type, refusals of the C ABI before any launch, refusals of the wrappers (no GPU)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp8 as F8
+
+
+def test_oracle_codes_are_those_of_torch():
+    c = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    assert np.array_equal(F8.VALUES, c.double().numpy(), equal_nan=True)
+    rs = np.random.RandomState(0)
+    mids = (F8._POS[1:] + F8._POS[:-1]) / 2
+    x = np.concatenate([mids, np.nextafter(mids, 0), np.nextafter(mids, 1e3), F8._POS, rs.uniform(0, 448, 5000), 2.0 ** rs.uniform(-12, 8.8, 5000)])
+    x = np.concatenate([x, -x]).astype(np.float32)
+    x = x[np.abs(x) <= 448]
+    want = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(F8.encode(x), want)
+
+
+def test_oracle_scale_exponent_borders():
+    for e in (-120, -3, 0, 5, 100):
+        top = 448.0 * 2.0 ** e
+        assert F8.scale_exponent(top) == e and F8.scale_exponent(np.nextafter(top, np.inf)) == e + 1
+    assert F8.scale_exponent(0.0) == 0 and F8.scale_exponent(1e-45) == -126
+
+
+def _rc(name, *args):
+    import quantized_cnn_amd._lib as L
+    rc = getattr(L.lib(), name)(*args)
+    return rc, L.lib().aq_last_error().decode()
+
+
+P = 4096  # an address that no call below reads
+
+
+@pytest.mark.parametrize("args,word", [
+    ((P, 7, 4, 128, 128, P, 128, P, 1, None, 0, None, 0, 1, 0, None, None, 0, None), "element type"),
+    ((P, 0, 4, 128, 128, P, 128, P, 1, None, 0, None, 0, 1, 5, None, None, 0, None), "scale type"),
+    ((P, 0, 4, 128, 128, P, 128, P, 1, None, 0, None, 0, 2, 0, None, None, 0, None), "blocks of 2 rows"),
+    ((P, 0, -1, 128, 128, P, 128, P, 1, None, 0, None, 0, 1, 0, None, None, 0, None), "bad sizes"),
+    ((P, 0, 4, 128, 128, None, 0, None, 0, None, 0, None, 0, 1, 0, None, None, 0, None), "no output"),
+    ((P, 0, 4, 128, 100, P, 128, P, 1, None, 0, None, 0, 1, 0, None, None, 0, None), "pitch"),
+    ((P, 0, 4, 128, 128, P, 128, None, 1, None, 0, None, 0, 1, 0, None, None, 0, None), "NULL"),
+    ((P, 0, 4, 128, 128, P, 128, P, 1, None, 0, None, 0, 1, 0, P, None, 0, None), "column sums"),
+    ((P, 0, 4, 128, 128, None, 0, None, 0, P, 4, P, 1, 1, 0, P, None, 0, None), "workspace"),
+    ((P, 0, 1 << 40, 128, 128, P, 128, P, 1, None, 0, None, 0, 1, 0, None, None, 0, None), "too large"),
+])
+def test_quantize_refusals(args, word):
+    rc, err = _rc("aq_fp8_quantize", *args)
+    assert rc < 0 and word in err, err
+
+
+@pytest.mark.parametrize("change,word", [
+    ({"a_br": 3}, "blocks of 3"), ({"st": 9}, "scale type"), ({"K": 0}, "bad sizes"), ({"M": -2}, "bad sizes"), ({"lda": 24}, "pitch"),
+    ({"lda": 136}, "multiples of 16"), ({"a": P + 8}, "multiples of 16"), ({"yt": 3}, "element type"), ({"ldy": 2}, "pitch"), ({"a": None}, "NULL"),
+    ({"M": 1 << 40}, "too large")])
+def test_matmul_refusals(change, word):
+    v = dict(a=P, lda=128, a_br=1, st=0, M=4, K=128, yt=1, ldy=8)
+    v.update(change)
+    rc, err = _rc("aq_fp8_matmul", v["a"], v["lda"], P, 1, v["a_br"], P, 128, P, 1, 128, v["M"], 8, v["K"], v["st"], None, P, v["yt"], v["ldy"], None, 0, None)
+    assert rc < 0 and word in err, err
+
+
+def test_norm_and_clip_refusals():
+    import ctypes as C
+    rc, err = _rc("aq_rms_norm_fwd", P, 64, None, 0, 3, P, 4, 64, 1e-6, P, 64, None, 0, None, 0, 0, None, 0, P, None)
+    assert rc < 0 and "element type" in err
+    rc, err = _rc("aq_rms_norm_fwd", P, 64, None, 0, 0, P, 4, 0, 1e-6, P, 64, None, 0, None, 0, 0, None, 0, P, None)
+    assert rc < 0 and "bad sizes" in err
+    rc, err = _rc("aq_rms_norm_fwd", P, 64, None, 0, 0, P, 4, 64, -1.0, P, 64, None, 0, None, 0, 0, None, 0, P, None)
+    assert rc < 0 and "eps" in err
+    rc, err = _rc("aq_rms_norm_fwd", P, 63, None, 0, 0, P, 4, 64, 1e-6, P, 64, None, 0, None, 0, 0, None, 0, P, None)
+    assert rc < 0 and "pitch" in err
+    rc, err = _rc("aq_rms_norm_bwd", P, 64, None, 0, P, 64, 0, P, P, 4, 64, None, 0, None, None, 0, None)
+    assert rc < 0 and "no output" in err
+    rc, err = _rc("aq_rms_norm_bwd", P, 64, None, 0, P, 64, 0, P, P, 4, 64, P, 64, P, None, 0, None)
+    assert rc < 0 and "workspace" in err
+    one = lambda t, v: (t * 1)(v)  # noqa: E731
+    p, n, t = one(C.c_void_p, P), one(C.c_longlong, 10), one(C.c_int, 0)
+    rc, err = _rc("aq_clip_grad_norm", p, p, n, t, 1, -1.0, P, P, 64, None)
+    assert rc < 0 and "max_norm" in err
+    rc, err = _rc("aq_clip_grad_norm", p, p, n, one(C.c_int, 9), 1, 1.0, P, P, 64, None)
+    assert rc < 0 and "element type" in err
+    rc, err = _rc("aq_clip_grad_norm", p, p, n, t, 1, 1.0, P, P, 8, None)
+    assert rc < 0 and "workspace" in err
+
+
+def test_cpu_tensors_are_refused_loudly():
+    from quantized_cnn_amd import ops
+    x = torch.randn(4, 256)
+    with pytest.raises(RuntimeError, match="HIP device only"):
+        ops.fp8_quantize(x)
+    with pytest.raises(RuntimeError, match="HIP device only"):
+        ops.Fp8Blocks(x.to(torch.float8_e4m3fn), torch.ones(4, 2))
+    with pytest.raises(RuntimeError, match="HIP device only"):
+        ops.rms_norm_forward(x, torch.ones(256))
+    with pytest.raises(RuntimeError, match="HIP device only"):
+        ops.clip_grad_norm([x], 1.0)
+    with pytest.raises(ValueError, match="empty"):
+        ops.clip_grad_norm([], 1.0)
+    with pytest.raises(ValueError):
+        ops.fp8_matmul(x, x)
+
+
+def test_training_steps_check_max_norm():
+    from quantized_cnn_amd import train
+    m = torch.nn.Linear(2, 2)
+    for bad in (0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            train.CapturedStep(m, torch.optim.SGD(m.parameters(), 0.1), torch.nn.functional.mse_loss, max_norm=bad)

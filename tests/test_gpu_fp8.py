@@ -1,0 +1,722 @@
+"""8-bit floating point kernels (quantiser, scaled product), row norm and gradient clipping against float64 (oracle/fp8.py).
+
+Codes and scales are held to equality: scaling by a power of two is exact, so there is one rounding and it has one result.
+Tolerances of the others, by arithmetic (u = 2^-24, one rounding of an fp32 result; r = eps / 2 of the output's type):
+  product, 16-bit outputs: the matrix instruction aligns the products of 8 neighbouring k to the largest of them, p, and keeps what
+      lies above 2^-13 p: at most 7 terms are cut, each by less than that: 7 * 2^-13 * (sum of the groups' largest products), and K roundings
+      of the running sum (2u each, whichever way they go), then r * |y| for the output.
+  product, fp32 output: products of codes are exact, K additions and three more roundings a block (scales): (K + 4 blocks) * 2u * sum |terms|,
+      and u * |y| with a bias.
+  norm: rstd is the double result rounded once (u), two products (2u), then r: |y| * (3u + r).
+  norm gradients: a chain of at most 32 + 6 + 16 fp32 additions for the mean of g n: 60u * mean|g n|; dx: rstd * (|n| * that + 4u * (|g| + |n m|)), then
+      r * |dx|; with dh one more rounding.  dw: a chain of at most rows / 512 + 1 additions, each term with 3 roundings.
+  clipping: norm u (double sums), factor u, product u, then r."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp8 as F8
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    import quantized_cnn_amd.ops as ops
+    from quantized_cnn_amd import fp8, train
+DEV = "cuda"
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+E8 = torch.float8_e8m0fnu
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def codes_of(q):
+    return q.data.contiguous().view(torch.uint8).cpu().numpy()
+
+
+def exps_of(q):
+    s = q.scale.contiguous()
+    if s.dtype == torch.float32:
+        return np.frexp(s.cpu().numpy().astype(np.float64))[1] - 1
+    return s.view(torch.uint8).cpu().numpy().astype(np.int64) - 127
+
+
+def same_codes(got, want):
+    """Equal, any NaN code for a NaN."""
+    n = (got & 0x7f) == 0x7f
+    assert np.array_equal(n, (want & 0x7f) == 0x7f)
+    assert np.array_equal(got[~n], want[~n])
+
+
+def features(rows, cols, dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(rows, cols, device=DEV, generator=g) * torch.exp(torch.randn(rows, 1, device=DEV, generator=g))
+    x = x * torch.exp(torch.randn(1, cols, device=DEV, generator=g))
+    return x.to(dtype)
+
+
+# -------------------------------------------------------------------------------------- quantiser
+
+SIZES = [(1, 1), (1, 128), (3, 129), (127, 300), (128, 128), (130, 257), (64, 1000), (257, 511), (2, 4096)]
+
+
+@pytest.mark.parametrize("rows,cols", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_rows_and_columns(rows, cols, dtype):
+    x = features(rows, cols, dtype, rows + cols)
+    want, exps = F8.quantize(f64(x))
+    q = ops.fp8_quantize(x)
+    same_codes(codes_of(q), want)
+    assert np.array_equal(exps_of(q), exps)
+    q2, qt, sums = ops.fp8_quantize(x, forms="both", colsum=True)
+    assert np.array_equal(codes_of(q2), codes_of(q)) and np.array_equal(exps_of(q2), exps)
+    wt, et = F8.quantize(f64(x).T)
+    same_codes(codes_of(qt), wt)
+    assert np.array_equal(exps_of(qt), et)
+    exact = f64(x).sum(0)
+    assert np.all(np.abs(f64(sums) - exact) <= U * np.abs(exact) * 1.01 + 1e-12 * np.abs(f64(x)).sum(0) + 2.0 ** -149)
+    only = ops.fp8_quantize(x, forms="cols", scale_dtype=torch.float32)
+    assert np.array_equal(codes_of(only), codes_of(qt)) and np.array_equal(exps_of(only), et)
+    # values
+    for q, c, e in ((q2, want, exps), (qt, wt, et)):
+        v = F8.values(c, 2.0 ** e.astype(np.float64))
+        assert np.array_equal(f64(ops.fp8_dequantize(q, torch.float32)), v)
+        assert np.array_equal(f64(ops.fp8_dequantize(q)), v)  # exact in bf16 too
+
+
+@pytest.mark.parametrize("rows,cols", SIZES)
+def test_quantize_tiles_and_transposes(rows, cols):
+    x = features(rows, cols, torch.float32, 3)
+    want, exps = F8.quantize(f64(x), 128)
+    q, qt = ops.fp8_quantize(x, forms="both", block_rows=128)
+    same_codes(codes_of(q), want)
+    assert np.array_equal(exps_of(q), exps)
+    assert np.array_equal(codes_of(qt), codes_of(q).T) and np.array_equal(exps_of(qt), exps.T)
+    assert np.array_equal(f64(ops.fp8_dequantize(qt)), F8.values(want, 2.0 ** exps.astype(np.float64), 128).T)
+    t = ops.fp8_transpose(q)
+    assert np.array_equal(codes_of(t), codes_of(qt)) and np.array_equal(exps_of(t), exps.T)
+    # 1 x 128 blocks: the values, quantised anew along the other axis
+    r = ops.fp8_quantize(x)
+    t = ops.fp8_transpose(r)
+    c, e = F8.quantize(f64(ops.fp8_dequantize(r, torch.float32)).T)
+    same_codes(codes_of(t), c)
+    assert np.array_equal(exps_of(t), e)
+    # scales of any value travel with the tiles
+    s = torch.rand(q.scale.shape, device=DEV) + 0.5
+    t = ops.fp8_transpose(ops.Fp8Blocks(q.data, s, 128))
+    assert np.array_equal(codes_of(t), codes_of(qt)) and torch.equal(t.scale, s.t())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_special_values(dtype):
+    x = features(6, 400, dtype, 1)
+    x[0, 3], x[0, 200], x[1, 130] = float("nan"), float("inf"), float("-inf")
+    x[2] = 0.0
+    x[3, :128] = float("nan")  # a block with nothing finite
+    x[4, :128] = torch.finfo(dtype).max
+    x[4, 128:256] = torch.finfo(dtype).tiny
+    x[5, :128] = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # the smallest subnormal
+    for form in ("rows", "cols"):
+        for br in (1, 128):
+            q = ops.fp8_quantize(x, forms=form, block_rows=br)
+            want, exps = F8.quantize(f64(x) if form == "rows" else f64(x).T, br)
+            same_codes(codes_of(q), want)
+            assert np.array_equal(exps_of(q), exps)
+
+
+def test_quantize_borders_between_codes_and_scales():
+    mids = (F8._POS[1:] + F8._POS[:-1]) / 2
+    v = np.concatenate([mids, np.nextafter(mids.astype(np.float32), np.float32(0)), np.nextafter(mids.astype(np.float32), np.float32(1e3)), F8._POS])
+    for top in (448.0, np.nextafter(np.float32(448), np.float32(1e3)), 224.0, 447.5, 256.0):
+        rows = []
+        for i in range(0, len(v), 127):
+            part = v[i:i + 127]
+            rows.append(np.concatenate([part, np.zeros(127 - len(part)), [top]]))
+        x = np.array(rows, np.float32)
+        x[:, :127] = np.minimum(x[:, :127], np.float32(top))
+        want, exps = F8.quantize(x)
+        q = ops.fp8_quantize(torch.from_numpy(x).to(DEV))
+        assert np.array_equal(codes_of(q), want) and np.array_equal(exps_of(q), exps)
+
+
+def test_quantize_strides_and_neighbours():
+    big = features(200, 700, torch.bfloat16, 5)
+    x = big[3:140, 5:518]  # rows 1400 bytes apart, starting at an odd place
+    want, exps = F8.quantize(f64(x))
+    q, qt = ops.fp8_quantize(x, forms="both")
+    same_codes(codes_of(q), want)
+    same_codes(codes_of(qt), F8.quantize(f64(x).T)[0])
+    with pytest.raises(ValueError, match="strides"):
+        ops.fp8_quantize(big.t())
+    with pytest.raises(ValueError, match="strides"):
+        ops.fp8_quantize(big[:1].expand(4, 700))
+    # the C entry writes rows x cols codes and no more
+    from quantized_cnn_amd import _lib
+    rows, cols, ld = 5, 131, 160
+    src = features(rows, cols, torch.float32, 6)
+    out = torch.full((rows + 1, ld), 0x55, dtype=torch.uint8, device=DEV)
+    sc = torch.full((rows + 1, 4), 0x55, dtype=torch.uint8, device=DEV)
+    _lib.check(_lib.lib().aq_fp8_quantize(src.data_ptr(), 0, rows, cols, cols, out.data_ptr(), ld, sc.data_ptr(), 4, None, 0, None, 0, 1, 0, None, None, 0,
+                                          _lib.stream()))
+    same_codes(out[:rows, :cols].cpu().numpy(), F8.quantize(f64(src))[0])
+    assert bool((out[:, cols:] == 0x55).all()) and bool((out[rows] == 0x55).all()) and bool((sc[:, 2:] == 0x55).all()) and bool((sc[rows] == 0x55).all())
+
+
+def test_empty_matrices():
+    e = ops.fp8_quantize(torch.empty(0, 256, device=DEV))
+    assert e.shape == (0, 256) and ops.fp8_dequantize(e).shape == (0, 256)
+    w = ops.fp8_quantize(features(40, 256, torch.float32))
+    assert ops.fp8_matmul(e, w).shape == (0, 40) and ops.fp8_matmul(w, e).shape == (40, 0)
+    _, sums = ops.fp8_quantize(torch.empty(0, 256, device=DEV), forms="cols", colsum=True)
+    assert torch.equal(sums, torch.zeros(256, device=DEV))
+    k0 = ops.fp8_quantize(torch.empty(3, 0, device=DEV))
+    assert torch.equal(ops.fp8_matmul(k0, k0), torch.zeros(3, 3, device=DEV, dtype=torch.bfloat16))
+
+
+# ---------------------------------------------------------------------------------------- product
+
+def operand(rows, k, block_rows, pow2, seed, spread=True):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(rows, k, device=DEV, generator=g)
+    if spread:
+        x = x * torch.exp(2 * torch.randn(rows, k, device=DEV, generator=g))
+    q = ops.fp8_quantize(x, block_rows=block_rows, scale_dtype=E8 if pow2 else torch.float32)
+    if not pow2:
+        q = ops.Fp8Blocks(q.data, q.scale * (0.5 + torch.rand(q.scale.shape, device=DEV, generator=g)), block_rows)
+    return q
+
+
+def check_product(a, b, bias, dtype):
+    y = f64(ops.fp8_matmul(a, b, bias=bias, out_dtype=dtype))
+    va = F8.values(codes_of(a), f64(a.scale.float()), a.block_rows)
+    vb = F8.values(codes_of(b), f64(b.scale.float()), b.block_rows)
+    K = va.shape[1]
+    want, mag = va @ vb.T, np.abs(va) @ np.abs(vb).T
+    if bias is not None:
+        want = want + f64(bias)
+        mag = mag + np.abs(f64(bias))
+    if dtype == torch.float32:
+        tol = (K + 4 * -(-K // 128)) * 2 * U * mag + U * np.abs(want)
+    else:
+        pad = -K % 8
+        ga = np.pad(np.abs(va), ((0, 0), (0, pad))).reshape(len(va), -1, 8)
+        gb = np.pad(np.abs(vb), ((0, 0), (0, pad))).reshape(len(vb), -1, 8)
+        top = np.zeros_like(mag)
+        for j in range(ga.shape[1]):
+            top += (ga[:, None, j] * gb[None, :, j]).max(2)
+        tol = 7 * 2.0 ** -13 * top + (K + 4 * -(-K // 128)) * 2 * U * mag
+        tol = tol + half_step(dtype) * (np.abs(want) + tol)
+    # fp16: from 65520 on the nearest fp16 number is the infinity (of the sum's sign)
+    lim = 65520.0 if dtype == torch.float16 else np.inf
+    over = np.abs(want) - tol >= lim
+    assert np.array_equal(y[over], np.copysign(np.inf, want[over]))
+    maybe = (np.abs(want) + tol >= lim) & np.isinf(y) & (np.sign(y) == np.sign(want))
+    ok = over | maybe
+    bad = np.abs(np.where(ok, 0, y) - np.where(ok, 0, want)) > tol
+    assert not bad.any(), (y[bad][:3], want[bad][:3], tol[bad][:3], np.argwhere(bad)[:3])
+    return y
+
+
+PRODUCTS = [(1, 64, 128), (1, 1000, 4096), (2, 16, 16), (3, 17, 1), (5, 130, 200), (16, 128, 1000), (17, 257, 384), (33, 65, 130), (64, 64, 128), (65, 300, 513),
+            (100, 1000, 512), (128, 128, 256), (200, 129, 1040), (257, 511, 640), (300, 300, 2048)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_product(m, n, k, dtype, pow2):
+    a, b = operand(m, k, 1, pow2, m + n), operand(n, k, 128 if (m + n) % 2 else 1, pow2, k + 1)
+    bias = torch.randn(n, device=DEV) if m % 2 else None
+    check_product(a, b, bias, dtype)
+
+
+@pytest.mark.parametrize("pow2", [True, False])
+def test_product_other_forms(pow2):
+    check_product(operand(140, 300, 128, pow2, 1), operand(260, 300, 128, pow2, 2), None, torch.bfloat16)
+    check_product(operand(140, 300, 128, pow2, 1), operand(260, 300, 1, pow2, 2), None, torch.float16)
+    check_product(operand(7, 300, 128, pow2, 1), operand(260, 300, 1, pow2, 2), torch.randn(260, device=DEV), torch.float16)
+
+
+def test_product_of_whole_numbers_is_exact():
+    """Small integers: every partial sum is a whole number below 2^24, so each path has to give the result itself."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    for m, n, k in ((3, 50, 700), (70, 90, 1300), (300, 260, 640)):
+        ai = torch.randint(-4, 5, (m, k), device=DEV, generator=g)
+        bi = torch.randint(-4, 5, (n, k), device=DEV, generator=g)
+        for sdt in (E8, torch.float32):
+            one = lambda r: torch.ones(r, -(-k // 128), device=DEV).to(sdt)  # noqa: E731
+            a, b = ops.Fp8Blocks(ai.float().to(torch.float8_e4m3fn), one(m)), ops.Fp8Blocks(bi.float().to(torch.float8_e4m3fn), one(n))
+            want = (ai.double() @ bi.double().t())
+            assert torch.equal(ops.fp8_matmul(a, b, out_dtype=torch.float32).double(), want)
+            assert torch.equal(ops.fp8_matmul(a, b, out_dtype=torch.float16), want.half())
+            assert torch.equal(ops.fp8_matmul(a, b), want.bfloat16())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [1, 20, 150])
+def test_product_ignores_what_lies_behind_its_rows(m, dtype):
+    """Codes behind K (NaN), rows behind M and N, in operands that are views of larger ones."""
+    k, n = 200, 90
+    full_a = torch.full((m + 2, 256), float("nan"), device=DEV).to(torch.float8_e4m3fn)
+    full_b = torch.full((n + 2, 256), float("nan"), device=DEV).to(torch.float8_e4m3fn)
+    a0, b0 = operand(m, k, 1, True, 1), operand(n, k, 1, True, 2)
+    full_a[:m, :k], full_b[:n, :k] = a0.data, b0.data
+    a, b = ops.Fp8Blocks(full_a[:m, :k], a0.scale), ops.Fp8Blocks(full_b[:n, :k], b0.scale)
+    y = check_product(a, b, None, dtype)
+    assert np.isfinite(y).all()
+    # rows at odd places, and one that ends with its storage
+    odd = torch.zeros(m * 201 + 3, device=DEV).to(torch.float8_e4m3fn)[3:].view(m, 201)[:, :k]
+    odd.copy_(a0.data)
+    assert np.array_equal(check_product(ops.Fp8Blocks(odd, a0.scale), b, None, dtype), y)
+    tight = torch.empty(m * k, device=DEV, dtype=torch.float8_e4m3fn).view(m, k)
+    tight.copy_(a0.data)
+    assert np.array_equal(check_product(ops.Fp8Blocks(tight, a0.scale), b, None, dtype), y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m", [2, 40, 140])
+def test_product_special_values(m, dtype):
+    """A NaN code spoils its row (or column) and nothing else; extreme scales."""
+    a, b = operand(m, 300, 1, True, 1), operand(150, 300, 1, True, 2)
+    clean = ops.fp8_matmul(a, b, out_dtype=dtype)
+    a.data[1, 250] = float("nan")
+    b.data[77, 3] = float("nan")
+    y = ops.fp8_matmul(a, b, out_dtype=dtype)
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[1], bad[:, 77] = True, True
+    assert torch.equal(torch.isnan(y), bad) and torch.equal(y[~bad], clean[~bad])
+    z = operand(m, 300, 1, True, 1)
+    z.scale[0, 1] = 2.0 ** -127
+    z.scale[1, 0] = 2.0 ** 100
+    check_product(z, operand(150, 300, 1, True, 2), None, dtype)
+
+
+@pytest.mark.parametrize("shape", [(1, 512, 4096), (24, 1000, 4096), (300, 700, 1024)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_product_twice_streams_and_graphs(shape, dtype):
+    m, n, k = shape
+    a, b = operand(m, k, 1, True, 1), operand(n, k, 128, True, 2)
+    y = ops.fp8_matmul(a, b, out_dtype=dtype)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y2 = ops.fp8_matmul(a, b, out_dtype=dtype)
+        y3 = ops.fp8_matmul(a, b, out_dtype=dtype)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y, y2) and torch.equal(y, y3)
+    # two captured products with different operands, replayed with eager work between
+    a2 = operand(m, k, 1, True, 7)
+    graphs = []
+    for src in (a, a2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops.fp8_matmul(src, b, out_dtype=dtype)
+        graphs.append((g, out, ops.fp8_matmul(src, b, out_dtype=dtype)))
+    for i in range(4):
+        for g, out, want in graphs:
+            out.zero_()
+            g.replay()
+            ops.fp8_matmul(a, b, out_dtype=dtype)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), i
+    for g, out, _ in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    for _, out, want in graphs:
+        assert torch.equal(out, want)
+
+
+def test_product_refusals():
+    a, b = operand(4, 256, 1, True, 1), operand(8, 256, 128, True, 2)
+    with pytest.raises(ValueError, match="scales"):
+        ops.fp8_matmul(a, operand(8, 256, 128, False, 2))
+    with pytest.raises(ValueError):
+        ops.fp8_matmul(a, operand(8, 128, 1, True, 2))
+    with pytest.raises(ValueError, match="bias"):
+        ops.fp8_matmul(a, b, bias=torch.zeros(8, device=DEV, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="out_dtype"):
+        ops.fp8_matmul(a, b, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="does not belong"):
+        ops.Fp8Blocks(a.data, a.scale[:, :1])
+    with pytest.raises(ValueError, match="block_rows"):
+        ops.Fp8Blocks(a.data, a.scale, 64)
+    with pytest.raises(ValueError, match="forms"):
+        ops.fp8_quantize(torch.zeros(2, 2, device=DEV), forms="neither")
+    with pytest.raises(ValueError, match="scale_dtype"):
+        ops.fp8_quantize(torch.zeros(2, 2, device=DEV), scale_dtype=torch.float16)
+    with pytest.raises(ValueError, match="dtype"):
+        ops.fp8_quantize(torch.zeros(2, 2, device=DEV, dtype=torch.float64))
+    with pytest.raises(ValueError, match="column sums"):
+        ops.fp8_quantize(torch.zeros(2, 2, device=DEV), colsum=True)
+
+
+# ------------------------------------------------------------------------------------------- norm
+
+NORMS = [(1, 1), (3, 7), (2, 128), (5, 300), (4, 512), (4, 1000), (3, 1031), (7, 2048), (2, 4096), (3, 5000), (2, 8192), (2, 12000), (1, 20001), (2, 40000)]
+
+
+@pytest.mark.parametrize("rows,cols", NORMS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("with_res", [True, False])
+def test_norm_forward(rows, cols, dtype, with_res):
+    g = torch.Generator(device=DEV).manual_seed(rows + cols)
+    x = torch.randn(rows, cols, device=DEV, generator=g).to(dtype) * 3
+    r = torch.randn(rows, cols, device=DEV, generator=g).to(dtype) if with_res else None
+    w = torch.randn(cols, device=DEV, generator=g)
+    y, h, rstd = ops.rms_norm_forward(x, w, residual=r, eps=1e-6)
+    want_h = (x.float() + r.float()).to(dtype) if with_res else x
+    assert torch.equal(h, want_h)
+    want, wr = F8.rms_norm(f64(h), f64(w), 1e-6)
+    assert np.array_equal(rstd.cpu().numpy(), wr.astype(np.float32))
+    tol = np.abs(want) * (3 * U * 1.001 + half_step(dtype) * (1 + 4 * U)) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert np.all(np.abs(f64(y) - want) <= tol)
+    # codes of the fp32 values (h * rstd) * w
+    q, h2, _ = ops.rms_norm_forward(x, w, residual=r, eps=1e-6, quantize=True)
+    assert torch.equal(h2, h)
+    v = (h.float().cpu().numpy() * wr.astype(np.float32)[:, None]) * w.cpu().numpy()
+    c, e = F8.quantize(v)
+    same_codes(codes_of(q), c)
+    assert np.array_equal(exps_of(q), e)
+
+
+@pytest.mark.parametrize("rows,cols", NORMS + [(700, 256), (1100, 1031), (600, 4096), (530, 9000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_backward(rows, cols, dtype):
+    g = torch.Generator(device=DEV).manual_seed(rows + cols)
+    h = torch.randn(rows, cols, device=DEV, generator=g).to(dtype) * 2
+    dy = torch.randn(rows, cols, device=DEV, generator=g).to(dtype)
+    dh = torch.randn(rows, cols, device=DEV, generator=g).to(dtype) if rows % 2 else None
+    w = torch.randn(cols, device=DEV, generator=g)
+    _, _, rstd = ops.rms_norm_forward(h, w, eps=1e-5)
+    dx, dw = ops.rms_norm_backward(dy, h, w, rstd, dh=dh)
+    want_dx, want_dw = F8.rms_norm_grad(f64(dy), f64(h), f64(w), 1e-5, f64(dh) if dh is not None else None)
+    rs = f64(rstd)[:, None]
+    n, gg = f64(h) * rs, f64(dy) * f64(w)
+    chain = 60 if cols <= 16384 else cols // 1024 + 30
+    m_err = chain * U * np.abs(gg * n).mean(1, keepdims=True)
+    m = np.abs((gg * n).mean(1, keepdims=True))
+    tol = rs * (np.abs(n) * m_err + 6 * U * (np.abs(gg) + np.abs(n) * m))
+    if dh is not None:
+        tol = tol + 2 * U * np.abs(f64(dh))
+    tol = tol * 1.01 + half_step(dtype) * np.abs(want_dx) * 1.01 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert np.all(np.abs(f64(dx) - want_dx) <= tol)
+    terms = np.abs(f64(dy) * n).sum(0)
+    assert np.all(np.abs(f64(dw) - want_dw) <= (rows / (64 if cols > 16384 else 512) + 5) * U * terms * 1.01 + U * np.abs(want_dw))
+    dx2, none = ops.rms_norm_backward(dy, h, w, rstd, dh=dh, need_dweight=False)
+    assert none is None and torch.equal(dx2, dx)
+    none, dw2 = ops.rms_norm_backward(dy, h, w, rstd, dh=dh, need_dx=False)
+    assert none is None and torch.equal(dw2, dw)
+
+
+def test_norm_gradient_against_differences():
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(3, 200, device=DEV, generator=g)
+    w = torch.randn(200, device=DEV, generator=g)
+    dy = torch.randn(3, 200, device=DEV, generator=g)
+    _, h, rstd = ops.rms_norm_forward(x, w)
+    dx, dw = ops.rms_norm_backward(dy, h, w, rstd)
+
+    def loss(xv, wv):
+        return (F8.rms_norm(xv, wv, 1e-6)[0] * f64(dy)).sum()
+    rs, d = np.random.RandomState(0), 1e-5
+    for _ in range(20):
+        v = rs.standard_normal((3, 200))
+        num = (loss(f64(x) + d * v, f64(w)) - loss(f64(x) - d * v, f64(w))) / (2 * d)
+        # central differences in double: d^2 / 6 of a third derivative of order 10, and 1e-15 |loss| / d; the kernel: 1e-6 of its terms
+        assert abs(num - (f64(dx) * v).sum()) <= 1e-6 * np.abs(f64(dx) * v).sum() + 1e-7
+        u = rs.standard_normal(200)
+        num = (loss(f64(x), f64(w) + d * u) - loss(f64(x), f64(w) - d * u)) / (2 * d)
+        assert abs(num - (f64(dw) * u).sum()) <= 1e-6 * np.abs(f64(dw) * u).sum() + 1e-7
+
+
+def test_norm_special_rows_strides_and_places():
+    g = torch.Generator(device=DEV).manual_seed(0)
+    big = torch.randn(9, 1100, device=DEV, generator=g).bfloat16()
+    x, r = big[1:7, 3:1003], big[2:8, 50:1050]
+    w = torch.randn(1000, device=DEV, generator=g)
+    y, h, rstd = ops.rms_norm_forward(x, w, residual=r)
+    y2, h2, rstd2 = ops.rms_norm_forward(x.contiguous(), w, residual=r.contiguous())
+    assert torch.equal(y, y2) and torch.equal(h, h2) and torch.equal(rstd, rstd2)
+    dy = big[0:6, 7:1007]
+    for a, b in zip(ops.rms_norm_backward(dy, h, w, rstd, dh=x), ops.rms_norm_backward(dy.contiguous(), h, w, rstd, dh=x.contiguous())):
+        assert torch.equal(a, b)
+    z = torch.randn(6, 1000, device=DEV, generator=g)
+    z[0] = 0.0                                  # 1 / sqrt(eps), outputs zero
+    z[1, 5], z[2, 6] = float("nan"), float("inf")
+    z[3] = 1e30                                 # squares beyond fp32
+    z[4] = 1e-30
+    y, _, rstd = ops.rms_norm_forward(z, w, eps=1e-6)
+    q, _, _ = ops.rms_norm_forward(z, w, eps=1e-6, quantize=True)
+    assert bool((y[0] == 0).all()) and abs(float(rstd[0]) - 1e3) < 1e-3
+    assert bool(torch.isnan(y[1]).all()) and float(rstd[2]) == 0.0 and bool(torch.isnan(y[2, 6])) and bool((y[2, :6] == 0).all())
+    # the factor is a little below the smallest normal over 1e30: compared with the product of the rounded factor
+    want = z[3].double() * rstd[3].double() * w.double()
+    assert bool(((y[3].double() - want).abs() <= 4 * U * want.abs()).all()) and abs(float(rstd[3]) * 1e30 - 1) < 1e-6
+    c = codes_of(q)
+    assert ((c[1] & 0x7f) == 0x7f).all() and ((c[3] & 0x7f) != 0x7f).all() and (c[0] & 0x7f == 0).all()
+    with pytest.raises(ValueError, match="weight"):
+        ops.rms_norm_forward(z, w[:-1].contiguous())
+    with pytest.raises(ValueError, match="residual"):
+        ops.rms_norm_forward(z, w, residual=z.bfloat16())
+    with pytest.raises(ValueError, match="no columns"):
+        ops.rms_norm_forward(torch.empty(3, 0, device=DEV), torch.empty(0, device=DEV))
+    assert ops.rms_norm_forward(torch.empty(0, 1000, device=DEV), w)[0].shape == (0, 1000)
+    dx, dw = ops.rms_norm_backward(torch.empty(0, 1000, device=DEV), torch.empty(0, 1000, device=DEV), w, torch.empty(0, device=DEV))
+    assert dx.shape == (0, 1000) and torch.equal(dw, torch.zeros(1000, device=DEV))
+
+
+# --------------------------------------------------------------------------------------- clipping
+
+def grads(sizes, types, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return [(torch.randn(n, device=DEV, generator=g) * 2.0 ** (i % 5 - 2)).to(types[i % len(types)]) for i, n in enumerate(sizes)]
+
+
+@pytest.mark.parametrize("sizes", [[1], [0, 5, 0], [8191, 8192, 8193], [1000003], [17 * i for i in range(1, 200)], [3000000, 1, 70000]])
+@pytest.mark.parametrize("types", [[torch.float32], TYPES])
+@pytest.mark.parametrize("share", [0.25, 4.0])
+def test_clip(sizes, types, share):
+    gs = grads(sizes, types)
+    norm = F8.grad_norm([f64(t) for t in gs])
+    max_norm = norm * share
+    assert abs(float(ops.grad_norm(gs)) - norm) <= U * norm * 1.01
+    keep = [t.clone() for t in gs]
+    out = [torch.full_like(t, 7.0) for t in gs]
+    got = ops.clip_grad_norm(gs, max_norm, out=out)
+    assert abs(float(got) - norm) <= U * norm * 1.01
+    k = min(1.0, max_norm / (norm + 1e-6))
+    for t, o, orig in zip(gs, out, keep):
+        assert torch.equal(t, orig)
+        if k == 1.0:
+            assert torch.equal(o, t)
+        want = f64(t) * k
+        tol = np.abs(want) * (3 * U + half_step(t.dtype)) * 1.01 + torch.finfo(t.dtype).smallest_normal * torch.finfo(t.dtype).eps
+        assert np.all(np.abs(f64(o) - want) <= tol)
+    again = ops.clip_grad_norm(gs, max_norm)
+    assert torch.equal(again, got)
+    for t, o in zip(gs, out):
+        assert torch.equal(t, o)
+
+
+def test_clip_special_values_and_refusals():
+    gs = grads([1000, 20], [torch.float32])
+    gs[0][:3] = 1e30  # squares beyond fp32
+    norm = F8.grad_norm([f64(t) for t in gs])
+    assert abs(float(ops.clip_grad_norm(gs, 1.0)) - norm) <= U * norm * 1.01
+    assert abs(F8.grad_norm([f64(t) for t in gs]) - 1.0) < 1e-6
+    gs = grads([1000, 20], [torch.bfloat16])
+    gs[0][5] = float("inf")
+    assert float(ops.clip_grad_norm(gs, 1.0)) == float("inf")
+    assert bool(torch.isnan(gs[0][5])) and bool((gs[1] == 0).all())
+    gs = grads([1000, 20], [torch.float16])
+    gs[1][5] = float("nan")
+    assert np.isnan(float(ops.clip_grad_norm(gs, 1.0))) and bool(torch.isnan(gs[0]).all())
+    z = [torch.zeros(100, device=DEV)]
+    assert float(ops.clip_grad_norm(z, 1.0)) == 0.0 and bool((z[0] == 0).all())
+    t = torch.randn(10, device=DEV)
+    with pytest.raises(ValueError, match="twice"):
+        ops.clip_grad_norm([t, t], 1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        ops.clip_grad_norm([t], -1.0)
+    with pytest.raises(ValueError, match="out"):
+        ops.clip_grad_norm([t], 1.0, out=[torch.empty(11, device=DEV)])
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.clip_grad_norm([torch.randn(4, 4, device=DEV).t()], 1.0)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.clip_grad_norm([t.double()], 1.0)
+
+
+def test_clip_in_two_graphs():
+    gs, g2 = grads([5000, 70001, 3], TYPES, 1), grads([9000, 20], [torch.float32], 2)
+    outs, o2 = [torch.empty_like(t) for t in gs], [torch.empty_like(t) for t in g2]
+    caps = []
+    for src, dst in ((gs, outs), (g2, o2)):
+        ops.clip_grad_norm(src, 1.0, out=dst)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            norm = ops.clip_grad_norm(src, 1.0, out=dst)
+        caps.append((g, norm, src, dst))
+    for i in range(4):
+        for g, norm, src, dst in caps:
+            for t in src:
+                t.mul_(1.5)
+            g.replay()
+            torch.cuda.synchronize()
+            ref = [torch.empty_like(t) for t in src]
+            assert torch.equal(ops.clip_grad_norm(src, 1.0, out=ref), norm)
+            assert all(torch.equal(a, b) for a, b in zip(ref, dst))
+
+
+# ------------------------------------------------------------------------- layers, and all of them together
+
+def rounded(t, block_rows=1, turn=False):
+    """Float64 values of the codes of t (of its transpose)."""
+    v = f64(t).T if turn else f64(t)
+    c, e = F8.quantize(v, block_rows)
+    return F8.values(c, 2.0 ** e.astype(np.float64), block_rows)
+
+
+def near(got, want, mag, dtype, k):
+    """Product of k terms with magnitudes that add up to mag: 2^-10 mag bounds the cut of 7 terms a group of 8 (7 * 2^-13)."""
+    cut = 2.0 ** -10 if dtype != torch.float32 else 0.0
+    tol = (cut + (k + 4 * -(-k // 128)) * 2 * U) * mag
+    tol = tol + half_step(dtype) * (np.abs(want) + tol)
+    assert np.all(np.abs(f64(got) - want) <= tol)
+
+
+@pytest.mark.parametrize("m,n_in,n_out", [(1, 64, 10), (50, 200, 300), (130, 256, 128)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("wtype", [torch.float32, torch.bfloat16])
+def test_linear_and_its_gradients(m, n_in, n_out, dtype, wtype):
+    x = features(m, n_in, torch.float32, 1).clamp(-100, 100).to(dtype).requires_grad_(True)
+    w = (torch.randn(n_in, n_out, device=DEV) / n_in ** 0.5).to(wtype).requires_grad_(True)
+    b = torch.randn(n_out, device=DEV, requires_grad=True)
+    dy = torch.randn(m, n_out, device=DEV).to(dtype)
+    y = fp8.linear(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert y.dtype == dtype and dx.dtype == dtype and dw.dtype == wtype and db.dtype == torch.float32
+    xv, wv = rounded(x), rounded(w, 128)
+    near(y, xv @ wv + f64(b), np.abs(xv) @ np.abs(wv) + np.abs(f64(b)), dtype, n_in)
+    dv = rounded(dy)
+    near(dx, dv @ wv.T, np.abs(dv) @ np.abs(wv.T), dtype, n_out)
+    xt, dt = rounded(x, turn=True), rounded(dy, turn=True)
+    near(dw, xt @ dt.T, np.abs(xt) @ np.abs(dt.T), wtype, m)
+    assert np.all(np.abs(f64(db) - f64(dy).sum(0)) <= U * np.abs(f64(dy).sum(0)) * 1.01 + 1e-12 * np.abs(f64(dy)).sum(0))
+    # parts of the gradients alone, three dimensions, no bias
+    (only,) = torch.autograd.grad(fp8.linear(x, w.detach(), None), (x,), dy)
+    assert torch.equal(only, dx)
+    (only,) = torch.autograd.grad(fp8.linear(x.detach(), w, b.detach()), (w,), dy)
+    assert torch.equal(only, dw)
+    (only,) = torch.autograd.grad(fp8.linear(x.detach(), w.detach(), b), (b,), dy)
+    assert torch.equal(only, db)
+    assert torch.equal(fp8.linear(x.detach().view(1, m, n_in), w, b), y.view(1, m, n_out))
+
+
+def test_packed_layer_serves_the_same():
+    layer = fp8.Fp8Linear(300, 70).to(DEV)
+    x = torch.randn(5, 300, device=DEV)
+    y = layer(x)
+    layer.eval()
+    layer.pack()
+    with torch.no_grad():
+        assert torch.equal(layer(x), y) and layer._packed is not None
+    layer(x).sum().backward()  # with gradients: from the weights
+    layer.load_state_dict(layer.state_dict())
+    assert layer._packed is None
+    with pytest.raises(RuntimeError, match="packed"):
+        fp8.linear(x.requires_grad_(True), layer.pack()._packed, layer.bias)
+    layer.train()
+    assert layer._packed is None
+    with pytest.raises(ValueError, match="need"):
+        fp8.linear(x, torch.zeros(301, 5, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_linear_equals_its_parts(dtype):
+    m, c, n = 60, 520, 200
+    g = torch.Generator(device=DEV).manual_seed(2)
+    mk = lambda *s: torch.randn(*s, device=DEV, generator=g)  # noqa: E731
+    x, r = mk(m, c).to(dtype).requires_grad_(True), mk(m, c).to(dtype).requires_grad_(True)
+    nw, w, b = (1 + 0.1 * mk(c)).requires_grad_(True), (mk(c, n) / 20).requires_grad_(True), mk(n).requires_grad_(True)
+    dy, dh = mk(m, n).to(dtype), mk(m, c).to(dtype)
+    y, h = fp8.norm_linear(x, nw, w, b, residual=r)
+    got = torch.autograd.grad((y, h), (x, r, nw, w, b), (dy, dh))
+    # by the operators one by one
+    q, h2, rstd = ops.rms_norm_forward(x.detach(), nw.detach(), residual=r.detach(), quantize=True)
+    wr, wt = ops.fp8_quantize(w.detach(), forms="both", block_rows=128)
+    assert torch.equal(h, h2) and torch.equal(y, ops.fp8_matmul(q, wt, bias=b.detach(), out_dtype=dtype))
+    dq, dt, db = ops.fp8_quantize(dy, forms="both", colsum=True)
+    dn = ops.fp8_matmul(dq, wr, out_dtype=dtype)
+    dx, dnw = ops.rms_norm_backward(dn, h2, nw.detach(), rstd, dh=dh)
+    dw = ops.fp8_matmul(ops.fp8_transpose(q), dt, out_dtype=torch.float32)
+    for a, want in zip(got, (dx, dx, dnw, dw, db)):
+        assert torch.equal(a, want)
+    # without residual, and with h alone used
+    y1 = fp8.norm_linear(x, nw, w, b)
+    assert torch.equal(y1, ops.fp8_matmul(ops.rms_norm_forward(x.detach(), nw.detach(), quantize=True)[0], wt, bias=b.detach(), out_dtype=dtype))
+    (gx,) = torch.autograd.grad(fp8.norm_linear(x, nw, w, b, residual=r)[1], (x,), dh)
+    assert torch.equal(gx, dh)
+    yn, hn = fp8.rms_norm(x, nw, residual=r)
+    gx, gr, gw = torch.autograd.grad((yn, hn), (x, r, nw), (dh, dh))
+    dx, dnw = ops.rms_norm_backward(dh, h2, nw.detach(), rstd, dh=dh)
+    assert torch.equal(gx, dx) and torch.equal(gr, dx) and torch.equal(gw, dnw)
+
+
+class Block(torch.nn.Module):
+    """Two residual blocks of norm, wide layer, ReLU, narrow layer, and a head: every operator of this file in one model."""
+
+    def __init__(self, c=256, wide=512, classes=10):
+        super().__init__()
+        self.up = torch.nn.ModuleList(fp8.Fp8Linear(c, wide) for _ in range(2))
+        self.down = torch.nn.ModuleList(fp8.Fp8Linear(wide, c) for _ in range(2))
+        self.norms = torch.nn.ModuleList(fp8.RMSNorm(c) for _ in range(3))
+        self.head = fp8.Fp8Linear(c, classes)
+
+    def forward(self, x):
+        h, d = x, None
+        for i in range(2):
+            if d is None:
+                u = fp8.norm_linear(h, self.norms[i].weight, self.up[i].weight, self.up[i].bias)
+            else:
+                u, h = fp8.norm_linear(h, self.norms[i].weight, self.up[i].weight, self.up[i].bias, residual=d)
+            d = self.down[i](torch.relu(u))
+        y, _ = self.norms[2](h, d)
+        return self.head(y)
+
+
+def test_a_model_trains_eagerly_and_as_one_graph():
+    torch.manual_seed(0)
+    a = Block().to(DEV)
+    b = Block().to(DEV)
+    b.load_state_dict(a.state_dict())
+    x, y = torch.randn(96, 256, device=DEV), torch.randint(0, 10, (96,), device=DEV)
+    loss = torch.nn.functional.cross_entropy
+    opt = torch.optim.SGD(a.parameters(), 0.05, momentum=0.9)
+    norms = []
+
+    def eager():
+        opt.zero_grad(set_to_none=True)
+        v = loss(a(x), y)
+        v.backward()
+        gs = [p.grad for p in a.parameters()]
+        assert all(g is not None and bool(torch.isfinite(g).all()) for g in gs)
+        norms.append(float(ops.clip_grad_norm(gs, 0.5)))
+        assert F8.grad_norm([f64(g) for g in gs]) <= 0.5 * (1 + 1e-5)
+        opt.step()
+    step = train.CapturedStep(b, torch.optim.SGD(b.parameters(), 0.05, momentum=0.9), loss, warmup=2, max_norm=0.5)
+    for i in range(5):
+        eager()
+        if i == 1:
+            eager()
+            step(x, y)  # two warm-up steps and a replay
+        elif i > 1:
+            torch.cuda.synchronize()
+            step(x, y)
+        if i >= 1:
+            assert abs(float(step.grad_norm) - norms[-1]) <= 1e-6 * norms[-1]
+            for p, q in zip(a.parameters(), b.parameters()):
+                assert torch.equal(p, q), i
+
+
+def test_train_step_clips():
+    import argparse
+    import quantized_cnn_amd.adp_qtz_fan as fan
+    c = argparse.Namespace(mode="train", prim_init="uniform", num_level_conv=32, num_level_fc=32, l2_reg=5e-4, liar=True, prim_lr=1e-2, q_lr=1e-3, lr=1e-2)
+    fan.beta = 1
+    torch.manual_seed(0)
+    m1 = fan.ResNet(c, 3).to(DEV).train()
+    m2 = fan.ResNet(c, 3).to(DEV).train()
+    m2.load_state_dict(m1.state_dict())
+    x, y = torch.randn(8, 3, 32, 32, device=DEV), torch.randint(0, 10, (8,), device=DEV)
+    s1 = train.TrainStep(m1, c, fan, max_norm=0.1)
+    s2 = train.TrainStep(m2, c, fan, use_graph=True, max_norm=0.1)
+    for _ in range(3):
+        l1, l2 = float(s1(x, y)), float(s2(x, y))
+        assert abs(l1 - l2) <= 1e-4 * abs(l1)
+        assert float(s1.grad_norm) > 0.1 and abs(float(s1.grad_norm) - float(s2.grad_norm)) <= 1e-2 * float(s1.grad_norm)
