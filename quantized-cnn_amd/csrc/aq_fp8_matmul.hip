@@ -200,8 +200,253 @@ __global__ __launch_bounds__(WM *WN * 64) void fp8_matmul_kernel(const MatArgs p
     }
 }
 
+typedef float f16_t __attribute__((ext_vector_type(16)));
+
+// 64 lanes x 16 bytes (or one byte, widened to four) from base + off (per lane) to LDS address lds + 16 * lane (4 * lane).  Inline,
+// because the compiler would wait for every such load before any LDS read that follows; the wait is written where the
+// pipeline needs it.
+__device__ inline void load_to_lds(uint32_t lds, uint32_t off, const uint8_t *base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ inline void load_byte_to_lds(uint32_t lds, uint32_t off, const uint8_t *base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+template <typename P> __device__ inline uint32_t lds_address(P *p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) P *)p; }
+
+// tile number -> tile: each XCD (workgroups go round the 8 of them) takes a contiguous run of numbers, and a run walks the
+// tile grid in bands of 8 tile rows, so that the workgroups of an XCD share operand panels in its L2
+__device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, int &tm, int &tn)
+{
+    const uint32_t total = tiles_m * tiles_n, share = total / 8, rest = total % 8, xcd = id % 8;
+    const uint32_t t = xcd * share + min(xcd, rest) + id / 8;
+    const uint32_t band = t / (8 * tiles_n), height = min(8u, tiles_m - band * 8), in = t - band * 8 * tiles_n;
+    tm = (int)(band * 8 + in % height);
+    tn = (int)(in / height);
+}
+
+// Large products with power-of-two scales.  Two stages of LDS, each a block of K of all tile rows; WM x WN wavefronts.  Half a block
+// (64 codes) is multiplied from registers while the next half is read from LDS:
+//   half 0 of block b:  read half 1 of b;  then wait for block b + 1 in LDS, and for everybody to have read b;
+//   half 1 of block b:  load block b + 2 into the stage that b has left;  read half 0 of b + 1.
+// Reads, loads and matrix instructions stand in the order written (the scheduling fences hold them there): a fragment of B is
+// overwritten by its successor right behind its last use, those of A alternate between two sets.
+template <int BM, int BN, int WM, int WN, typename T>
+__global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kernel(const MatArgs p)
+{
+    constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 fragments of a wavefront
+    constexpr int LOADS = (BM + BN) / 8 / WAVES;                          // 1 KiB loads of 8 rows per wavefront and block
+    constexpr int SLOADS = (BM + BN) / 64 / WAVES;                        // loads of 64 scales per wavefront and block
+    constexpr int STAGE = (BM + BN) * FP8_BLK;
+    static_assert((BM + BN) % (64 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM % 64 == 0, "");
+    static_assert(BM / WM * (BN / WN) * 2 * WAVES <= 2 * STAGE, "the output tile passes through the stages");
+    __shared__ __attribute__((aligned(128))) uint8_t tile[2 * STAGE];
+    __shared__ uint32_t scale[2][BM + BN];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+    // the last tile of a row or column moves back inside the matrix (M >= BM, N >= BN): it computes some outputs again, the same way
+    const int m0 = min(tm * BM, p.M - BM), n0 = min(tn * BN, p.N - BN);
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK, kround = (p.K + 15) & ~15;
+
+    // 16-byte chunk c of tile row r lies at place c ^ (r / 2 & 7): the 16 rows that a fragment reads at a time lie in different
+    // banks.
+    const int chunk = ((lane & 7) ^ (4 * (wave & 1) + (lane >> 4))) * 16;
+    const uint32_t aoff = (uint32_t)(lane >> 3) * (uint32_t)p.lda, boff = (uint32_t)(lane >> 3) * (uint32_t)p.ldb;
+    const uint8_t *abase = p.a + (long long)(m0 + wave * 8) * p.lda, *bbase = p.b + (long long)(n0 + wave * 8) * p.ldb;
+    const uint32_t lds0 = lds_address(tile) + wave * 1024, slds0 = lds_address(&scale[0][0]) + wave * 256;
+    // load i of block kb; what lies past a row's end reads the block's first chunk, masked below
+    auto fetch = [&](int i, int kb, int stage) {
+        const int k = kb * FP8_BLK, r = i * WAVES * 8;
+        const uint32_t c = k + chunk < kround ? chunk : 0;
+        if (r < BM) load_to_lds(lds0 + (stage * BM + r) * FP8_BLK, aoff + c, abase + (long long)r * p.lda + k);
+        else load_to_lds(lds0 + (2 * BM + stage * BN + r - BM) * FP8_BLK, boff + c, bbase + (long long)(r - BM) * p.ldb + k);
+    };
+    uint32_t soff[SLOADS];
+    const uint8_t *sbase[SLOADS];
+#pragma unroll
+    for (int i = 0; i < SLOADS; ++i) {
+        const int r = (i * WAVES + wave) * 64;  // (the wavefront's 64 rows are all A's or all B's)
+        const bool is_a = r < BM;
+        const int first = is_a ? m0 + r : n0 + r - BM, shift = is_a ? p.ashift : p.bshift;
+        const long long ld = is_a ? p.ldas : p.ldbs;
+        sbase[i] = static_cast<const uint8_t *>(is_a ? p.as : p.bs) + (long long)(first >> shift) * ld;
+        soff[i] = (uint32_t)(((first + lane) >> shift) - (first >> shift)) * (uint32_t)ld;
+    }
+    auto fetch_scales = [&](int kb, int stage) {
+#pragma unroll
+        for (int i = 0; i < SLOADS; ++i) load_byte_to_lds(slds0 + stage * (BM + BN) * 4 + i * WAVES * 256, soff[i], sbase[i] + kb);
+    };
+
+    f16_t acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+    // LDS: A of both stages, then B of both, so that stage and fragment are constants in the reads' offset field; one address for
+    // each 16-byte part of a half and operand (kept in registers: the compiler would otherwise keep many more)
+    const int row = lane & 31, gg = lane >> 5;
+    const int o = row * FP8_BLK + ((gg ^ (row >> 1 & 7)) * 16);
+    uint32_t aread[4], bread[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        aread[x] = lds_address(tile) + wm * FP8_BLK + (o ^ (32 * x));
+        bread[x] = lds_address(tile) + (2 * BM + wn) * FP8_BLK + (o ^ (32 * x));
+        asm("" : "+v"(aread[x]), "+v"(bread[x]));
+    }
+    typedef const __attribute__((address_space(3))) i4_t *lds_i4;
+    typedef const __attribute__((address_space(3))) uint32_t *lds_u1;
+    auto read_a = [&](int i, int stage, int h) {
+        const i4_t lo = *(lds_i4)(aread[2 * h] + stage * BM * FP8_BLK + i * 4096), hi = *(lds_i4)(aread[2 * h + 1] + stage * BM * FP8_BLK + i * 4096);
+        return i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    auto read_b = [&](int j, int stage, int h) {
+        const i4_t lo = *(lds_i4)(bread[2 * h] + stage * BN * FP8_BLK + j * 4096), hi = *(lds_i4)(bread[2 * h + 1] + stage * BN * FP8_BLK + j * 4096);
+        return i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    uint32_t asread = lds_address(&scale[0][0]) + (wm + row) * 4, bsread = lds_address(&scale[0][0]) + (BM + wn + row) * 4;
+    asm("" : "+v"(asread), "+v"(bsread));
+    auto read_sa = [&](int i, int stage) { return *(lds_u1)(asread + stage * (BM + BN) * 4 + i * 128); };
+    auto read_sb = [&](int j, int stage) { return *(lds_u1)(bsread + stage * (BM + BN) * 4 + j * 128); };
+    auto mask_half = [&](int kb, int h, i8_t &f) {
+        const int k = kb * FP8_BLK + 64 * h + 16 * gg;
+        const i4_t lo = mask16(i4_t{f[0], f[1], f[2], f[3]}, k, p.K), hi = mask16(i4_t{f[4], f[5], f[6], f[7]}, k + 32, p.K);
+        f = i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    i8_t a0[TM], a1[TM], b[TN];
+    uint32_t sa[TM], sb[TN], sa1[TM];
+    // the matrix instructions of a half; next(t): what goes out behind the t-th of them
+    auto multiply = [&](const i8_t(&a)[TM], auto next) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 0, 0, 0, (int)sb[j], 0, (int)sa[i]);
+                next(j * TM + i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
+    constexpr int LPER = (LOADS + TM * TN - 1) / (TM * TN);
+    auto block = [&](int kb, int stage, bool tail) {
+        if (tail) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) mask_half(kb, 0, a0[i]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) mask_half(kb, 0, b[j]);
+        }
+        multiply(a0, [&](int t) {
+            if (t < TM) a1[t] = read_a(t, stage, 1);
+            if (t % TM == TM - 1) b[t / TM] = read_b(t / TM, stage, 1);
+        });
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if (tail) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) mask_half(kb, 1, a1[i]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) mask_half(kb, 1, b[j]);
+        }
+        multiply(a1, [&](int t) {
+            if (t < TM) {
+                a0[t] = read_a(t, stage ^ 1, 0);
+                sa1[t] = read_sa(t, stage ^ 1);
+            }
+            if (t % TM == TM - 1) {
+                b[t / TM] = read_b(t / TM, stage ^ 1, 0);
+                sb[t / TM] = read_sb(t / TM, stage ^ 1);
+            }
+#pragma unroll
+            for (int e = 0; e < LPER; ++e)
+                if (t * LPER + e < LOADS) fetch(t * LPER + e, min(kb + 2, nkb - 1), stage);
+            if (t == TM * TN - 1) fetch_scales(min(kb + 2, nkb - 1), stage);
+        });
+#pragma unroll
+        for (int i = 0; i < TM; ++i) sa[i] = sa1[i];
+    };
+
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) fetch(i, min(s, nkb - 1), s);
+        fetch_scales(min(s, nkb - 1), s);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS + SLOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        a0[i] = read_a(i, 0, 0);
+        sa[i] = read_sa(i, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        b[j] = read_b(j, 0, 0);
+        sb[j] = read_sb(j, 0);
+    }
+    const int whole = p.K / FP8_BLK;
+    int kb = 0;
+    for (; kb + 2 <= whole; kb += 2) {
+        block(kb, 0, false);
+        block(kb + 1, 1, false);
+    }
+    if (kb < nkb) block(kb, 0, kb >= whole);
+    if (kb + 1 < nkb) block(kb + 1, 1, true);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+
+    // Through LDS to rows: a wavefront's part of the tile, 16-byte chunk c of its row m at place c ^ (m & mask), then whole rows of
+    // it leave with 16 bytes a lane.
+    constexpr int CH = BN / WN / 8;  // chunks of a row
+    T *out = reinterpret_cast<T *>(tile) + wave * (BM / WM) * (BN / WN);
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = 32 * j + 8 * q + 4 * gg;
+            f4_t bias = {0.f, 0.f, 0.f, 0.f};
+            if (p.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n0 + wn + n + e < p.N) bias[e] = p.bias[n0 + wn + n + e];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int m = 32 * i + row;
+                const f4_t v = f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]} + bias;
+                *reinterpret_cast<u2_t *>(out + m * (BN / WN) + ((n / 8) ^ (m & (CH - 1))) * 8 + 4 * gg) = u2_t{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])};
+            }
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    T *y = static_cast<T *>(p.y);
+    const int c = lane & (CH - 1);
+#pragma unroll
+    for (int i = 0; i < BM / WM * CH / 64; ++i) {
+        const int m = i * (64 / CH) + lane / CH, gm = m0 + wm + m, gn = n0 + wn + 8 * c, left = p.N - gn;
+        const u4_t v = *reinterpret_cast<const u4_t *>(out + m * (BN / WN) + (c ^ (m & (CH - 1))) * 8);
+        T *to = y + (long long)gm * p.ldy + gn;
+        if (left >= 8) *reinterpret_cast<u4_any *>(to) = v;
+        else
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+                if (e < left) to[e] = T{(uint16_t)(v[e >> 1] >> 16 * (e & 1))};
+    }
+}
+
 template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t st)
 {
+    if constexpr (MODE == POW2) {
+        if (p.M >= 1024 && p.N >= 1024 && p.K >= 512 && std::max(p.lda, p.ldb) < (1 << 28)) {
+            p.tiles_m = (p.M + 255) / 256;
+            p.tiles_n = (p.N + 255) / 256;
+            hipLaunchKernelGGL((fp8_matmul_large_kernel<256, 256, 4, 2, T>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
+            return;
+        }
+    }
     constexpr int BM = 64, BN = 64;
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;

@@ -193,25 +193,25 @@ def operand(rows, k, block_rows, pow2, seed, spread=True):
 
 
 def check_product(a, b, bias, dtype):
-    y = f64(ops.fp8_matmul(a, b, bias=bias, out_dtype=dtype))
-    va = F8.values(codes_of(a), f64(a.scale.float()), a.block_rows)
-    vb = F8.values(codes_of(b), f64(b.scale.float()), b.block_rows)
+    """Compares with float64 (on the device: the larger ones take long on the host); returns the product as numpy."""
+    y = ops.fp8_matmul(a, b, bias=bias, out_dtype=dtype).double()
+    va, vb = (torch.from_numpy(F8.values(codes_of(q), f64(q.scale.float()), q.block_rows)).to(DEV) for q in (a, b))
     K = va.shape[1]
-    want, mag = va @ vb.T, np.abs(va) @ np.abs(vb).T
+    want, mag = va @ vb.t(), va.abs() @ vb.abs().t()
     if bias is not None:
-        want = want + f64(bias)
-        mag = mag + np.abs(f64(bias))
+        want, mag = want + bias.double(), mag + bias.double().abs()
     if dtype == torch.float32:
-        tol = (K + 4 * -(-K // 128)) * 2 * U * mag + U * np.abs(want)
+        tol = (K + 4 * -(-K // 128)) * 2 * U * mag + U * want.abs()
     else:
-        pad = -K % 8
-        ga = np.pad(np.abs(va), ((0, 0), (0, pad))).reshape(len(va), -1, 8)
-        gb = np.pad(np.abs(vb), ((0, 0), (0, pad))).reshape(len(vb), -1, 8)
-        top = np.zeros_like(mag)
+        pad = (0, -K % 8)
+        ga = torch.nn.functional.pad(va.abs(), pad).view(len(va), -1, 8)
+        gb = torch.nn.functional.pad(vb.abs(), pad).view(len(vb), -1, 8)
+        top = torch.zeros_like(mag)
         for j in range(ga.shape[1]):
-            top += (ga[:, None, j] * gb[None, :, j]).max(2)
+            top += torch.stack([ga[:, j, e, None] * gb[None, :, j, e] for e in range(8)]).amax(0)
         tol = 7 * 2.0 ** -13 * top + (K + 4 * -(-K // 128)) * 2 * U * mag
-        tol = tol + half_step(dtype) * (np.abs(want) + tol)
+        tol = tol + half_step(dtype) * (want.abs() + tol)
+    y, want, tol = (t.cpu().numpy() for t in (y, want, tol))
     # fp16: from 65520 on the nearest fp16 number is the infinity (of the sum's sign)
     lim = 65520.0 if dtype == torch.float16 else np.inf
     over = np.abs(want) - tol >= lim
@@ -243,10 +243,18 @@ def test_product_other_forms(pow2):
     check_product(operand(7, 300, 128, pow2, 1), operand(260, 300, 1, pow2, 2), torch.randn(260, device=DEV), torch.float16)
 
 
+@pytest.mark.parametrize("m,n,k", [(1024, 1024, 512), (1030, 1300, 700), (1100, 1025, 1029), (1281, 1150, 576), (1024, 1400, 650)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_large_product(m, n, k, dtype, pow2):
+    a, b = operand(m, k, 1, pow2, m + n, False), operand(n, k, 128 if n % 2 else 1, pow2, k + 1, False)
+    check_product(a, b, torch.randn(n, device=DEV) if m % 2 else None, dtype)
+
+
 def test_product_of_whole_numbers_is_exact():
     """Small integers: every partial sum is a whole number below 2^24, so each path has to give the result itself."""
     g = torch.Generator(device=DEV).manual_seed(0)
-    for m, n, k in ((3, 50, 700), (70, 90, 1300), (300, 260, 640)):
+    for m, n, k in ((3, 50, 700), (70, 90, 1300), (300, 260, 640), (2000, 1500, 1984), (1111, 2222, 3333)):
         ai = torch.randint(-4, 5, (m, k), device=DEV, generator=g)
         bi = torch.randint(-4, 5, (n, k), device=DEV, generator=g)
         for sdt in (E8, torch.float32):
