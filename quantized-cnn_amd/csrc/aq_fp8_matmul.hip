@@ -14,6 +14,8 @@
 
 #include "aq_fp8.h"
 
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"  // LDS addresses have 32 bits; the host pass does not know
+
 namespace aq {
 
 typedef int i8_t __attribute__((ext_vector_type(8)));
@@ -437,6 +439,165 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
     }
 }
 
+// Products whose blocks pass through fp32 (FP32S, EXACT): the tile's blocks of K in two stages of LDS as above; per block and pair of
+// fragments the block's sum from zero, then acc += sum * (sA * sB).  EXACT takes each fragment's codes through fp16.
+// BTILE: B's scales are of 128 x 128 tiles, one for the 32 columns of a fragment; otherwise one for each column.
+template <int BM, int BN, int WM, int WN, int MODE, bool BTILE, typename T>
+__global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kernel(const MatArgs p)
+{
+    constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+    constexpr int LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
+    static_assert((BM + BN) % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM + BN <= WAVES * 64, "");
+    __shared__ __attribute__((aligned(128))) uint8_t tile[2 * STAGE];
+    __shared__ __attribute__((aligned(16))) float scale[2][BM + BN];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+    const int m0 = min(tm * BM, p.M - BM), n0 = min(tn * BN, p.N - BN);
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK, kround = (p.K + 15) & ~15;
+    const int chunk = ((lane & 7) ^ (4 * (wave & 1) + (lane >> 4))) * 16;
+    const uint32_t aoff = (uint32_t)(lane >> 3) * (uint32_t)p.lda, boff = (uint32_t)(lane >> 3) * (uint32_t)p.ldb;
+    const uint8_t *abase = p.a + (long long)(m0 + wave * 8) * p.lda, *bbase = p.b + (long long)(n0 + wave * 8) * p.ldb;
+    const uint32_t lds0 = lds_address(tile) + wave * 1024;
+    auto fetch = [&](int kb, int stage) {
+        const int k = kb * FP8_BLK;
+        const uint32_t c = k + chunk < kround ? chunk : 0;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = i * WAVES * 8;
+            if (r < BM) load_to_lds(lds0 + stage * STAGE + r * FP8_BLK, aoff + c, abase + (long long)r * p.lda + k);
+            else load_to_lds(lds0 + stage * STAGE + r * FP8_BLK, boff + c, bbase + (long long)(r - BM) * p.ldb + k);
+        }
+    };
+    // the scale of one tile row per thread
+    const void *ssrc = nullptr;
+    long long sfirst = 0;
+    if (tid < BM) ssrc = p.as, sfirst = (long long)((m0 + tid) >> p.ashift) * p.ldas;
+    else if (tid < BM + BN) ssrc = p.bs, sfirst = (long long)((n0 + tid - BM) >> p.bshift) * p.ldbs;
+    auto read_scale = [&](int kb) { return tid < BM + BN ? load_scale(ssrc, sfirst + kb, p.scale_f32) : 0.0f; };
+
+    f16_t acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    const int row = lane & 31, gg = lane >> 5;
+    const int o = row * FP8_BLK + ((gg ^ (row >> 1 & 7)) * 16);
+    constexpr int W = MODE == EXACT ? 4 : 1;  // matrix instructions of a half block
+    union half_t {
+        i8_t codes;
+        h8_t fp16[W];
+    };
+    auto read_half = [&](const uint8_t *t, int kb, int h, bool tail) {
+        i4_t lo = *reinterpret_cast<const i4_t *>(t + (o ^ (64 * h))), hi = *reinterpret_cast<const i4_t *>(t + (o ^ (64 * h) ^ 32));
+        if (tail) {
+            lo = mask16(lo, kb * FP8_BLK + 64 * h + 16 * gg, p.K);
+            hi = mask16(hi, kb * FP8_BLK + 64 * h + 16 * gg + 32, p.K);
+        }
+        half_t v;
+        if (MODE == EXACT) {
+            v.fp16[0] = codes_to_fp16(lo[0], lo[1]);
+            v.fp16[W > 1 ? 1 : 0] = codes_to_fp16(lo[2], lo[3]);
+            v.fp16[W > 1 ? 2 : 0] = codes_to_fp16(hi[0], hi[1]);
+            v.fp16[W > 1 ? 3 : 0] = codes_to_fp16(hi[2], hi[3]);
+        } else {
+            v.codes = i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
+        return v;
+    };
+    auto block = [&](int kb, int stage, bool tail) {
+        const uint8_t *ta = tile + stage * STAGE + wm * FP8_BLK, *tb = tile + stage * STAGE + (BM + wn) * FP8_BLK;
+        half_t a[TM][2];
+        float sa[TM];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            a[i][0] = read_half(ta + i * 4096, kb, 0, tail);
+            a[i][1] = read_half(ta + i * 4096, kb, 1, tail);
+            sa[i] = scale[stage][wm + 32 * i + row];
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const half_t b0 = read_half(tb + j * 4096, kb, 0, tail), b1 = read_half(tb + j * 4096, kb, 1, tail);
+            f16_t sum[TM];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sum[i][e] = 0.0f;
+            if constexpr (MODE == EXACT) {
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b0.fp16[w], a[i][0].fp16[w], sum[i], 0, 0, 0);
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b1.fp16[w], a[i][1].fp16[w], sum[i], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b0.codes, a[i][0].codes, sum[i], 0, 0, 0, 127, 0, 127);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b1.codes, a[i][1].codes, sum[i], 0, 0, 0, 127, 0, 127);
+            }
+            if (BTILE) {
+                const float sb = scale[stage][BM + wn + 32 * j];
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    const float s = sa[i] * sb;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(sum[i][e], s, acc[i][j][e]);
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f4_t sb = *reinterpret_cast<const f4_t *>(&scale[stage][BM + wn + 32 * j + 8 * q + 4 * gg]);
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = __builtin_fmaf(sum[i][4 * q + e], sa[i] * sb[e], acc[i][j][4 * q + e]);
+                }
+            }
+        }
+    };
+
+    fetch(0, 0);
+    const float first = read_scale(0);
+    if (tid < BM + BN) scale[0][tid] = first;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    for (int kb = 0; kb < nkb; ++kb) {
+        const int stage = kb & 1;
+        // the next block's scale is asked for before its codes, so that the wait for the one is not a wait for the other
+        const float next = kb + 1 < nkb ? read_scale(kb + 1) : 0.0f;
+        if (kb + 1 < nkb) fetch(kb + 1, stage ^ 1);
+        if ((kb + 1) * FP8_BLK <= p.K) block(kb, stage, false);
+        else block(kb, stage, true);
+        if (tid < BM + BN) scale[stage ^ 1][tid] = next;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+    T *y = static_cast<T *>(p.y);
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = n0 + wn + 32 * j + 8 * q + 4 * gg;
+            f4_t bias = {0.f, 0.f, 0.f, 0.f};
+            if (p.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bias[e] = p.bias[n + e];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const f4_t v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                store4(y + (long long)(m0 + wm + 32 * i + row) * p.ldy + n, 4, v + bias);
+            }
+        }
+}
+
 template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t st)
 {
     if constexpr (MODE == POW2) {
@@ -444,6 +605,16 @@ template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t
             p.tiles_m = (p.M + 255) / 256;
             p.tiles_n = (p.N + 255) / 256;
             hipLaunchKernelGGL((fp8_matmul_large_kernel<256, 256, 4, 2, T>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
+            return;
+        }
+    }
+    if constexpr (MODE != POW2) {
+        if (p.M >= 128 && p.N >= 256 && p.M * (long long)p.N >= 512 * 1024) {
+            p.tiles_m = (p.M + 127) / 128;
+            p.tiles_n = (p.N + 255) / 256;
+            // (the last tile of a row may start anywhere: a fragment's 32 columns then have scales of two tiles)
+            if (p.bshift && p.N % 32 == 0) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, true, T>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
+            else hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, false, T>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
             return;
         }
     }
