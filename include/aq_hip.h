@@ -486,7 +486,7 @@ int aq_fp8_dequantize(const uint8_t *q, long long ldq, const void *qs, long long
  * the next multiple of 16 bytes (what lies behind K does not matter).  Sums in fp32.  bf16 / fp16 outputs: the 8-bit matrix
  * instructions, which align the products of a group of 8 to the largest of them and drop what lies 2^-14 below it; fp32
  * output: the codes as fp16 through the 16-bit instructions, whose sums keep fp32.  workspace:
- * aq_fp8_matmul_workspace_bytes(M, N, K) bytes, 16-byte aligned (partial sums of products with few rows). */
+ * aq_fp8_matmul_workspace_bytes(M, N, K) bytes, 16-byte aligned (partial sums of products with few tiles and long rows). */
 size_t aq_fp8_matmul_workspace_bytes(long long M, long long N, long long K);
 int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long ldas, int a_block_rows, const uint8_t *b, long long ldb,
                   const void *bs, long long ldbs, int b_block_rows, long long M, long long N, long long K, int scale_type,

@@ -35,6 +35,8 @@ struct MatArgs {
     int ashift, bshift;  // rows that share a scale: 2^shift
     int scale_f32;
     uint32_t tiles_m, tiles_n;
+    int splits, split_blocks;  // fp8_matmul_large_kernel: K in `splits` parts of `split_blocks` blocks, sums to `part`
+    float *part;
 };
 
 // zero what lies at K or behind it in 16 codes that start at k
@@ -77,131 +79,6 @@ template <typename T> __device__ inline void store4(T *p, int n, const f4_t &v)
         if (i < n) p[i] = from_f32<T>(v[i]);
 }
 
-// Tiles of BM x BN, WM x WN wavefronts, K in steps of one block of 128 bytes.  Operands go from memory to LDS without passing
-// registers, 16 bytes a lane; row r of a tile lies at 128 r with its 16-byte chunk c at place c ^ (r & 7), which spreads the
-// 16 rows that a fragment reads over all banks.  A lane of a fragment takes chunks g and g + 4 of its row (g = lane / 16): the
-// same K order for both operands, which is all that a sum over k needs.
-template <int BM, int BN, int WM, int WN, int MODE, typename T>
-__global__ __launch_bounds__(WM *WN * 64) void fp8_matmul_kernel(const MatArgs p)
-{
-    constexpr int THREADS = WM * WN * 64, WAVES = WM * WN;
-    constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-    constexpr int LOADS = (BM + BN) / 8 / WAVES;  // 1 KiB loads of 8 rows per wavefront and step
-    static_assert((BM + BN) % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM + BN <= THREADS, "");
-    __shared__ __attribute__((aligned(16))) uint8_t tile[2][(BM + BN) * FP8_BLK];
-    __shared__ __attribute__((aligned(16))) uint32_t scale[2][BM + BN];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int m0 = (int)(blockIdx.x % p.tiles_m) * BM, n0 = (int)(blockIdx.x / p.tiles_m) * BN;
-    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
-    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK, kround = (p.K + 15) & ~15;
-
-    // sources of this lane's 16-byte loads: rows past the end read the last row (their results are not stored)
-    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
-    const uint8_t *src[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int r = (i * WAVES + wave) * 8 + (lane >> 3);  // tile rows: A's, then B's (uniform over the wavefront's eight)
-        src[i] = r < BM ? p.a + (long long)min(m0 + r, p.M - 1) * p.lda : p.b + (long long)min(n0 + r - BM, p.N - 1) * p.ldb;
-    }
-    // the scale of one tile row per thread
-    const uint8_t *ssrc = nullptr;
-    if (tid < BM + BN) {
-        const long long i = tid < BM ? (long long)(min(m0 + tid, p.M - 1) >> p.ashift) * p.ldas : (long long)(min(n0 + tid - BM, p.N - 1) >> p.bshift) * p.ldbs;
-        ssrc = static_cast<const uint8_t *>(tid < BM ? p.as : p.bs) + i * (p.scale_f32 ? 4 : 1);
-    }
-    auto read_scale = [&](int kb) -> uint32_t {
-        if (tid >= BM + BN) return 0;
-        if (MODE == POW2) return ssrc[kb];
-        return __float_as_uint(load_scale(ssrc, kb, p.scale_f32));
-    };
-    auto fetch = [&](int kb, int buf) {
-        const int k = kb * FP8_BLK + chunk;
-        const int at = k < kround ? k : 0;  // a chunk past the row's end reads its first one and is masked below
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[i] + at),
-                                             (__attribute__((address_space(3))) void *)(tile[buf] + (i * WAVES + wave) * 1024), 16, 0, 0);
-    };
-
-    f4_t acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
-
-    const int g = lane >> 4, off = (lane & 15) * FP8_BLK + ((g ^ (lane & 7)) * 16);
-    auto compute = [&](int kb, int buf, bool tail) {
-        const uint8_t *ta = tile[buf] + wm * FP8_BLK, *tb = tile[buf] + (BM + wn) * FP8_BLK;
-        const uint32_t *sa = scale[buf] + wm, *sb = scale[buf] + BM + wn;
-        auto fragment = [&](const uint8_t *t, int i) {
-            i4_t lo = *reinterpret_cast<const i4_t *>(t + i * 2048 + off), hi = *reinterpret_cast<const i4_t *>(t + i * 2048 + (off ^ 64));
-            if (tail) {
-                lo = mask16(lo, kb * FP8_BLK + g * 16, p.K);
-                hi = mask16(hi, kb * FP8_BLK + g * 16 + 64, p.K);
-            }
-            return i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        };
-        i8_t af[TM];
-        uint32_t av[TM];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            af[i] = fragment(ta, i);
-            av[i] = sa[16 * i + (lane & 15)];
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const i8_t bf = fragment(tb, j);
-            if (MODE == POW2) {
-                const int bv = (int)sb[16 * j + (lane & 15)];
-#pragma unroll
-                for (int i = 0; i < TM; ++i) acc[i][j] = block_product<MODE>(bf, af[i], acc[i][j], bv, (int)av[i]);
-            } else {
-                const f4_t bv = *reinterpret_cast<const f4_t *>(sb + 16 * j + 4 * g);
-#pragma unroll
-                for (int i = 0; i < TM; ++i) {
-                    const f4_t s = block_product<MODE>(bf, af[i], acc[i][j], 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(s[e], bv[e] * __uint_as_float(av[i]), acc[i][j][e]);
-                }
-            }
-        }
-    };
-
-    fetch(0, 0);
-    if (tid < BM + BN) scale[0][tid] = read_scale(0);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    for (int kb = 0; kb < nkb; ++kb) {
-        const int buf = kb & 1;
-        uint32_t next = 0;
-        if (kb + 1 < nkb) {
-            fetch(kb + 1, buf ^ 1);
-            next = read_scale(kb + 1);
-        }
-        if ((kb + 1) * FP8_BLK <= p.K) compute(kb, buf, false);
-        else compute(kb, buf, true);
-        if (tid < BM + BN) scale[buf ^ 1][tid] = next;
-        __builtin_amdgcn_s_waitcnt(0);  // the next step's tile is in LDS before anybody passes the barrier
-        __syncthreads();
-    }
-
-    T *y = static_cast<T *>(p.y);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int n = n0 + wn + 16 * j + 4 * g;
-        f4_t bias = {0.f, 0.f, 0.f, 0.f};
-        if (p.bias)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < p.N) bias[e] = p.bias[n + e];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int m = m0 + wm + 16 * i + (lane & 15);
-            if (m < p.M) store4(y + (long long)m * p.ldy + n, p.N - n, acc[i][j] + bias);
-        }
-    }
-}
-
 typedef float f16_t __attribute__((ext_vector_type(16)));
 
 // 64 lanes x 16 bytes (or one byte, widened to four) from base + off (per lane) to LDS address lds + 16 * lane (4 * lane).  Inline,
@@ -228,26 +105,35 @@ __device__ inline void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, 
     tn = (int)(in / height);
 }
 
-// Large products with power-of-two scales.  Two stages of LDS, each a block of K of all tile rows; WM x WN wavefronts.  Half a block
+// Large products with power-of-two scales.  NS stages of LDS, each a block of K of all tile rows; WM x WN wavefronts.  Half a block
 // (64 codes) is multiplied from registers while the next half is read from LDS:
 //   half 0 of block b:  read half 1 of b;  then wait for block b + 1 in LDS, and for everybody to have read b;
-//   half 1 of block b:  load block b + 2 into the stage that b has left;  read half 0 of b + 1.
+//   half 1 of block b:  load block b + NS into the stage that b has left;  read half 0 of b + 1.
 // Reads, loads and matrix instructions stand in the order written (the scheduling fences hold them there): a fragment of B is
 // overwritten by its successor right behind its last use, those of A alternate between two sets.
-template <int BM, int BN, int WM, int WN, typename T>
-__global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kernel(const MatArgs p)
+template <int BM, int BN, int WM, int WN, int NS, bool SPLIT, typename T>
+__global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kernel(MatArgs p)
 {
     constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 fragments of a wavefront
     constexpr int LOADS = (BM + BN) / 8 / WAVES;                          // 1 KiB loads of 8 rows per wavefront and block
-    constexpr int SLOADS = (BM + BN) / 64 / WAVES;                        // loads of 64 scales per wavefront and block
+    constexpr int SLOADS = ((BM + BN) / 64 + WAVES - 1) / WAVES;          // loads of 64 scales per wavefront and block, at most
     constexpr int STAGE = (BM + BN) * FP8_BLK;
-    static_assert((BM + BN) % (64 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM % 64 == 0, "");
-    static_assert(BM / WM * (BN / WN) * 2 * WAVES <= 2 * STAGE, "the output tile passes through the stages");
-    __shared__ __attribute__((aligned(128))) uint8_t tile[2 * STAGE];
-    __shared__ uint32_t scale[2][BM + BN];
+    static_assert((BM + BN) % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM % 64 == 0 && BN % 64 == 0, "");
+    static_assert(BM * BN * 2 <= NS * STAGE, "the output tile passes through the stages");
+    __shared__ __attribute__((aligned(128))) uint8_t tile[NS * STAGE];
+    __shared__ uint32_t scale[NS][BM + BN];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int tm, tn;
-    tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+    const uint32_t tiles = p.tiles_m * p.tiles_n, part = SPLIT ? blockIdx.x / tiles : 0;
+    tile_of(SPLIT ? blockIdx.x - part * tiles : blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+    if (SPLIT) {  // this part of K as if it were the whole
+        const int first = (int)part * p.split_blocks;
+        p.a += (long long)first * FP8_BLK;
+        p.b += (long long)first * FP8_BLK;
+        p.as = static_cast<const uint8_t *>(p.as) + first;
+        p.bs = static_cast<const uint8_t *>(p.bs) + first;
+        p.K = min(p.K - first * FP8_BLK, p.split_blocks * FP8_BLK);
+    }
     // the last tile of a row or column moves back inside the matrix (M >= BM, N >= BN): it computes some outputs again, the same way
     const int m0 = min(tm * BM, p.M - BM), n0 = min(tn * BN, p.N - BN);
     const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
@@ -264,13 +150,13 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
         const int k = kb * FP8_BLK, r = i * WAVES * 8;
         const uint32_t c = k + chunk < kround ? chunk : 0;
         if (r < BM) load_to_lds(lds0 + (stage * BM + r) * FP8_BLK, aoff + c, abase + (long long)r * p.lda + k);
-        else load_to_lds(lds0 + (2 * BM + stage * BN + r - BM) * FP8_BLK, boff + c, bbase + (long long)(r - BM) * p.ldb + k);
+        else load_to_lds(lds0 + (NS * BM + stage * BN + r - BM) * FP8_BLK, boff + c, bbase + (long long)(r - BM) * p.ldb + k);
     };
     uint32_t soff[SLOADS];
     const uint8_t *sbase[SLOADS];
 #pragma unroll
     for (int i = 0; i < SLOADS; ++i) {
-        const int r = (i * WAVES + wave) * 64;  // (the wavefront's 64 rows are all A's or all B's)
+        const int r = min((i * WAVES + wave) * 64, BM + BN - 64);  // (the wavefront's 64 rows are all A's or all B's)
         const bool is_a = r < BM;
         const int first = is_a ? m0 + r : n0 + r - BM, shift = is_a ? p.ashift : p.bshift;
         const long long ld = is_a ? p.ldas : p.ldbs;
@@ -279,7 +165,8 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
     }
     auto fetch_scales = [&](int kb, int stage) {
 #pragma unroll
-        for (int i = 0; i < SLOADS; ++i) load_byte_to_lds(slds0 + stage * (BM + BN) * 4 + i * WAVES * 256, soff[i], sbase[i] + kb);
+        for (int i = 0; i < SLOADS; ++i)
+            if ((BM + BN) % (64 * WAVES) == 0 || (i * WAVES + wave) * 64 < BM + BN) load_byte_to_lds(slds0 + stage * (BM + BN) * 4 + i * WAVES * 256, soff[i], sbase[i] + kb);
     };
 
     f16_t acc[TM][TN];
@@ -290,7 +177,7 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
-    // LDS: A of both stages, then B of both, so that stage and fragment are constants in the reads' offset field; one address for
+    // LDS: A of all stages, then B of all, so that stage and fragment are constants in the reads' offset field; one address for
     // each 16-byte part of a half and operand (kept in registers: the compiler would otherwise keep many more)
     const int row = lane & 31, gg = lane >> 5;
     const int o = row * FP8_BLK + ((gg ^ (row >> 1 & 7)) * 16);
@@ -298,7 +185,7 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
         aread[x] = lds_address(tile) + wm * FP8_BLK + (o ^ (32 * x));
-        bread[x] = lds_address(tile) + (2 * BM + wn) * FP8_BLK + (o ^ (32 * x));
+        bread[x] = lds_address(tile) + (NS * BM + wn) * FP8_BLK + (o ^ (32 * x));
         asm("" : "+v"(aread[x]), "+v"(bread[x]));
     }
     typedef const __attribute__((address_space(3))) i4_t *lds_i4;
@@ -315,11 +202,6 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
     asm("" : "+v"(asread), "+v"(bsread));
     auto read_sa = [&](int i, int stage) { return *(lds_u1)(asread + stage * (BM + BN) * 4 + i * 128); };
     auto read_sb = [&](int j, int stage) { return *(lds_u1)(bsread + stage * (BM + BN) * 4 + j * 128); };
-    auto mask_half = [&](int kb, int h, i8_t &f) {
-        const int k = kb * FP8_BLK + 64 * h + 16 * gg;
-        const i4_t lo = mask16(i4_t{f[0], f[1], f[2], f[3]}, k, p.K), hi = mask16(i4_t{f[4], f[5], f[6], f[7]}, k + 32, p.K);
-        f = i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    };
     i8_t a0[TM], a1[TM], b[TN];
     uint32_t sa[TM], sb[TN], sa1[TM];
     // the matrix instructions of a half; next(t): what goes out behind the t-th of them
@@ -334,74 +216,90 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
             }
     };
     constexpr int LPER = (LOADS + TM * TN - 1) / (TM * TN);
-    auto block = [&](int kb, int stage, bool tail) {
-        if (tail) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i) mask_half(kb, 0, a0[i]);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) mask_half(kb, 0, b[j]);
-        }
+    auto block = [&](int kb, int stage) {
         multiply(a0, [&](int t) {
             if (t < TM) a1[t] = read_a(t, stage, 1);
             if (t % TM == TM - 1) b[t / TM] = read_b(t / TM, stage, 1);
         });
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * LOADS) : "memory");  // block kb + 1 is here, NS - 2 later ones on their way
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        if (tail) {
-#pragma unroll
-            for (int i = 0; i < TM; ++i) mask_half(kb, 1, a1[i]);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) mask_half(kb, 1, b[j]);
-        }
         multiply(a1, [&](int t) {
             if (t < TM) {
-                a0[t] = read_a(t, stage ^ 1, 0);
-                sa1[t] = read_sa(t, stage ^ 1);
+                a0[t] = read_a(t, (stage + 1) % NS, 0);
+                sa1[t] = read_sa(t, (stage + 1) % NS);
             }
             if (t % TM == TM - 1) {
-                b[t / TM] = read_b(t / TM, stage ^ 1, 0);
-                sb[t / TM] = read_sb(t / TM, stage ^ 1);
+                b[t / TM] = read_b(t / TM, (stage + 1) % NS, 0);
+                sb[t / TM] = read_sb(t / TM, (stage + 1) % NS);
             }
 #pragma unroll
             for (int e = 0; e < LPER; ++e)
-                if (t * LPER + e < LOADS) fetch(t * LPER + e, min(kb + 2, nkb - 1), stage);
-            if (t == TM * TN - 1) fetch_scales(min(kb + 2, nkb - 1), stage);
+                if (t * LPER + e < LOADS) fetch(t * LPER + e, min(kb + NS, nkb - 1), stage);
+            if (t == TM * TN - 1) fetch_scales(min(kb + NS, nkb - 1), stage);
         });
 #pragma unroll
         for (int i = 0; i < TM; ++i) sa[i] = sa1[i];
     };
 
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NS; ++s) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) fetch(i, min(s, nkb - 1), s);
         fetch_scales(min(s, nkb - 1), s);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS + SLOADS) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * LOADS) : "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
+    auto begin = [&](int stage) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        a0[i] = read_a(i, 0, 0);
-        sa[i] = read_sa(i, 0);
-    }
+        for (int i = 0; i < TM; ++i) a0[i] = read_a(i, stage, 0), sa[i] = read_sa(i, stage);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        b[j] = read_b(j, 0, 0);
-        sb[j] = read_sb(j, 0);
-    }
+        for (int j = 0; j < TN; ++j) b[j] = read_b(j, stage, 0), sb[j] = read_sb(j, stage);
+    };
+    // Zeros in LDS for what lies at K or behind it in the last block.  Everybody has it in LDS when it is cut, and reads its first half
+    // again.
+    auto cut = [&](int kb, int stage) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        for (int t = tid; t < (BM + BN) * 8; t += WAVES * 64) {
+            const int r = t >> 3, c = t & 7, k = kb * FP8_BLK + 16 * c;
+            if (k + 16 <= p.K) continue;
+            i4_t *at = reinterpret_cast<i4_t *>(tile + (r < BM ? (stage * BM + r) * FP8_BLK : (NS * BM + stage * BN + r - BM) * FP8_BLK) + (c ^ (r >> 1 & 7)) * 16);
+            *at = mask16(*at, k, p.K);
+        }
+        __syncthreads();
+        begin(stage);
+    };
+    begin(0);
     const int whole = p.K / FP8_BLK;
     int kb = 0;
-    for (; kb + 2 <= whole; kb += 2) {
-        block(kb, 0, false);
-        block(kb + 1, 1, false);
+    for (; kb + NS <= whole; kb += NS) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) block(kb + s, s);
     }
-    if (kb < nkb) block(kb, 0, kb >= whole);
-    if (kb + 1 < nkb) block(kb + 1, 1, true);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+        if (kb + s < nkb) {
+            if (kb + s >= whole) cut(kb + s, s);
+            block(kb + s, s);
+        }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
 
+    if (SPLIT) {
+        float *to = p.part + (long long)part * p.M * p.N;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+                    *reinterpret_cast<f4_any *>(to + (long long)(m0 + wm + 32 * i + row) * p.N + n0 + wn + 32 * j + 8 * q + 4 * gg) =
+                        f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        return;
+    }
     // Through LDS to rows: a wavefront's part of the tile, 16-byte chunk c of its row m at place c ^ (m & mask), then whole rows of
     // it leave with 16 bytes a lane.
     constexpr int CH = BN / WN / 8;  // chunks of a row
@@ -598,30 +496,209 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
         }
 }
 
-template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t st)
+// Few rows: bound by the reading of B.  A workgroup has 16 TN columns and 16 TM rows, its wavefronts share out the blocks of K, U
+// neighbouring ones at a time with all their loads in flight, fragments straight from memory (a row's 128 bytes come in one
+// piece); the wavefronts' sums meet in LDS, in a fixed order.
+template <int TM, int TN, int U, int MODE, typename T>
+__global__ __launch_bounds__(512, 2) void fp8_matmul_rows_kernel(const MatArgs p)
 {
-    if constexpr (MODE == POW2) {
-        if (p.M >= 1024 && p.N >= 1024 && p.K >= 512 && std::max(p.lda, p.ldb) < (1 << 28)) {
-            p.tiles_m = (p.M + 255) / 256;
-            p.tiles_n = (p.N + 255) / 256;
-            hipLaunchKernelGGL((fp8_matmul_large_kernel<256, 256, 4, 2, T>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
-            return;
+    constexpr int WAVES = 8;
+    __shared__ __attribute__((aligned(16))) f4_t sums[WAVES][TM * TN][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = (int)(blockIdx.x % p.tiles_n) * 16 * TN, m0 = (int)(blockIdx.x / p.tiles_n) * 16 * TM;
+    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK, kround = (p.K + 15) & ~15;
+    const int r = lane & 15, g = lane >> 4;
+    // rows past the end read the last row (their results are not stored)
+    const uint8_t *arow[TM], *brow[TN];
+    long long as[TM], bs[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int m = min(m0 + 16 * i + r, p.M - 1);
+        arow[i] = p.a + (long long)m * p.lda + 16 * g;
+        as[i] = (long long)(m >> p.ashift) * p.ldas;
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int n = min(n0 + 16 * j + r, p.N - 1);
+        brow[j] = p.b + (long long)n * p.ldb + 16 * g;
+        bs[j] = (long long)(n >> p.bshift) * p.ldbs;
+    }
+    f4_t acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
+
+    auto load_scale_bits = [&](const void *s, long long i) -> uint32_t {
+        return MODE == POW2 ? static_cast<const uint8_t *>(s)[i] : __float_as_uint(load_scale(s, i, p.scale_f32));
+    };
+    auto multiply = [&](const i8_t(&af)[TM], const i8_t(&bf)[TN], const uint32_t(&sa)[TM], const uint32_t(&sb)[TN]) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            if (MODE == POW2) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i) acc[i][j] = block_product<MODE>(bf[j], af[i], acc[i][j], (int)sb[j], (int)sa[i]);
+            } else {
+                f4_t sn;  // the scales of the four columns that this lane's results belong to
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sn[e] = __uint_as_float(__shfl((int)sb[j], 4 * g + e, 64));
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    const f4_t s = block_product<MODE>(bf[j], af[i], acc[i][j], 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(s[e], sn[e] * __uint_as_float(sa[i]), acc[i][j][e]);
+                }
+            }
+        }
+    };
+    const int whole = p.K / FP8_BLK;
+    for (int kb = wave * U; kb < nkb; kb += WAVES * U) {
+        if (kb + U <= whole) {
+            i8_t af[U][TM], bf[U][TN];
+            uint32_t sa[U][TM], sb[U][TN];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = (kb + u) * FP8_BLK;
+                auto fragment = [&](const uint8_t *row) {
+                    const i4_t lo = *reinterpret_cast<const i4_t *>(row + k), hi = *reinterpret_cast<const i4_t *>(row + k + 64);
+                    return i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                };
+#pragma unroll
+                for (int j = 0; j < TN; ++j) bf[u][j] = fragment(brow[j]), sb[u][j] = load_scale_bits(p.bs, bs[j] + kb + u);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) af[u][i] = fragment(arow[i]), sa[u][i] = load_scale_bits(p.as, as[i] + kb + u);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) multiply(af[u], bf[u], sa[u], sb[u]);
+            continue;
+        }
+        for (int at = kb; at < min(kb + U, nkb); ++at) {  // the last blocks; what lies past the row's end reads as zero
+            const int k = at * FP8_BLK;
+            auto fragment = [&](const uint8_t *row) {
+                i4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+                if (k + 16 * g < kround) lo = *reinterpret_cast<const i4_t *>(row + k);
+                if (k + 16 * g + 64 < kround) hi = *reinterpret_cast<const i4_t *>(row + k + 64);
+                lo = mask16(lo, k + 16 * g, p.K);
+                hi = mask16(hi, k + 16 * g + 64, p.K);
+                return i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            i8_t af[TM], bf[TN];
+            uint32_t sa[TM], sb[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) bf[j] = fragment(brow[j]), sb[j] = load_scale_bits(p.bs, bs[j] + at);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) af[i] = fragment(arow[i]), sa[i] = load_scale_bits(p.as, as[i] + at);
+            multiply(af, bf, sa, sb);
         }
     }
-    if constexpr (MODE != POW2) {
-        if (p.M >= 128 && p.N >= 256 && p.M * (long long)p.N >= 512 * 1024) {
-            p.tiles_m = (p.M + 127) / 128;
-            p.tiles_n = (p.N + 255) / 256;
-            // (the last tile of a row may start anywhere: a fragment's 32 columns then have scales of two tiles)
-            if (p.bshift && p.N % 32 == 0) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, true, T>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
-            else hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, false, T>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
-            return;
-        }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) sums[wave][i * TN + j][lane] = acc[i][j];
+    __syncthreads();
+    T *y = static_cast<T *>(p.y);
+    for (int t = tid; t < TM * TN * 64; t += 512) {
+        const int f = t >> 6, l = t & 63, m = m0 + 16 * (f / TN) + (l & 15), n = n0 + 16 * (f % TN) + 4 * (l >> 4);
+        f4_t v = sums[0][f][l];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) v += sums[w][f][l];
+        if (p.bias)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) v[e] += p.bias[n + e];
+        if (m < p.M) store4(y + (long long)m * p.ldy + n, p.N - n, v);
     }
-    constexpr int BM = 64, BN = 64;
+}
+
+template <int TM, int TN, int U, int MODE, typename T> static void launch_rows(MatArgs p, hipStream_t st)
+{
+    p.tiles_m = (p.M + 16 * TM - 1) / (16 * TM);
+    p.tiles_n = (p.N + 16 * TN - 1) / (16 * TN);
+    hipLaunchKernelGGL((fp8_matmul_rows_kernel<TM, TN, U, MODE, T>), dim3(p.tiles_m * p.tiles_n), dim3(512), 0, st, p);
+}
+
+// y = the sum of the parts of K, in their order, + bias; four columns a thread
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_matmul_join_kernel(const float *__restrict__ part, int splits, int M, int N, const float *__restrict__ bias,
+                                                              T *__restrict__ y, long long ldy)
+{
+    const long long t = (long long)blockIdx.x * 256 + threadIdx.x, quads = (N + 3) / 4;
+    const int m = (int)(t / quads), n = (int)(t - m * quads) * 4;
+    if (m >= M) return;
+    const float *p = part + (long long)m * N + n;
+    f4_t v = {0.f, 0.f, 0.f, 0.f};
+    if (n + 4 <= N) {
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f4_any *>(p + (long long)s * M * N);
+    } else {
+        for (int s = 0; s < splits; ++s)
+            for (int e = 0; n + e < N; ++e) v[e] += p[(long long)s * M * N + e];
+    }
+    if (bias)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < N) v[e] += bias[n + e];
+    store4(y + (long long)m * ldy + n, N - n, v);
+}
+
+template <int BM, int BN, int WM, int WN, int NS, typename T> static void launch_large(MatArgs p, hipStream_t st)
+{
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
-    hipLaunchKernelGGL((fp8_matmul_kernel<BM, BN, 2, 2, MODE, T>), dim3(p.tiles_m * p.tiles_n), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((fp8_matmul_large_kernel<BM, BN, WM, WN, NS, false, T>), dim3(p.tiles_m * p.tiles_n), dim3(WM * WN * 64), 0, st, p);
+}
+
+static long long tiles_of(long long M, long long N, long long bm, long long bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); }
+// Parts of K for the 64 x 128 tiles: as many as bring the launch to 256 workgroups, none shorter than four blocks.  Joining them
+// costs about 8 us and a block of K about 0.4 us, so rows of 24 blocks and more only.
+static int matmul_splits(long long M, long long N, long long K)
+{
+    const long long tiles = tiles_of(M, N, 64, 128), nkb = (K + FP8_BLK - 1) / FP8_BLK;
+    if (M <= 64 || N < 128 || tiles > 32 || nkb < 24) return 1;
+    return (int)std::max(1LL, std::min(256 / tiles, nkb / 4));
+}
+
+template <typename T> static void launch_pow2(MatArgs p, hipStream_t st)
+{
+    if (p.N < 128) return launch_rows<4, 2, 2, POW2, T>(p, st);
+    if (p.M >= 256 && p.N >= 256 && tiles_of(p.M, p.N, 256, 256) >= 192) return launch_large<256, 256, 4, 2, 2, T>(p, st);
+    if (p.M >= 128 && tiles_of(p.M, p.N, 128, 128) > 256) return launch_large<128, 128, 2, 2, 2, T>(p, st);
+    if (p.M >= 128 && tiles_of(p.M, p.N, 64, 128) > 256) return launch_large<128, 128, 2, 2, 4, T>(p, st);
+    const int splits = matmul_splits(p.M, p.N, p.K);
+    if (splits == 1) return launch_large<64, 128, 1, 4, 4, T>(p, st);
+    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK;
+    p.split_blocks = (nkb + splits - 1) / splits;
+    p.splits = (nkb + p.split_blocks - 1) / p.split_blocks;
+    p.tiles_m = (p.M + 63) / 64;
+    p.tiles_n = (p.N + 127) / 128;
+    hipLaunchKernelGGL((fp8_matmul_large_kernel<64, 128, 1, 4, 4, true, T>), dim3(p.tiles_m * p.tiles_n * p.splits), dim3(256), 0, st, p);
+    const long long quads = (long long)p.M * ((p.N + 3) / 4);
+    hipLaunchKernelGGL((fp8_matmul_join_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p.part, p.splits, p.M, p.N, p.bias,
+                       static_cast<T *>(p.y), p.ldy);
+}
+
+template <int MODE, typename T> static void launch_block(MatArgs p, hipStream_t st)
+{
+    p.tiles_m = (p.M + 127) / 128;
+    p.tiles_n = (p.N + 255) / 256;
+    const dim3 g(p.tiles_m * p.tiles_n), b(512);
+    // (the last tile of a row may start at any multiple of N's factors: only at a multiple of 32 a fragment's columns have one scale)
+    if (p.bshift && p.N % 32 == 0) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, true, T>), g, b, 0, st, p);
+    else hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, false, T>), g, b, 0, st, p);
+}
+
+template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t st)
+{
+    if (p.M <= 16) return launch_rows<1, 1, 4, MODE, T>(p, st);
+    if (p.M <= 32) return launch_rows<2, 1, 4, MODE, T>(p, st);
+    if (p.M <= 64) return launch_rows<4, 1, 2, MODE, T>(p, st);
+    if constexpr (MODE == POW2) {
+        launch_pow2<T>(p, st);
+    } else {
+        if (tiles_of(p.M, p.N, 64, 16) <= 256) return launch_rows<4, 1, 2, MODE, T>(p, st);
+        if (p.M < 128 || p.N < 256 || tiles_of(p.M, p.N, 64, 32) <= 512) return launch_rows<4, 2, 2, MODE, T>(p, st);
+        launch_block<MODE, T>(p, st);
+    }
 }
 
 } // namespace aq
@@ -630,8 +707,9 @@ extern "C" {
 
 size_t aq_fp8_matmul_workspace_bytes(long long M, long long N, long long K)
 {
-    (void)M, (void)N, (void)K;
-    return 0;
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const int splits = aq::matmul_splits(M, N, K);
+    return splits == 1 ? 0 : (size_t)splits * (size_t)M * (size_t)N * sizeof(float);
 }
 
 int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long ldas, int a_block_rows, const uint8_t *b, long long ldb,
@@ -645,7 +723,7 @@ int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long lda
                "aq_fp8_matmul: blocks of %d and %d rows: 1 or %d", a_block_rows, b_block_rows, FP8_BLK);
     AQ_REQUIRE(M >= 0 && N >= 0 && K >= 1, -EINVAL, "aq_fp8_matmul: bad sizes M=%lld N=%lld K=%lld", M, N, K);
     // a launch holds fewer than 2^32 threads, row and column numbers stay below 2^31
-    AQ_REQUIRE(M < (1LL << 30) && N < (1LL << 30) && K < (1LL << 30) && ((M + 63) / 64) * ((N + 63) / 64) < (1LL << 22), -E2BIG,
+    AQ_REQUIRE(M < (1LL << 30) && N < (1LL << 30) && K < (1LL << 30) && ((M + 63) / 64) * ((N + 15) / 16) < (1LL << 23), -E2BIG,
                "aq_fp8_matmul: M=%lld N=%lld K=%lld is too large for one call", M, N, K);
     if (M == 0 || N == 0) return 0;
     AQ_REQUIRE(a && as && b && bs && y, -EFAULT, "aq_fp8_matmul: NULL pointer");
@@ -657,7 +735,7 @@ int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long lda
     AQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), -ENOSPC,
                "aq_fp8_matmul: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
     const MatArgs p = {a, b, as, bs, bias, y, lda, ldb, ldas, ldbs, ldy, (int)M, (int)N, (int)K, a_block_rows == 1 ? 0 : 7, b_block_rows == 1 ? 0 : 7,
-                       scale_type == AQ_SCALE_F32, 0, 0};
+                       scale_type == AQ_SCALE_F32, 0, 0, 1, 0, static_cast<float *>(workspace)};
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (ytype == AQ_F32) launch_matmul<EXACT, float>(p, st);
     else if (scale_type == AQ_SCALE_POW2) ytype == AQ_BF16 ? launch_matmul<POW2, bf16_el>(p, st) : launch_matmul<POW2, f16_el>(p, st);

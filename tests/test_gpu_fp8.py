@@ -224,7 +224,7 @@ def check_product(a, b, bias, dtype):
 
 
 PRODUCTS = [(1, 64, 128), (1, 1000, 4096), (2, 16, 16), (3, 17, 1), (5, 130, 200), (16, 128, 1000), (17, 257, 384), (33, 65, 130), (64, 64, 128), (65, 300, 513),
-            (100, 1000, 512), (128, 128, 256), (200, 129, 1040), (257, 511, 640), (300, 300, 2048)]
+            (100, 1000, 512), (128, 128, 256), (200, 129, 1040), (257, 511, 640), (300, 300, 2048), (70, 130, 5000), (65, 128, 4100), (129, 257, 1536), (190, 700, 1300)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
@@ -305,7 +305,7 @@ def test_product_special_values(m, dtype):
     check_product(z, operand(150, 300, 1, True, 2), None, dtype)
 
 
-@pytest.mark.parametrize("shape", [(1, 512, 4096), (24, 1000, 4096), (300, 700, 1024)])
+@pytest.mark.parametrize("shape", [(1, 512, 4096), (24, 1000, 4096), (300, 700, 1024), (100, 300, 4096), (1000, 1100, 600)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_product_twice_streams_and_graphs(shape, dtype):
     m, n, k = shape
