@@ -10,6 +10,9 @@
 //          lies 2^-14 below it (measured; 1.5e-5 of a sum of 128 normally distributed products): nothing beside the rounding of
 //          a 16-bit output, too much for an fp32 one.  The codes, which are exact in fp16, go through the 16x16x32 fp16
 //          instruction instead (measured 1e-8), then as FP32S.
+//   WIDE:  the same for large products with power-of-two scales: code * scale is exact in bf16 (for scales of 2^-117 and more; below,
+//          a code's last bits fall under bf16's smallest step), so the scales go into the conversion, the blocks' sums into
+//          one accumulator through the bf16 instruction, and the fp32 multiplications per block are saved.
 #include <algorithm>
 
 #include "aq_fp8.h"
@@ -55,6 +58,15 @@ __device__ inline h8_t codes_to_fp16(int lo, int hi)
     const h2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
     const h2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
     return h8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+__device__ inline b8_t codes_to_bf16(int lo, int hi, float scale)
+{
+    const b2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const b2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return b8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 template <int MODE> __device__ inline f4_t block_product(const i8_t &b, const i8_t &a, f4_t acc, int sb, int sa)
@@ -337,7 +349,7 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
     }
 }
 
-// Products whose blocks pass through fp32 (FP32S, EXACT): the tile's blocks of K in two stages of LDS as above; per block and pair of
+// Large products whose blocks pass through fp32 (FP32S, EXACT): the tile's blocks of K in two stages of LDS as above; per block and pair of
 // fragments the block's sum from zero, then acc += sum * (sA * sB).  EXACT takes each fragment's codes through fp16.
 // BTILE: B's scales are of 128 x 128 tiles, one for the 32 columns of a fragment; otherwise one for each column.
 template <int BM, int BN, int WM, int WN, int MODE, bool BTILE, typename T>
@@ -412,9 +424,9 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
         float sa[TM];
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
+            sa[i] = scale[stage][wm + 32 * i + row];
             a[i][0] = read_half(ta + i * 4096, kb, 0, tail);
             a[i][1] = read_half(ta + i * 4096, kb, 1, tail);
-            sa[i] = scale[stage][wm + 32 * i + row];
         }
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
@@ -493,6 +505,149 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
                 const f4_t v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                 store4(y + (long long)(m0 + wm + 32 * i + row) * p.ldy + n, 4, v + bias);
             }
+        }
+}
+
+// Large products with power-of-two scales and fp32 outputs: tiles of 128 x 256, eight wavefronts with 64 x 64 each.  K in half blocks of
+// 64; three things go on at once, one behind each of the 16 matrix instructions of a half:
+//   the matrix instructions of half s;  the conversion to bf16 of half s + 1, four codes' pairs at a time;  the LDS reads of half s + 2,
+//   into the registers that the conversion has emptied.
+// At the start of block b, block b + 1 is in LDS, everybody has read b, and the load of b + 2 takes its place.
+__global__ __launch_bounds__(512, 2) void fp8_matmul_wide_kernel(const MatArgs p)
+{
+    constexpr int BM = 128, BN = 256, WAVES = 8, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
+    __shared__ __attribute__((aligned(128))) uint8_t tile[2 * STAGE];
+    __shared__ uint32_t scale[2][WAVES * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+    const int m0 = min(tm * BM, p.M - BM), n0 = min(tn * BN, p.N - BN);
+    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK, kround = (p.K + 15) & ~15, whole = p.K / FP8_BLK;
+
+    const int chunk = ((lane & 7) ^ (4 * (wave & 1) + (lane >> 4))) * 16;  // as in fp8_matmul_large_kernel
+    const uint32_t aoff = (uint32_t)(lane >> 3) * (uint32_t)p.lda, boff = (uint32_t)(lane >> 3) * (uint32_t)p.ldb;
+    const uint8_t *abase = p.a + (long long)(m0 + wave * 8) * p.lda, *bbase = p.b + (long long)(n0 + wave * 8) * p.ldb;
+    const uint32_t lds0 = lds_address(tile) + wave * 1024;
+    auto fetch = [&](int i, int kb, int stage) {
+        const int k = kb * FP8_BLK, r = i * WAVES * 8;
+        const uint32_t c = k + chunk < kround ? chunk : 0;
+        if (r < BM) load_to_lds(lds0 + stage * STAGE + r * FP8_BLK, aoff + c, abase + (long long)r * p.lda + k);
+        else load_to_lds(lds0 + stage * STAGE + r * FP8_BLK, boff + c, bbase + (long long)(r - BM) * p.ldb + k);
+    };
+    // 64 scales for each of the first six wavefronts (the others load some again, to a place that nobody reads)
+    const int srow = min(wave * 64, BM + BN - 64);
+    const int sfirst = srow < BM ? m0 + srow : n0 + srow - BM, sshift = srow < BM ? p.ashift : p.bshift;
+    const long long sld = srow < BM ? p.ldas : p.ldbs;
+    const uint8_t *sbase = static_cast<const uint8_t *>(srow < BM ? p.as : p.bs) + (long long)(sfirst >> sshift) * sld;
+    const uint32_t soff = (uint32_t)(((sfirst + lane) >> sshift) - (sfirst >> sshift)) * (uint32_t)sld;
+    const uint32_t slds0 = lds_address(&scale[0][0]) + wave * 256;
+    auto fetch_scales = [&](int kb, int stage) {
+        load_byte_to_lds(slds0 + stage * WAVES * 256, soff, sbase + kb);
+    };
+    auto cut = [&](int kb, int stage) {  // zeros for what lies at K or behind it
+        for (int t = tid; t < (BM + BN) * 8; t += WAVES * 64) {
+            const int r = t >> 3, c = t & 7, k = kb * FP8_BLK + 16 * c;
+            if (k + 16 <= p.K) continue;
+            i4_t *at = reinterpret_cast<i4_t *>(tile + stage * STAGE + r * FP8_BLK + (c ^ (r >> 1 & 7)) * 16);
+            *at = mask16(*at, k, p.K);
+        }
+        __syncthreads();
+    };
+
+    f16_t acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+    const int row = lane & 31, gg = lane >> 5;
+    const uint32_t o = row * FP8_BLK + ((gg ^ (row >> 1 & 7)) * 16);
+    const uint32_t aread = lds_address(tile) + wm * FP8_BLK + o, bread = lds_address(tile) + (BM + wn) * FP8_BLK + o;
+    typedef const __attribute__((address_space(3))) i4_t *lds_i4;
+    typedef const __attribute__((address_space(3))) uint32_t *lds_u1;
+    const uint32_t asread = lds_address(&scale[0][0]) + (wm + row) * 4, bsread = lds_address(&scale[0][0]) + (BM + wn + row) * 4;
+    // fragments: 0, 1 of A, 2, 3 of B
+    i4_t raw[4][2];
+    b8_t even[4][4], odd[4][4];
+    uint32_t sc[2][4];
+    auto read_raw = [&](int f, int stage, int h) {
+        const uint32_t base = f < 2 ? aread : bread;
+        uint32_t p0 = base, p1;  // (turned at the read: there are no registers to keep the four addresses)
+        if (h) asm volatile("v_xor_b32 %0, 64, %1" : "=v"(p0) : "v"(base));
+        if (h) asm volatile("v_xor_b32 %0, 0x60, %1" : "=v"(p1) : "v"(base));
+        else asm volatile("v_xor_b32 %0, 32, %1" : "=v"(p1) : "v"(base));
+        raw[f][0] = *(lds_i4)(p0 + stage * STAGE + (f & 1) * 4096);
+        raw[f][1] = *(lds_i4)(p1 + stage * STAGE + (f & 1) * 4096);
+    };
+    auto read_scales = [&](int stage) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f) sc[stage][f] = *(lds_u1)((f < 2 ? asread : bsread) + stage * WAVES * 256 + (f & 1) * 128);
+    };
+    auto convert = [&](b8_t(&to)[4][4], int f, int w, uint32_t s) {  // (the conversion takes the exponent field alone: 2^(b - 127) for b = 0 too)
+        to[f][w] = codes_to_bf16(raw[f][w >> 1][2 * (w & 1)], raw[f][w >> 1][2 * (w & 1) + 1], __uint_as_float(s << 23));
+    };
+    auto half = [&](const b8_t(&now)[4][4], b8_t(&next)[4][4], const uint32_t(&s)[4], int rstage, int h, int kb, int fstage) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const int w = t >> 2, i = t >> 1 & 1, j = t & 1;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now[2 + j][w], now[i][w], acc[i][j], 0, 0, 0);
+            convert(next, t >> 2, t & 3, s[t >> 2]);
+            if ((t & 3) == 3) read_raw(t >> 2, rstage, h);
+            if (h == 0 && t < LOADS) fetch(t, min(kb + 2, nkb - 1), fstage);
+            if (h == 0 && t == LOADS) fetch_scales(min(kb + 2, nkb - 1), fstage);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto block = [&](int kb, int stage) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if (kb + 1 == whole && whole < nkb) cut(kb + 1, stage ^ 1);
+        read_scales(stage ^ 1);
+        half(even, odd, sc[stage], stage ^ 1, 0, kb, stage);
+        half(odd, even, sc[stage ^ 1], stage ^ 1, 1, kb, stage);
+    };
+
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) fetch(i, min(s, nkb - 1), s);
+        fetch_scales(min(s, nkb - 1), s);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if (whole == 0) cut(0, 0);
+    read_scales(0);
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+        read_raw(f, 0, 0);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) convert(even, f, w, sc[0][f]);
+        read_raw(f, 0, 1);
+    }
+    for (int kb = 0; kb < nkb; kb += 2) {
+        block(kb, 0);
+        if (kb + 1 < nkb) block(kb + 1, 1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    float *y = static_cast<float *>(p.y);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = n0 + wn + 32 * j + 8 * q + 4 * gg;
+            f4_t bias = {0.f, 0.f, 0.f, 0.f};
+            if (p.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bias[e] = p.bias[n + e];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<f4_any *>(y + (long long)(m0 + wm + 32 * i + row) * p.ldy + n) =
+                    f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]} + bias;
         }
 }
 
@@ -682,6 +837,12 @@ template <int MODE, typename T> static void launch_block(MatArgs p, hipStream_t 
     p.tiles_m = (p.M + 127) / 128;
     p.tiles_n = (p.N + 255) / 256;
     const dim3 g(p.tiles_m * p.tiles_n), b(512);
+    if constexpr (MODE == EXACT) {
+        if (!p.scale_f32) {
+            hipLaunchKernelGGL(fp8_matmul_wide_kernel, g, b, 0, st, p);
+            return;
+        }
+    }
     // (the last tile of a row may start at any multiple of N's factors: only at a multiple of 32 a fragment's columns have one scale)
     if (p.bshift && p.N % 32 == 0) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, true, T>), g, b, 0, st, p);
     else hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, false, T>), g, b, 0, st, p);
