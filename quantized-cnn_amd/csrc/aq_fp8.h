@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/aq_hip.h"
 #include "aq_common.h"
@@ -62,22 +63,70 @@ __device__ inline void load8(const e4m3_el *p, float (&v)[8])
         v[4 * i] = lo[0], v[4 * i + 1] = lo[1], v[4 * i + 2] = hi[0], v[4 * i + 3] = hi[1];
     }
 }
-__device__ inline void store8(float *p, const float (&v)[8])
-{
-    f4_t a, b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = v[i], b[i] = v[4 + i];
-    *reinterpret_cast<f4_any *>(p) = a;
-    *reinterpret_cast<f4_any *>(p + 4) = b;
-}
 template <typename T> __device__ inline uint32_t pack2(float a, float b) { return (uint32_t)from_f32<T>(a).b | (uint32_t)from_f32<T>(b).b << 16; }
-template <typename T> __device__ inline void store8(T *p, const float (&v)[8])
+// the same, eight elements as they lie in memory (half the registers for 16-bit types), and their values one by one
+template <typename T> struct raw8 { u4_t a; };
+template <> struct raw8<float> { f4_t a, b; };
+template <> struct raw8<e4m3_el> { u2_t a; };
+#define AQ_ACCESS(V, ANY)                                                                                                     \
+    template <bool NT> __device__ inline V load_any(const ANY *p) { return NT ? __builtin_nontemporal_load(p) : *p; }            \
+    template <bool NT> __device__ inline void store_any(V v, ANY *p)                                                             \
+    {                                                                                                                            \
+        if (NT) __builtin_nontemporal_store(v, p);                                                                               \
+        else *p = v;                                                                                                             \
+    }
+AQ_ACCESS(f4_t, f4_any)
+AQ_ACCESS(u4_t, u4_any)
+AQ_ACCESS(u2_t, u2_any)
+#undef AQ_ACCESS
+// NT: streaming (nontemporal) accesses, for calls that move more than the last-level cache holds
+template <bool NT> __device__ inline raw8<float> load_raw(const float *p)
 {
-    u4_t a;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<u4_any *>(p) = a;
+    return {load_any<NT>(reinterpret_cast<const f4_any *>(p)), load_any<NT>(reinterpret_cast<const f4_any *>(p + 4))};
 }
+template <bool NT> __device__ inline raw8<bf16_el> load_raw(const bf16_el *p) { return {load_any<NT>(reinterpret_cast<const u4_any *>(p))}; }
+template <bool NT> __device__ inline raw8<f16_el> load_raw(const f16_el *p) { return {load_any<NT>(reinterpret_cast<const u4_any *>(p))}; }
+template <bool NT> __device__ inline raw8<e4m3_el> load_raw(const e4m3_el *p) { return {load_any<NT>(reinterpret_cast<const u2_any *>(p))}; }
+// the first n (0..8); the others zero
+__device__ inline raw8<float> load_raw_n(const float *p, int n)
+{
+    if (n >= 8) return load_raw<false>(p);
+    raw8<float> r = {};
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) (i < 4 ? r.a : r.b)[i & 3] = p[i];
+    return r;
+}
+template <typename T> __device__ inline raw8<T> load_raw_n(const T *p, int n)
+{
+    if (n >= 8) return load_raw<false>(p);
+    constexpr int PER = 4 / sizeof(T);
+    raw8<T> r = {};
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) r.a[i / PER] |= (uint32_t)p[i].b << 32 / PER * (i % PER);
+    return r;
+}
+__device__ inline float value(const raw8<float> &r, int i) { return i < 4 ? r.a[i & 3] : r.b[i & 3]; }
+__device__ inline float value(const raw8<bf16_el> &r, int i) { return __uint_as_float(i & 1 ? r.a[i >> 1] & 0xffff0000u : r.a[i >> 1] << 16); }
+__device__ inline float value(const raw8<f16_el> &r, int i) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(r.a[i >> 1] >> 16 * (i & 1))); }
+__device__ inline float value(const raw8<e4m3_el> &r, int i)
+{
+    const int w = (int)r.a[i >> 2];
+    return (i & 3) == 0 ? __builtin_amdgcn_cvt_f32_fp8(w, 0) : (i & 3) == 1 ? __builtin_amdgcn_cvt_f32_fp8(w, 1)
+         : (i & 3) == 2 ? __builtin_amdgcn_cvt_f32_fp8(w, 2) : __builtin_amdgcn_cvt_f32_fp8(w, 3);
+}
+template <bool NT> __device__ inline void store8_any(float *p, const float (&v)[8])
+{
+    store_any<NT>(f4_t{v[0], v[1], v[2], v[3]}, reinterpret_cast<f4_any *>(p));
+    store_any<NT>(f4_t{v[4], v[5], v[6], v[7]}, reinterpret_cast<f4_any *>(p + 4));
+}
+template <bool NT, typename T> __device__ inline void store8_any(T *p, const float (&v)[8])
+{
+    store_any<NT>(u4_t{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])}, reinterpret_cast<u4_any *>(p));
+}
+constexpr long long LAST_LEVEL_CACHE = 256LL << 20;  // bytes
+
 // the first n (0..8) of eight elements; the others read as zero and are not written
 template <typename T> __device__ inline void load_n(const T *p, int n, float (&v)[8])
 {
@@ -91,10 +140,10 @@ template <typename T> __device__ inline void load_n(const T *p, int n, float (&v
     for (int i = 0; i < 7; ++i)
         if (i < n) v[i] = to_f32(p[i]);
 }
-template <typename T> __device__ inline void store_n(T *p, int n, const float (&v)[8])
+template <bool NT = false, typename T> __device__ inline void store_n(T *p, int n, const float (&v)[8])
 {
     if (n >= 8) {
-        store8(p, v);
+        store8_any<NT>(p, v);
         return;
     }
 #pragma unroll
@@ -131,10 +180,10 @@ __device__ inline u2_t e4m3x8(const float (&v)[8], float inv)
     r[1] = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
     return r;
 }
-__device__ inline void store_codes(uint8_t *p, int n, u2_t c)  // the first n (0..8) of eight codes
+template <bool NT = false> __device__ inline void store_codes(uint8_t *p, int n, u2_t c)  // the first n (0..8) of eight codes
 {
     if (n >= 8) {
-        *reinterpret_cast<u2_any *>(p) = c;
+        store_any<NT>(c, reinterpret_cast<u2_any *>(p));
         return;
     }
 #pragma unroll
@@ -152,12 +201,62 @@ __device__ inline float load_scale(const void *s, long long i, int scale_f32)
 {
     return scale_f32 ? static_cast<const float *>(s)[i] : pow2_scale(static_cast<const uint8_t *>(s)[i]);
 }
-// max over the 16 lanes of an aligned group of 16
+// max over the 16 lanes of an aligned group of 16, of numbers that are not negative
 __device__ inline float max16(float v)
 {
+    uint32_t u = __float_as_uint(v);
 #pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-    return v;
+    for (int m = 8; m >= 1; m >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, m, 64));
+    return __uint_as_float(u);
+}
+// Largest finite magnitude of eight values.  Magnitudes compare like their bit patterns as whole numbers, two 16-bit ones at a
+// time; patterns from infinity on are not finite, and only where there is one the values are looked at singly.
+__device__ inline float amax8(const float (&v)[8])
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    if (m < 0x7f800000u) return __uint_as_float(m);
+    float a = 0.0f;
+    for (int i = 0; i < 8; ++i) a = fmaxf(a, finite_abs(v[i]));
+    return a;
+}
+typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+__device__ inline us2_t abs2(uint32_t w) { return __builtin_bit_cast(us2_t, w & 0x7fff7fffu); }
+template <typename T> __device__ constexpr uint32_t infinity16() { return std::is_same<T, bf16_el>::value ? 0x7f80 : 0x7c00; }
+template <typename T> __device__ inline float amax8(const raw8<T> &r)
+{
+    if constexpr (sizeof(T) == 2) {
+        const us2_t m = __builtin_elementwise_max(__builtin_elementwise_max(abs2(r.a[0]), abs2(r.a[1])), __builtin_elementwise_max(abs2(r.a[2]), abs2(r.a[3])));
+        const uint32_t u = max((uint32_t)m[0], (uint32_t)m[1]);
+        if (u < infinity16<T>()) return to_f32(T{(uint16_t)u});
+    }
+    const float v[8] = {value(r, 0), value(r, 1), value(r, 2), value(r, 3), value(r, 4), value(r, 5), value(r, 6), value(r, 7)};
+    return amax8(v);
+}
+// the same for each of the eight columns of eight rows
+template <typename T> __device__ inline void column_amax8(const raw8<T> (&r)[8], float (&m)[8])
+{
+    if constexpr (sizeof(T) == 2) {
+        us2_t c[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            c[k] = abs2(r[0].a[k]);
+#pragma unroll
+            for (int i = 1; i < 8; ++i) c[k] = __builtin_elementwise_max(c[k], abs2(r[i].a[k]));
+        }
+        const us2_t t = __builtin_elementwise_max(__builtin_elementwise_max(c[0], c[1]), __builtin_elementwise_max(c[2], c[3]));
+        if (max((uint32_t)t[0], (uint32_t)t[1]) < infinity16<T>()) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m[j] = to_f32(T{c[j >> 1][j & 1]});
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float v[8] = {value(r[0], j), value(r[1], j), value(r[2], j), value(r[3], j), value(r[4], j), value(r[5], j), value(r[6], j), value(r[7], j)};
+        m[j] = amax8(v);
+    }
 }
 
 template <typename F> inline int by_type(int type, F f)

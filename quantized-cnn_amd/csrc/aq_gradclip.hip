@@ -45,30 +45,37 @@ __device__ inline double grad_block_sum(double v, double *sh)  // 256 threads, f
     return s;
 }
 
-template <typename T> __device__ inline double chunk_squares(const T *p, long long n)
+// 16 bytes of elements and their values
+template <typename T> constexpr int PER16 = 16 / (int)sizeof(T);
+__device__ inline float value16(u4_t v, int i, float) { return __uint_as_float(v[i]); }
+__device__ inline float value16(u4_t v, int i, bf16_el) { return __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16); }
+__device__ inline float value16(u4_t v, int i, f16_el) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(v[i >> 1] >> 16 * (i & 1))); }
+
+template <bool NT, typename T> __device__ inline double chunk_squares(const T *p, long long n)
 {
+    constexpr int P = PER16<T>, ITER = GRAD_CHUNK / (256 * P);
     double s[4] = {0.0, 0.0, 0.0, 0.0};
     if (n >= GRAD_CHUNK) {
-        float v[4][8];
+        u4_t v[ITER];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load8(p + (i * 256 + threadIdx.x) * 8, v[i]);
+        for (int i = 0; i < ITER; ++i) v[i] = load_any<NT>(reinterpret_cast<const u4_any *>(p + (i * 256 + threadIdx.x) * P));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < ITER; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s[i] = __builtin_fma((double)v[i][j], (double)v[i][j], s[i]);
+            for (int j = 0; j < P; ++j) {
+                const double d = (double)value16(v[i], j, T{});
+                s[j & 3] = __builtin_fma(d, d, s[j & 3]);
+            }
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = (i * 256 + threadIdx.x) * 8;
-            float v[8];
-            load_n(p + c, (int)max(0LL, min(8LL, n - c)), v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[i] = __builtin_fma((double)v[j], (double)v[j], s[i]);
+        for (int c = threadIdx.x; c < n; c += 256) {
+            const double d = (double)to_f32(p[c]);
+            s[0] = __builtin_fma(d, d, s[0]);
         }
     }
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
+template <bool NT>
 __global__ __launch_bounds__(256) void grad_squares_kernel(const GradTab t, double *__restrict__ part)
 {
     __shared__ double sh[4];
@@ -76,9 +83,9 @@ __global__ __launch_bounds__(256) void grad_squares_kernel(const GradTab t, doub
     for (int c = blockIdx.x; c < t.blk0[t.count]; c += gridDim.x) {
         const int i = grad_tensor(t, c);
         const long long lo = (long long)(c - t.blk0[i]) * GRAD_CHUNK, n = t.n[i] - lo;
-        if (t.type[i] == AQ_F32) s += chunk_squares(static_cast<const float *>(t.p[i]) + lo, n);
-        else if (t.type[i] == AQ_BF16) s += chunk_squares(static_cast<const bf16_el *>(t.p[i]) + lo, n);
-        else s += chunk_squares(static_cast<const f16_el *>(t.p[i]) + lo, n);
+        if (t.type[i] == AQ_F32) s += chunk_squares<NT>(static_cast<const float *>(t.p[i]) + lo, n);
+        else if (t.type[i] == AQ_BF16) s += chunk_squares<NT>(static_cast<const bf16_el *>(t.p[i]) + lo, n);
+        else s += chunk_squares<NT>(static_cast<const f16_el *>(t.p[i]) + lo, n);
     }
     s = grad_block_sum(s, sh);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
@@ -97,31 +104,29 @@ __global__ __launch_bounds__(256) void grad_finish_kernel(const double *__restri
     }
 }
 
-template <typename T> __device__ inline void chunk_scale(const T *p, T *o, long long n, float k)
+template <bool NT, typename T> __device__ inline void chunk_scale(const T *p, T *o, long long n, float k)
 {
+    constexpr int P = PER16<T>, ITER = GRAD_CHUNK / (256 * P);
     if (n >= GRAD_CHUNK) {
-        float v[4][8];
+        u4_t v[ITER];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load8(p + (i * 256 + threadIdx.x) * 8, v[i]);
+        for (int i = 0; i < ITER; ++i) v[i] = load_any<NT>(reinterpret_cast<const u4_any *>(p + (i * 256 + threadIdx.x) * P));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < ITER; ++i) {
+            u4_t r;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] *= k;
-            store8(o + (i * 256 + threadIdx.x) * 8, v[i]);
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (P == 4) r[j] = __float_as_uint(value16(v[i], j, T{}) * k);
+                else r[j] = pack2<T>(value16(v[i], 2 * j, T{}) * k, value16(v[i], 2 * j + 1, T{}) * k);
+            }
+            store_any<NT>(r, reinterpret_cast<u4_any *>(o + (i * 256 + threadIdx.x) * P));
         }
         return;
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = (i * 256 + threadIdx.x) * 8, m = (int)max(0LL, min(8LL, n - c));
-        float v[8];
-        load_n(p + c, m, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= k;
-        store_n(o + c, m, v);
-    }
+    for (int c = threadIdx.x; c < n; c += 256) o[c] = from_f32<T>(to_f32(p[c]) * k);
 }
 
+template <bool NT>
 __global__ __launch_bounds__(256) void grad_scale_kernel(const GradTab t, const double *__restrict__ part, int nparts, double max_norm,
                                                          float *__restrict__ norm)
 {
@@ -137,9 +142,9 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const GradTab t, const 
         const int i = grad_tensor(t, b);
         if (k == 1.0f && t.p[i] == t.o[i]) continue;  // in place and not clipped
         const long long lo = (long long)(b - t.blk0[i]) * GRAD_CHUNK, n = t.n[i] - lo;
-        if (t.type[i] == AQ_F32) chunk_scale(static_cast<const float *>(t.p[i]) + lo, static_cast<float *>(t.o[i]) + lo, n, k);
-        else if (t.type[i] == AQ_BF16) chunk_scale(static_cast<const bf16_el *>(t.p[i]) + lo, static_cast<bf16_el *>(t.o[i]) + lo, n, k);
-        else chunk_scale(static_cast<const f16_el *>(t.p[i]) + lo, static_cast<f16_el *>(t.o[i]) + lo, n, k);
+        if (t.type[i] == AQ_F32) chunk_scale<NT>(static_cast<const float *>(t.p[i]) + lo, static_cast<float *>(t.o[i]) + lo, n, k);
+        else if (t.type[i] == AQ_BF16) chunk_scale<NT>(static_cast<const bf16_el *>(t.p[i]) + lo, static_cast<bf16_el *>(t.o[i]) + lo, n, k);
+        else chunk_scale<NT>(static_cast<const f16_el *>(t.p[i]) + lo, static_cast<f16_el *>(t.o[i]) + lo, n, k);
     }
 }
 
@@ -192,13 +197,16 @@ int aq_clip_grad_norm(const void *const *tensors, void *const *outs, const long 
         t.blk0[t.count] = (int)chunks;
         return chunks;
     };
-    long long total = 0;
+    long long total = 0, bytes = 0;
+    for (int i = 0; i < n; ++i) bytes += sizes[i] * type_size(types[i]);
+    const bool streaming = bytes > LAST_LEVEL_CACHE;
     for (int base = 0; base < n; base += GRAD_MAX) {
         GradTab t = {};
         AQ_REQUIRE(table(base, t) < (1LL << 31) - GRAD_PARTS, -E2BIG, "aq_clip_grad_norm: too many elements");
         const long long parts = grad_parts(sizes, base, n);
         if (parts == 0) continue;
-        hipLaunchKernelGGL(grad_squares_kernel, dim3((unsigned)parts), dim3(256), 0, st, t, part + total);
+        if (streaming) hipLaunchKernelGGL((grad_squares_kernel<true>), dim3((unsigned)parts), dim3(256), 0, st, t, part + total);
+        else hipLaunchKernelGGL((grad_squares_kernel<false>), dim3((unsigned)parts), dim3(256), 0, st, t, part + total);
         if (int rc = check_launch("aq_clip_grad_norm")) return rc;
         total += parts;
     }
@@ -211,8 +219,9 @@ int aq_clip_grad_norm(const void *const *tensors, void *const *outs, const long 
         GradTab t = {};
         const long long chunks = table(base, t);
         if (chunks == 0) continue;
-        hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)std::min<long long>(chunks, GRAD_PARTS)), dim3(256), 0, st, t, self ? part : sum,
-                           self ? (int)total : 1, max_norm, self ? norm : nullptr);
+        const dim3 g((unsigned)std::min<long long>(chunks, GRAD_PARTS));
+        if (streaming) hipLaunchKernelGGL((grad_scale_kernel<true>), g, dim3(256), 0, st, t, self ? part : sum, self ? (int)total : 1, max_norm, self ? norm : nullptr);
+        else hipLaunchKernelGGL((grad_scale_kernel<false>), g, dim3(256), 0, st, t, self ? part : sum, self ? (int)total : 1, max_norm, self ? norm : nullptr);
         if (int rc = check_launch("aq_clip_grad_norm")) return rc;
     }
     return 0;

@@ -17,16 +17,16 @@ template <typename S> __device__ inline S wave_sum(S v)
     for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
     return v;
 }
-// sum over the workgroup, the same value in every thread; sh: one element per wavefront, free to be used again on return
-template <int THREADS, typename S> __device__ inline S group_sum(S v, S *sh)
+// sum over the workgroup, the same value in every thread; sh: 16 elements, free to be used again on return
+template <typename S> __device__ inline S group_sum(S v, S *sh)
 {
     v = wave_sum(v);
-    if (THREADS == 64) return v;
+    const int waves = (int)blockDim.x / 64;
+    if (waves == 1) return v;
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     S s = sh[0];
-#pragma unroll
-    for (int i = 1; i < THREADS / 64; ++i) s += sh[i];
+    for (int i = 1; i < waves; ++i) s += sh[i];
     __syncthreads();
     return s;
 }
@@ -42,73 +42,61 @@ struct NormArgs {
     int scale_f32;
 };
 
-template <typename T> __device__ inline void norm_outputs(const NormArgs &a, long long r, long long c, int n, const float (&hv)[8], float rs)
+template <bool NT, typename T> __device__ inline void norm_outputs(const NormArgs &a, long long r, long long c, int n, const float (&hv)[8], float rs)
 {
     float wv[8], o[8];
     load_n(a.w + c, n, wv);
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j] = (hv[j] * rs) * wv[j];
-    if (a.y) store_n(static_cast<T *>(a.y) + r * a.ldy + c, n, o);
+    if (a.y) store_n<NT>(static_cast<T *>(a.y) + r * a.ldy + c, n, o);
     if (a.q) {
-        float m = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(o[j]));
-        const int e = scale_exponent(max16(m));  // 16 lanes with 8 elements each: one block
-        store_codes(a.q + r * a.ldq + c, n, e4m3x8(o, exp2_int(-e)));
+        const int e = scale_exponent(max16(amax8(o)));  // 16 lanes with 8 elements each: one block
+        store_codes<NT>(a.q + r * a.ldq + c, n, e4m3x8(o, exp2_int(-e)));
         if ((threadIdx.x & 15) == 0 && n > 0) store_scale(a.qs, r * a.ldqs + c / FP8_BLK, e, a.scale_f32);
     }
 }
 
 // one workgroup per row; a thread holds V chunks of 8 columns
-template <typename T, int THREADS, int V>
-__global__ __launch_bounds__(THREADS) void rms_norm_fwd_kernel(const NormArgs a)
+template <typename T, int V, bool NT>
+__global__ __launch_bounds__(1024) void rms_norm_fwd_kernel(const NormArgs a)
 {
-    __shared__ double sh[THREADS / 64];
+    __shared__ double sh[16];
     const long long r = blockIdx.x;
+    const int T0 = (int)blockDim.x;
     const T *x = static_cast<const T *>(a.x) + r * a.ldx, *res = static_cast<const T *>(a.res) + r * a.ldres;
-    float hv[V][8];
-    double s = 0.0;
-    const bool whole = a.cols == THREADS * V * 8;  // the same in all lanes: all loads in flight at once
-    if (whole) {
+    raw8<T> xv[V], rv[V];
+    if (a.cols == T0 * V * 8) {  // the same in all lanes: all loads in flight at once
 #pragma unroll
-        for (int i = 0; i < V; ++i) load8(x + (i * THREADS + threadIdx.x) * 8, hv[i]);
+        for (int i = 0; i < V; ++i) xv[i] = load_raw<NT>(x + (i * T0 + threadIdx.x) * 8);
+        if (a.res)
+#pragma unroll
+            for (int i = 0; i < V; ++i) rv[i] = load_raw<NT>(res + (i * T0 + threadIdx.x) * 8);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int c = (i * THREADS + threadIdx.x) * 8;
-            load_n(x + c, (int)min(8LL, a.cols - c), hv[i]);
+            const int c = (i * T0 + threadIdx.x) * 8, n = (int)min(8LL, a.cols - c);
+            xv[i] = load_raw_n(x + c, n);
+            if (a.res) rv[i] = load_raw_n(res + c, n);
         }
     }
-    if (a.res) {
-        float rv[V][8];
-        if (whole) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) load8(res + (i * THREADS + threadIdx.x) * 8, rv[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int c = (i * THREADS + threadIdx.x) * 8;
-                load_n(res + c, (int)min(8LL, a.cols - c), rv[i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) hv[i][j] = to_f32(from_f32<T>(hv[i][j] + rv[i][j]));
-    }
+    float hv[V][8];
+    double s = 0.0;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int c = (i * THREADS + threadIdx.x) * 8;
-        if (a.h) store_n(static_cast<T *>(a.h) + r * a.ldh + c, (int)min(8LL, a.cols - c), hv[i]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s = __builtin_fma((double)hv[i][j], (double)hv[i][j], s);
+        for (int j = 0; j < 8; ++j) {
+            hv[i][j] = a.res ? to_f32(from_f32<T>(value(xv[i], j) + value(rv[i], j))) : value(xv[i], j);
+            s = __builtin_fma((double)hv[i][j], (double)hv[i][j], s);
+        }
+        const int c = (i * T0 + threadIdx.x) * 8;
+        if (a.h) store_n<NT>(static_cast<T *>(a.h) + r * a.ldh + c, (int)min(8LL, a.cols - c), hv[i]);
     }
-    const float rs = (float)(1.0 / sqrt(group_sum<THREADS>(s, sh) / (double)a.cols + a.eps));
+    const float rs = (float)(1.0 / sqrt(group_sum(s, sh) / (double)a.cols + a.eps));
     if (a.rstd && threadIdx.x == 0) a.rstd[r] = rs;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int c = (i * THREADS + threadIdx.x) * 8;
-        norm_outputs<T>(a, r, c, (int)max(0LL, min(8LL, a.cols - c)), hv[i], rs);
+        const int c = (i * T0 + threadIdx.x) * 8;
+        norm_outputs<NT, T>(a, r, c, (int)max(0LL, min(8LL, a.cols - c)), hv[i], rs);
     }
 }
 
@@ -139,7 +127,7 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_long_kernel(const NormArgs 
 #pragma unroll
         for (int j = 0; j < 8; ++j) s = __builtin_fma((double)hv[j], (double)hv[j], s);
     }
-    const float rs = (float)(1.0 / sqrt(group_sum<1024>(s, sh) / (double)a.cols + a.eps));
+    const float rs = (float)(1.0 / sqrt(group_sum(s, sh) / (double)a.cols + a.eps));
     if (a.rstd && threadIdx.x == 0) a.rstd[r] = rs;
     for (long long i = 0; i < chunks; ++i) {
         const long long c = (i * 1024 + threadIdx.x) * 8;
@@ -147,7 +135,7 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_long_kernel(const NormArgs 
         float hv[8];
         if (a.h) load_n(static_cast<const T *>(h) + c, n, hv);  // (its own store: h may be x or res itself)
         else row_chunk(c, n, hv);
-        norm_outputs<T>(a, r, c, n, hv, rs);
+        norm_outputs<false, T>(a, r, c, n, hv, rs);
     }
 }
 
@@ -159,68 +147,82 @@ struct NormBwdArgs {
     long long lddy, lddh, ldh, lddx, rows, cols;
 };
 
-// A fixed number of workgroups, each over every gridDim.x-th row: the columns' partial dw stay in registers from row to row.
-template <typename T, int THREADS, int V>
-__global__ __launch_bounds__(THREADS) void rms_norm_bwd_kernel(const NormBwdArgs a)
+// A fixed number of workgroups, each over every gridDim.x-th row: the columns' partial dw stay in registers from row to row, and
+// (V = 1) a row's operands are on their way while the row before it is computed.
+template <typename T, int V, bool NT>
+__global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
 {
-    __shared__ float sh[THREADS / 64];
-    const bool whole = a.cols == THREADS * V * 8;
+    __shared__ float sh[16];
+    const int T0 = (int)blockDim.x;
+    const bool whole = a.cols == T0 * V * 8;
     float wv[V][8], acc[V][8];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int c = (i * THREADS + threadIdx.x) * 8;
+        const int c = (i * T0 + threadIdx.x) * 8;
         load_n(a.w + c, (int)max(0LL, min(8LL, a.cols - c)), wv[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
     }
     const float inv = 1.0f / (float)a.cols;
-    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    raw8<T> dyn[V], hn[V], dhn[V];
+    float rsn = 0.0f;
+    auto load = [&](long long r) {
         const T *dy = static_cast<const T *>(a.dy) + r * a.lddy, *h = static_cast<const T *>(a.h) + r * a.ldh;
         const T *dh = static_cast<const T *>(a.dh) + r * a.lddh;
-        const float rs = a.rstd[r];
-        float g[V][8], n[V][8];
+        rsn = a.rstd[r];
         if (whole) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) load8(dy + (i * THREADS + threadIdx.x) * 8, g[i]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) load8(h + (i * THREADS + threadIdx.x) * 8, n[i]);
+            for (int i = 0; i < V; ++i) {
+                const int c = (i * T0 + threadIdx.x) * 8;
+                dyn[i] = load_raw<NT>(dy + c);
+                hn[i] = load_raw<NT>(h + c);
+                if (a.dh && a.dx) dhn[i] = load_raw<NT>(dh + c);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const int c = (i * THREADS + threadIdx.x) * 8, k = (int)max(0LL, min(8LL, a.cols - c));
-                load_n(dy + c, k, g[i]);
-                load_n(h + c, k, n[i]);
+                const int c = (i * T0 + threadIdx.x) * 8, k = (int)max(0LL, min(8LL, a.cols - c));
+                dyn[i] = load_raw_n(dy + c, k);
+                hn[i] = load_raw_n(h + c, k);
+                if (a.dh && a.dx) dhn[i] = load_raw_n(dh + c, k);
             }
         }
+    };
+    if (V == 1) load(blockIdx.x);  // (the grid has no more workgroups than there are rows)
+    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        raw8<T> dyv[V], hv[V], dhv[V];
+        if (V > 1) load(r);
+        const float rs = rsn;
+#pragma unroll
+        for (int i = 0; i < V; ++i) dyv[i] = dyn[i], hv[i] = hn[i], dhv[i] = dhn[i];
+        if (V == 1 && r + gridDim.x < a.rows) load(r + gridDim.x);
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                n[i][j] *= rs;
-                acc[i][j] = __builtin_fmaf(g[i][j], n[i][j], acc[i][j]);
-                g[i][j] *= wv[i][j];
-                s = __builtin_fmaf(g[i][j], n[i][j], s);
+                const float d = value(dyv[i], j), n = value(hv[i], j) * rs;
+                acc[i][j] = __builtin_fmaf(d, n, acc[i][j]);
+                s = __builtin_fmaf(d * wv[i][j], n, s);
             }
         if (!a.dx) continue;
-        const float m = group_sum<THREADS>(s, sh) * inv;
+        const float m = group_sum(s, sh) * inv;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int c = (i * THREADS + threadIdx.x) * 8, k = (int)max(0LL, min(8LL, a.cols - c));
+            const int c = (i * T0 + threadIdx.x) * 8;
             float o[8];
-            if (a.dh) load_n(dh + c, k, o);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float d = rs * __builtin_fmaf(-n[i][j], m, g[i][j]);
-                o[j] = a.dh ? d + o[j] : d;
+                const float d = rs * __builtin_fmaf(-(value(hv[i], j) * rs), m, value(dyv[i], j) * wv[i][j]);
+                o[j] = a.dh ? d + value(dhv[i], j) : d;
             }
-            store_n(static_cast<T *>(a.dx) + r * a.lddx + c, k, o);
+            store_n<NT>(static_cast<T *>(a.dx) + r * a.lddx + c, (int)max(0LL, min(8LL, a.cols - c)), o);
         }
     }
     if (!a.part) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int c = (i * THREADS + threadIdx.x) * 8;
+        const int c = (i * T0 + threadIdx.x) * 8;
         store_n(a.part + (long long)blockIdx.x * a.cols + c, (int)max(0LL, min(8LL, a.cols - c)), acc[i]);
     }
 }
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(1024) void rms_norm_dx_long_kernel(const NormBwdArg
     const float rs = a.rstd[r];
     float s = 0.0f;
     for (long long c = threadIdx.x; c < a.cols; c += 1024) s = __builtin_fmaf(to_f32(dy[c]) * a.w[c], to_f32(h[c]) * rs, s);
-    const float m = group_sum<1024>(s, sh) / (float)a.cols;
+    const float m = group_sum(s, sh) / (float)a.cols;
     for (long long c = threadIdx.x; c < a.cols; c += 1024) {
         const float d = rs * __builtin_fmaf(-to_f32(h[c]) * rs, m, to_f32(dy[c]) * a.w[c]);
         static_cast<T *>(a.dx)[r * a.lddx + c] = from_f32<T>(a.dh ? d + to_f32(dh[c]) : d);
@@ -272,31 +274,10 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float *__restri
     dw[c] = (float)s;
 }
 
-constexpr long long NORM_LONG = 1024 * 4 * 8;  // columns that fit the registers of a workgroup
-// calls f(threads, chunks per thread) with the smallest shape that holds a row
-template <typename F> inline void norm_shape(long long cols, F f)
-{
-    using std::integral_constant;
-    if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    else if (cols <= 1024) f(integral_constant<int, 128>{}, integral_constant<int, 1>{});
-    else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-    else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    else if (cols <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-    else if (cols <= 16384) f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-    else f(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
-}
-constexpr long long NORM_BWD_LONG = 1024 * 2 * 8;
-// the backward kernel holds four arrays of a row, so more threads with fewer chunks each
-template <typename F> inline void norm_bwd_shape(long long cols, F f)
-{
-    using std::integral_constant;
-    if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    else if (cols <= 1024) f(integral_constant<int, 128>{}, integral_constant<int, 1>{});
-    else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-    else if (cols <= 4096) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
-    else if (cols <= 8192) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
-    else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
-}
+constexpr long long NORM_LONG = 1024 * 4 * 8, NORM_BWD_LONG = 1024 * 2 * 8;  // columns that fit the registers of a workgroup
+// threads for `cols` columns in chunks of 8, v of them a thread: whole wavefronts
+static unsigned norm_threads(long long cols, int v) { return (unsigned)((cols + 8 * v - 1) / (8 * v) + 63) / 64 * 64; }
+
 // workgroups of the backward kernel (= rows of partial dw)
 static int norm_parts(long long rows, long long cols) { return (int)std::min<long long>(rows, cols > NORM_BWD_LONG ? 64 : cols <= 1024 ? 2048 : 512); }
 
@@ -325,9 +306,18 @@ int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldr
             hipLaunchKernelGGL((rms_norm_fwd_long_kernel<T>), dim3((unsigned)rows), dim3(1024), 0, st, a);
             return 0;
         }
-        norm_shape(cols, [&](auto threads, auto v) {
-            hipLaunchKernelGGL((rms_norm_fwd_kernel<T, decltype(threads)::value, decltype(v)::value>), dim3((unsigned)rows), dim3(decltype(threads)::value), 0, st, a);
-        });
+        // few chunks a thread while a workgroup stays small enough to have several of them on a compute unit
+        const long long each = cols * type_size(type);
+        const bool stream = rows * (each + (res ? each : 0) + (h ? each : 0) + (y ? each : 0) + (q ? cols : 0)) > LAST_LEVEL_CACHE;
+        const dim3 g((unsigned)rows);
+        auto launch = [&](auto v) {
+            constexpr int V = decltype(v)::value;
+            if (stream) hipLaunchKernelGGL((rms_norm_fwd_kernel<T, V, true>), g, dim3(norm_threads(cols, V)), 0, st, a);
+            else hipLaunchKernelGGL((rms_norm_fwd_kernel<T, V, false>), g, dim3(norm_threads(cols, V)), 0, st, a);
+        };
+        if (cols <= 256 * 8) launch(std::integral_constant<int, 1>{});
+        else if (cols <= 512 * 2 * 8) launch(std::integral_constant<int, 2>{});
+        else launch(std::integral_constant<int, 4>{});
         return 0;
     });
     return check_launch("aq_rms_norm_fwd");
@@ -365,10 +355,15 @@ int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long ld
                 if (dw) hipLaunchKernelGGL((rms_norm_dw_long_kernel<T>), dim3((unsigned)((cols + 255) / 256 * parts)), dim3(256), 0, st, a, parts);
                 return 0;
             }
-            norm_bwd_shape(cols, [&](auto threads, auto v) {
-                hipLaunchKernelGGL((rms_norm_bwd_kernel<T, decltype(threads)::value, decltype(v)::value>), dim3((unsigned)parts),
-                                   dim3(decltype(threads)::value), 0, st, a);
-            });
+            const long long each = cols * type_size(type);
+            const bool stream = rows * (2 * each + (dh ? each : 0) + (dx ? each : 0)) > LAST_LEVEL_CACHE;
+            auto launch = [&](auto v) {
+                constexpr int V = decltype(v)::value;
+                if (stream) hipLaunchKernelGGL((rms_norm_bwd_kernel<T, V, true>), dim3((unsigned)parts), dim3(norm_threads(cols, V)), 0, st, a);
+                else hipLaunchKernelGGL((rms_norm_bwd_kernel<T, V, false>), dim3((unsigned)parts), dim3(norm_threads(cols, V)), 0, st, a);
+            };
+            if (cols <= 1024 * 8) launch(std::integral_constant<int, 1>{});
+            else launch(std::integral_constant<int, 2>{});
             return 0;
         });
         if (int rc = check_launch("aq_rms_norm_bwd")) return rc;
