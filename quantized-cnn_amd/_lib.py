@@ -186,8 +186,8 @@ def lib():
         L.aq_rms_norm_fwd.argtypes = [vp, ll, vp, ll, i, vp, ll, ll, C.c_double, vp, ll, vp, ll, vp, ll, i, vp, ll, vp, vp]
         L.aq_rms_norm_bwd_workspace_bytes.argtypes = [ll, ll]
         L.aq_rms_norm_bwd.argtypes = [vp, ll, vp, ll, vp, ll, i, vp, vp, ll, ll, vp, ll, vp, vp, sz, vp]
-        L.aq_clip_grad_norm_workspace_bytes.argtypes = [C.POINTER(ll), i]
-        L.aq_clip_grad_norm.argtypes = [C.POINTER(vp), C.POINTER(vp), C.POINTER(ll), C.POINTER(i), i, C.c_double, vp, vp, sz, vp]
+        L.aq_clip_grad_norm_workspace_bytes.argtypes = [vp, i]  # (arrays on the host, by address)
+        L.aq_clip_grad_norm.argtypes = [vp, vp, vp, vp, i, C.c_double, vp, vp, sz, vp]
         for name in ("aq_fp8_quantize_workspace_bytes", "aq_fp8_matmul_workspace_bytes", "aq_rms_norm_bwd_workspace_bytes",
                      "aq_clip_grad_norm_workspace_bytes"):
             getattr(L, name).restype = sz

@@ -125,7 +125,9 @@ template <bool NT, typename T> __device__ inline void store8_any(T *p, const flo
 {
     store_any<NT>(u4_t{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])}, reinterpret_cast<u4_any *>(p));
 }
-constexpr long long LAST_LEVEL_CACHE = 256LL << 20;  // bytes
+// Calls that move more than this many bytes (half the last-level cache, the rest being what other kernels have there) stream.
+// Measured at 134 + 134 MB of the quantiser: 66 us with plain accesses, 57 us streaming; at 34 + 34 MB no difference.
+constexpr long long STREAM_BYTES = 128LL << 20;
 
 // the first n (0..8) of eight elements; the others read as zero and are not written
 template <typename T> __device__ inline void load_n(const T *p, int n, float (&v)[8])

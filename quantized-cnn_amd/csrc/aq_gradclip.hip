@@ -199,7 +199,7 @@ int aq_clip_grad_norm(const void *const *tensors, void *const *outs, const long 
     };
     long long total = 0, bytes = 0;
     for (int i = 0; i < n; ++i) bytes += sizes[i] * type_size(types[i]);
-    const bool streaming = bytes > LAST_LEVEL_CACHE;
+    const bool streaming = bytes > STREAM_BYTES;
     for (int base = 0; base < n; base += GRAD_MAX) {
         GradTab t = {};
         AQ_REQUIRE(table(base, t) < (1LL << 31) - GRAD_PARTS, -E2BIG, "aq_clip_grad_norm: too many elements");

@@ -308,7 +308,7 @@ int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldr
         }
         // few chunks a thread while a workgroup stays small enough to have several of them on a compute unit
         const long long each = cols * type_size(type);
-        const bool stream = rows * (each + (res ? each : 0) + (h ? each : 0) + (y ? each : 0) + (q ? cols : 0)) > LAST_LEVEL_CACHE;
+        const bool stream = rows * (each + (res ? each : 0) + (h ? each : 0) + (y ? each : 0) + (q ? cols : 0)) > STREAM_BYTES;
         const dim3 g((unsigned)rows);
         auto launch = [&](auto v) {
             constexpr int V = decltype(v)::value;
@@ -356,7 +356,7 @@ int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long ld
                 return 0;
             }
             const long long each = cols * type_size(type);
-            const bool stream = rows * (2 * each + (dh ? each : 0) + (dx ? each : 0)) > LAST_LEVEL_CACHE;
+            const bool stream = rows * (2 * each + (dh ? each : 0) + (dx ? each : 0)) > STREAM_BYTES;
             auto launch = [&](auto v) {
                 constexpr int V = decltype(v)::value;
                 if (stream) hipLaunchKernelGGL((rms_norm_bwd_kernel<T, V, true>), dim3((unsigned)parts), dim3(norm_threads(cols, V)), 0, st, a);

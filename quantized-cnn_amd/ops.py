@@ -3,6 +3,7 @@
 Every function launches on torch's current HIP stream, allocates its outputs and workspace through
 torch's caching allocator (so calls are capturable in a HIP graph), and never synchronises.
 """
+import array
 import ctypes as C
 import functools
 
@@ -913,7 +914,7 @@ def _on_device(f):
     @functools.wraps(f)
     def call(first, *args, **kw):
         d = first.device if isinstance(first, (torch.Tensor, Fp8Blocks)) else first[0].device if len(first) else None
-        if d is None or d.type != "cuda" or d.index == torch.cuda.current_device():
+        if d is None or d.type != "cuda" or d.index == torch._C._cuda_getDevice():
             return f(first, *args, **kw)
         with torch.cuda.device(d):
             return f(first, *args, **kw)
@@ -958,7 +959,7 @@ class Fp8Blocks:
     start at multiples of 16 bytes, or the last one ends within such a piece at the end of its storage, it first copies the
     codes (those of `fp8_quantize` never need it)."""
 
-    __slots__ = ("data", "scale", "block_rows", "shape", "device", "_ld", "_lds", "_scale_type")
+    __slots__ = ("_data", "_scale", "_buf", "_soff", "block_rows", "shape", "device", "_ld", "_lds", "_scale_type")
 
     def __init__(self, data, scale, block_rows=1):
         if not isinstance(data, torch.Tensor) or not isinstance(scale, torch.Tensor) or data.dim() != 2 or scale.dim() != 2:
@@ -973,13 +974,41 @@ class Fp8Blocks:
         if scale.shape != (-(-rows // block_rows), -(-cols // FP8_BLOCK)):
             raise ValueError("Fp8Blocks: scale %s does not belong to data %s in blocks of %d x %d" % (
                 tuple(scale.shape), (rows, cols), block_rows, FP8_BLOCK))
-        self.data, self.scale, self.block_rows, self.shape, self.device = data, scale, block_rows, (rows, cols), data.device
+        self._data, self._scale, self._buf, self.block_rows, self.shape, self.device = data, scale, None, block_rows, (rows, cols), data.device
         self._ld, self._lds = _pitch(data, "data"), _pitch(scale, "scale")
         self._scale_type = _SCALE_TYPES[scale.dtype]
 
+    @property
+    def scale_dtype(self):
+        return torch.float32 if self._scale_type == _lib.SCALE_F32 else torch.float8_e8m0fnu
+
+    # codes and scales made here lie in one buffer; their views are made when they are asked for
+    @property
+    def data(self):
+        if self._data is None:
+            rows, cols = self.shape
+            self._data = self._buf[:rows * self._ld].view(torch.float8_e4m3fn).view(rows, self._ld)[:, :cols]
+        return self._data
+
+    @property
+    def scale(self):
+        if self._scale is None:
+            rows, nb = -(-self.shape[0] // self.block_rows), -(-self.shape[1] // FP8_BLOCK)
+            dt = self.scale_dtype
+            self._scale = self._buf[self._soff:self._soff + rows * self._lds * dt.itemsize].view(dt).view(rows, self._lds)[:, :nb]
+        return self._scale
+
+    def _ptrs(self):
+        if self._buf is not None:
+            p = self._buf.data_ptr()
+            return p, p + self._soff
+        return self._data.data_ptr(), self._scale.data_ptr()
+
     def _by16(self):
         """Codes whose rows can be read 16 bytes at a time up to their last: (tensor to keep alive, address, pitch)."""
-        d, cols = self.data, self.shape[1]
+        if self._buf is not None:
+            return self._buf, self._buf.data_ptr(), self._ld
+        d, cols = self._data, self.shape[1]
         p = d.data_ptr()
         if self._ld % 16 == 0 and p % 16 == 0 and (cols % 16 == 0 or d.storage_offset() + (self.shape[0] - 1) * self._ld + _up(cols, 16)
                                                    <= d.untyped_storage().nbytes()):
@@ -993,18 +1022,15 @@ def _up(n, m):
     return (n + m - 1) // m * m
 
 
-def _new_blocks(rows, cols, block_rows, scale_dtype, device):
+def _new_blocks(rows, cols, block_rows, scale_type, device):
     """Uninitialised storage: rows of codes start at multiples of 16 bytes, rows of scales at multiples of 4 elements."""
     b = Fp8Blocks.__new__(Fp8Blocks)
-    ld, nb = _up(cols, 16), -(-cols // FP8_BLOCK)
-    lds = _up(nb, 4)
-    b.data = torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)
-    if ld != cols:
-        b.data = b.data[:, :cols]
-    b.scale = torch.empty((rows if block_rows == 1 else -(-rows // block_rows), lds), dtype=scale_dtype, device=device)
-    if lds != nb:
-        b.scale = b.scale[:, :nb]
-    b.block_rows, b.shape, b.device, b._ld, b._lds, b._scale_type = block_rows, (rows, cols), device, ld, lds, _SCALE_TYPES[scale_dtype]
+    ld, lds = (cols + 15) & ~15, (cols + 511) // 512 * 4
+    soff = rows * ld
+    srows = rows if block_rows == 1 else (rows + 127) // 128
+    b._buf = torch.empty(soff + srows * lds * (4 if scale_type else 1), dtype=torch.uint8, device=device)
+    b._data = b._scale = None
+    b._soff, b.block_rows, b.shape, b.device, b._ld, b._lds, b._scale_type = soff, block_rows, (rows, cols), device, ld, lds, scale_type
     return b
 
 
@@ -1034,8 +1060,8 @@ def fp8_quantize(x, forms="rows", block_rows=1, scale_dtype=torch.float8_e8m0fnu
         raise ValueError("fp8_quantize: column sums come with the transposed form in 1 x 128 blocks only")
     rows, cols = x.shape
     dev = x.device
-    q = _new_blocks(rows, cols, block_rows, scale_dtype, dev) if forms != "cols" else None
-    qt = _new_blocks(cols, rows, block_rows, scale_dtype, dev) if forms != "rows" else None
+    q = _new_blocks(rows, cols, block_rows, st, dev) if forms != "cols" else None
+    qt = _new_blocks(cols, rows, block_rows, st, dev) if forms != "rows" else None
     sums = ws = None
     nbytes = 0
     if colsum:
@@ -1043,11 +1069,11 @@ def fp8_quantize(x, forms="rows", block_rows=1, scale_dtype=torch.float8_e8m0fnu
         nbytes = _lib.lib().aq_fp8_quantize_workspace_bytes(rows, cols)
         ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
     if cols and (rows or colsum):
+        pq, ps = q._ptrs() if q is not None else (None, None)
+        pt, pts = qt._ptrs() if qt is not None else (None, None)
         _lib.check(_lib.lib().aq_fp8_quantize(
-            x.data_ptr(), _lib.ELEMENT_TYPES[x.dtype], rows, cols, ldx,
-            q.data.data_ptr() if q else None, q._ld if q else 0, q.scale.data_ptr() if q else None, q._lds if q else 0,
-            qt.data.data_ptr() if qt else None, qt._ld if qt else 0, qt.scale.data_ptr() if qt else None, qt._lds if qt else 0,
-            block_rows, st, sums.data_ptr() if colsum else None, ws.data_ptr() if colsum else None, nbytes, _stream_of(dev)))
+            x.data_ptr(), _lib.ELEMENT_TYPES[x.dtype], rows, cols, ldx, pq, q._ld if pq else 0, ps, q._lds if pq else 0, pt, qt._ld if pt else 0, pts,
+            qt._lds if pt else 0, block_rows, st, sums.data_ptr() if colsum else None, ws.data_ptr() if colsum else None, nbytes, _stream_of(dev)))
     out = (q,) if forms == "rows" else (qt,) if forms == "cols" else (q, qt)
     if colsum:
         out += (sums,)
@@ -1059,10 +1085,11 @@ def fp8_transpose(q):
     """Fp8Blocks of the transposed matrix.  Tiles of 128 x 128 keep their codes; 1 x 128 blocks are formed anew along the other axis
     (exact but for values below the new block's smallest subnormal step)."""
     rows, cols = q.shape
-    t = _new_blocks(cols, rows, q.block_rows, q.scale.dtype, q.device)
+    t = _new_blocks(cols, rows, q.block_rows, q._scale_type, q.device)
     if rows and cols:
-        _lib.check(_lib.lib().aq_fp8_transpose(q.data.data_ptr(), q._ld, q.scale.data_ptr(), q._lds, rows, cols, t.data.data_ptr(), t._ld,
-                                               t.scale.data_ptr(), t._lds, q.block_rows, q._scale_type, _stream_of(q.device)))
+        pq, ps = q._ptrs()
+        pt, pts = t._ptrs()
+        _lib.check(_lib.lib().aq_fp8_transpose(pq, q._ld, ps, q._lds, rows, cols, pt, t._ld, pts, t._lds, q.block_rows, q._scale_type, _stream_of(q.device)))
     return t
 
 
@@ -1074,8 +1101,9 @@ def fp8_dequantize(q, dtype=torch.bfloat16):
     rows, cols = q.shape
     y = torch.empty((rows, cols), dtype=dtype, device=q.device)
     if rows and cols:
-        _lib.check(_lib.lib().aq_fp8_dequantize(q.data.data_ptr(), q._ld, q.scale.data_ptr(), q._lds, rows, cols, q.block_rows, q._scale_type,
-                                                y.data_ptr(), _lib.ELEMENT_TYPES[dtype], cols, _stream_of(q.device)))
+        pq, ps = q._ptrs()
+        _lib.check(_lib.lib().aq_fp8_dequantize(pq, q._ld, ps, q._lds, rows, cols, q.block_rows, q._scale_type, y.data_ptr(), _lib.ELEMENT_TYPES[dtype],
+                                                cols, _stream_of(q.device)))
     return y
 
 
@@ -1090,7 +1118,7 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     dev = a.device
     if b.shape[1] != K or b.device != dev or a._scale_type != b._scale_type:
         raise ValueError("fp8_matmul: a %s with %s scales on %s, b %s with %s scales on %s" % (
-            a.shape, a.scale.dtype, dev, b.shape, b.scale.dtype, b.device))
+            a.shape, a.scale_dtype, dev, b.shape, b.scale_dtype, b.device))
     if out_dtype not in _lib.ELEMENT_TYPES:
         raise ValueError("fp8_matmul: out_dtype %s, expected float32, bfloat16 or float16" % (out_dtype,))
     if bias is not None:
@@ -1108,7 +1136,7 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     db, pb, ldb = b._by16()
     nbytes = L.aq_fp8_matmul_workspace_bytes(M, N, K)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _lib.check(L.aq_fp8_matmul(pa, lda, a.scale.data_ptr(), a._lds, a.block_rows, pb, ldb, b.scale.data_ptr(), b._lds, b.block_rows, M, N, K,
+    _lib.check(L.aq_fp8_matmul(pa, lda, a._ptrs()[1], a._lds, a.block_rows, pb, ldb, b._ptrs()[1], b._lds, b.block_rows, M, N, K,
                                a._scale_type, bias.data_ptr() if bias is not None else None, y.data_ptr(), _lib.ELEMENT_TYPES[out_dtype], N,
                                ws.data_ptr() if nbytes else None, nbytes, _stream_of(dev)))
     return y
@@ -1135,15 +1163,15 @@ def rms_norm_forward(x, weight, residual=None, eps=1e-6, quantize=False, scale_d
     ldr = _matrix(residual, "residual", dev, x.dtype, x.shape) if residual is not None else 0
     w = _norm_vector(weight, cols, "weight", dev)
     st = _scale_dtype(scale_dtype)
-    y = _new_blocks(rows, cols, 1, scale_dtype, dev) if quantize else torch.empty((rows, cols), dtype=x.dtype, device=dev)
+    y = _new_blocks(rows, cols, 1, st, dev) if quantize else torch.empty((rows, cols), dtype=x.dtype, device=dev)
     h = torch.empty((rows, cols), dtype=x.dtype, device=dev) if residual is not None else x
     rstd = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows:
+        pq, ps = y._ptrs() if quantize else (None, None)
         _lib.check(_lib.lib().aq_rms_norm_fwd(
             x.data_ptr(), ldx, residual.data_ptr() if residual is not None else None, ldr, _lib.ELEMENT_TYPES[x.dtype], w, rows, cols, eps,
-            None if quantize else y.data_ptr(), cols, y.data.data_ptr() if quantize else None, y._ld if quantize else 0,
-            y.scale.data_ptr() if quantize else None, y._lds if quantize else 0, st, h.data_ptr() if residual is not None else None, cols,
-            rstd.data_ptr(), _stream_of(dev)))
+            None if quantize else y.data_ptr(), cols, pq, y._ld if quantize else 0, ps, y._lds if quantize else 0, st,
+            h.data_ptr() if residual is not None else None, cols, rstd.data_ptr(), _stream_of(dev)))
     return y, h, rstd
 
 
@@ -1176,26 +1204,31 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dx=True, need_dweight=T
 # ------------------------------------------------------------------- gradient norm over all tensors
 
 def _grad_lists(tensors):
-    dev = tensors[0].device if tensors else None
-    for i, t in enumerate(tensors):
-        if not t.is_cuda:
+    """(addresses, sizes, types) of a list of gradients as arrays, and their device; checked in bulk, a training step has many."""
+    dev = tensors[0].device
+    ptrs = array.array("q", [t.data_ptr() for t in tensors])
+    sizes = array.array("q", [t.numel() for t in tensors])
+    try:
+        types = array.array("i", [_lib.ELEMENT_TYPES[t.dtype] for t in tensors])
+    except KeyError:
+        types = None
+    if types is None or not all([t.is_contiguous() for t in tensors]) or len({t.get_device() for t in tensors}) != 1 or dev.type != "cuda":
+        for i, t in enumerate(tensors):
             _hip(t, "tensor[%d]" % i)
-        if t.device != dev or t.dtype not in _lib.ELEMENT_TYPES or not t.is_contiguous():
-            raise ValueError("tensor[%d]: %s on %s, strides %s: contiguous float32, bfloat16 or float16 tensors of one device are expected" % (
-                i, t.dtype, t.device, t.stride()))
-    n = len(tensors)
-    return (C.c_void_p * n)(*[t.data_ptr() for t in tensors]), (C.c_longlong * n)(*[t.numel() for t in tensors]), \
-        (C.c_int * n)(*[_lib.ELEMENT_TYPES[t.dtype] for t in tensors]), dev
+            if t.device != dev or t.dtype not in _lib.ELEMENT_TYPES or not t.is_contiguous():
+                raise ValueError("tensor[%d]: %s on %s, strides %s: contiguous float32, bfloat16 or float16 tensors of one device are expected" % (
+                    i, t.dtype, t.device, t.stride()))
+    return ptrs, sizes, types, dev
 
 
-def _grad_norm(tensors, outs, max_norm):
-    ptrs, sizes, types, dev = _grad_lists(tensors)
-    n = len(tensors)
+def _grad_norm(ptrs, outs, sizes, types, dev, max_norm):
     L = _lib.lib()
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = L.aq_clip_grad_norm_workspace_bytes(sizes, n)
+    n, at = len(ptrs), sizes.buffer_info()[0]
+    nbytes = L.aq_clip_grad_norm_workspace_bytes(at, n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _lib.check(L.aq_clip_grad_norm(ptrs, outs, sizes, types, n, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes, _stream_of(dev)))
+    _lib.check(L.aq_clip_grad_norm(ptrs.buffer_info()[0], outs.buffer_info()[0] if outs is not None else None, at, types.buffer_info()[0], n, max_norm,
+                                   norm.data_ptr(), ws.data_ptr(), nbytes, _stream_of(dev)))
     return norm
 
 
@@ -1204,27 +1237,31 @@ def grad_norm(tensors):
     """sqrt(sum of squares of all elements of all tensors), fp32 0-dim device tensor (sums in double)."""
     if len(tensors) == 0:
         raise ValueError("grad_norm: the list of tensors is empty")
-    return _grad_norm(tensors, None, 0.0)
+    ptrs, sizes, types, dev = _grad_lists(tensors)
+    return _grad_norm(ptrs, None, sizes, types, dev, 0.0)
 
 
 @_on_device
 def clip_grad_norm(tensors, max_norm, out=None):
     """Scales all tensors by min(1, max_norm / (norm + 1e-6)), norm = sqrt(sum of squares of all their elements): in place, or into
-    the tensors of `out` (same shapes and types).  -> norm, fp32 0-dim device tensor.  The host does not wait; a NaN makes
-    everything NaN, an infinity makes the finite elements 0.  Two launches per 64 tensors."""
+    the tensors of `out` (as many elements, of the same types).  -> norm, fp32 0-dim device tensor.  The host does not wait; a NaN
+    makes everything NaN, an infinity makes the finite elements 0.  Two launches per 64 tensors.  No two of the tensors may
+    share memory, nor an output with another one's tensor."""
     if len(tensors) == 0:
         raise ValueError("clip_grad_norm: the list of tensors is empty")
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("clip_grad_norm: max_norm %r" % max_norm)
-    seen = {t.data_ptr() for t in tensors if t.numel()}
-    if len(seen) != sum(1 for t in tensors if t.numel()):
+    ptrs, sizes, types, dev = _grad_lists(tensors)
+    if len(set(ptrs)) != len(ptrs) and len({p for p, n in zip(ptrs, sizes) if n}) != sum(1 for n in sizes if n):
         raise ValueError("clip_grad_norm: a tensor is in the list twice")
     if out is None:
-        return _grad_norm(tensors, (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors]), max_norm)
+        return _grad_norm(ptrs, ptrs, sizes, types, dev, max_norm)
     if len(out) != len(tensors):
         raise ValueError("clip_grad_norm: %d outputs for %d tensors" % (len(out), len(tensors)))
-    for i, (o, t) in enumerate(zip(out, tensors)):
-        if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or not o.is_contiguous():
-            raise ValueError("clip_grad_norm: out[%d] does not match its tensor" % i)
-    return _grad_norm(tensors, (C.c_void_p * len(out))(*[o.data_ptr() for o in out]), max_norm)
+    optrs, osizes, otypes, odev = _grad_lists(out)
+    if osizes != sizes or otypes != types or odev != dev:
+        raise ValueError("clip_grad_norm: the tensors of out do not match those of the list in size, type or device")
+    if len(set(optrs)) != len(optrs) and len({p for p, n in zip(optrs, sizes) if n}) != sum(1 for n in sizes if n):
+        raise ValueError("clip_grad_norm: a tensor is in out twice")
+    return _grad_norm(ptrs, optrs, sizes, types, dev, max_norm)
