@@ -93,7 +93,7 @@ template <typename T> __device__ inline void store4(T *p, int n, const f4_t &v)
 
 typedef float f16_t __attribute__((ext_vector_type(16)));
 
-// 64 lanes x 16 bytes (or one byte, widened to four) from base + off (per lane) to LDS address lds + 16 * lane (4 * lane).  Inline,
+// 64 lanes x 16 bytes (or one byte, widened to four, or four) from base + off (per lane) to LDS address lds + 16 * lane (4 * lane).  Inline,
 // because the compiler would wait for every such load before any LDS read that follows; the wait is written where the
 // pipeline needs it.
 __device__ inline void load_to_lds(uint32_t lds, uint32_t off, const uint8_t *base)
@@ -103,6 +103,10 @@ __device__ inline void load_to_lds(uint32_t lds, uint32_t off, const uint8_t *ba
 __device__ inline void load_byte_to_lds(uint32_t lds, uint32_t off, const uint8_t *base)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ inline void load_word_to_lds(uint32_t lds, uint32_t off, const uint8_t *base)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 template <typename P> __device__ inline uint32_t lds_address(P *p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) P *)p; }
 
@@ -349,10 +353,9 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
     }
 }
 
-// Large products whose blocks pass through fp32 (FP32S, EXACT): the tile's blocks of K in two stages of LDS as above; per block and pair of
-// fragments the block's sum from zero, then acc += sum * (sA * sB).  EXACT takes each fragment's codes through fp16.
-// BTILE: B's scales are of 128 x 128 tiles, one for the 32 columns of a fragment; otherwise one for each column.
-template <int BM, int BN, int WM, int WN, int MODE, bool BTILE, typename T>
+// Large products with scales of any value and fp32 outputs: the tile's blocks of K in two stages of LDS as above; per block and pair of
+// fragments the block's sum from zero, through fp16, then acc += sum * (sA * sB).
+template <int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kernel(const MatArgs p)
 {
     constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -385,7 +388,7 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
     long long sfirst = 0;
     if (tid < BM) ssrc = p.as, sfirst = (long long)((m0 + tid) >> p.ashift) * p.ldas;
     else if (tid < BM + BN) ssrc = p.bs, sfirst = (long long)((n0 + tid - BM) >> p.bshift) * p.ldbs;
-    auto read_scale = [&](int kb) { return tid < BM + BN ? load_scale(ssrc, sfirst + kb, p.scale_f32) : 0.0f; };
+    auto read_scale = [&](int kb) { return tid < BM + BN ? static_cast<const float *>(ssrc)[sfirst + kb] : 0.0f; };
 
     f16_t acc[TM][TN];
 #pragma unroll
@@ -396,9 +399,8 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
     const int row = lane & 31, gg = lane >> 5;
     const int o = row * FP8_BLK + ((gg ^ (row >> 1 & 7)) * 16);
-    constexpr int W = MODE == EXACT ? 4 : 1;  // matrix instructions of a half block
-    union half_t {
-        i8_t codes;
+    constexpr int W = 4;  // matrix instructions of a half block
+    struct half_t {
         h8_t fp16[W];
     };
     auto read_half = [&](const uint8_t *t, int kb, int h, bool tail) {
@@ -407,16 +409,7 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
             lo = mask16(lo, kb * FP8_BLK + 64 * h + 16 * gg, p.K);
             hi = mask16(hi, kb * FP8_BLK + 64 * h + 16 * gg + 32, p.K);
         }
-        half_t v;
-        if (MODE == EXACT) {
-            v.fp16[0] = codes_to_fp16(lo[0], lo[1]);
-            v.fp16[W > 1 ? 1 : 0] = codes_to_fp16(lo[2], lo[3]);
-            v.fp16[W > 1 ? 2 : 0] = codes_to_fp16(hi[0], hi[1]);
-            v.fp16[W > 1 ? 3 : 0] = codes_to_fp16(hi[2], hi[3]);
-        } else {
-            v.codes = i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        }
-        return v;
+        return half_t{{codes_to_fp16(lo[0], lo[1]), codes_to_fp16(lo[2], lo[3]), codes_to_fp16(hi[0], hi[1]), codes_to_fp16(hi[2], hi[3])}};
     };
     auto block = [&](int kb, int stage, bool tail) {
         const uint8_t *ta = tile + stage * STAGE + wm * FP8_BLK, *tb = tile + stage * STAGE + (BM + wn) * FP8_BLK;
@@ -436,38 +429,21 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sum[i][e] = 0.0f;
-            if constexpr (MODE == EXACT) {
 #pragma unroll
-                for (int w = 0; w < W; ++w)
+            for (int w = 0; w < W; ++w)
 #pragma unroll
-                    for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b0.fp16[w], a[i][0].fp16[w], sum[i], 0, 0, 0);
+                for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b0.fp16[w], a[i][0].fp16[w], sum[i], 0, 0, 0);
 #pragma unroll
-                for (int w = 0; w < W; ++w)
+            for (int w = 0; w < W; ++w)
 #pragma unroll
-                    for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b1.fp16[w], a[i][1].fp16[w], sum[i], 0, 0, 0);
-            } else {
+                for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b1.fp16[w], a[i][1].fp16[w], sum[i], 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b0.codes, a[i][0].codes, sum[i], 0, 0, 0, 127, 0, 127);
+            for (int q = 0; q < 4; ++q) {
+                const f4_t sb = *reinterpret_cast<const f4_t *>(&scale[stage][BM + wn + 32 * j + 8 * q + 4 * gg]);
 #pragma unroll
-                for (int i = 0; i < TM; ++i) sum[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b1.codes, a[i][1].codes, sum[i], 0, 0, 0, 127, 0, 127);
-            }
-            if (BTILE) {
-                const float sb = scale[stage][BM + wn + 32 * j];
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int i = 0; i < TM; ++i) {
-                    const float s = sa[i] * sb;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(sum[i][e], s, acc[i][j][e]);
-                }
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f4_t sb = *reinterpret_cast<const f4_t *>(&scale[stage][BM + wn + 32 * j + 8 * q + 4 * gg]);
-#pragma unroll
-                    for (int i = 0; i < TM; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = __builtin_fmaf(sum[i][4 * q + e], sa[i] * sb[e], acc[i][j][4 * q + e]);
-                }
+                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = __builtin_fmaf(sum[i][4 * q + e], sa[i] * sb[e], acc[i][j][4 * q + e]);
             }
         }
     };
@@ -490,7 +466,7 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
-    T *y = static_cast<T *>(p.y);
+    float *y = static_cast<float *>(p.y);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -505,6 +481,177 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
                 const f4_t v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                 store4(y + (long long)(m0 + wm + 32 * i + row) * p.ldy + n, 4, v + bias);
             }
+        }
+}
+
+// Large products with scales of any value and 16-bit outputs: tiles of 128 x 256, eight wavefronts with 64 x 64 each, LDS, loads and reads
+// as in fp8_matmul_large_kernel.  A block's sums start from zero in half 0 and are complete after half 1; they are scaled into the
+// accumulators in half 0 of the next block, each right before its registers are needed again, while the matrix instruction of
+// the one before runs.  BTILE: B's scales are of 128 x 128 tiles, one for the 32 columns of a fragment (tiles start at multiples of 32
+// columns: the last one of a row reaches past N, reads row N - 1 there and stores nothing).
+template <bool BTILE, typename T>
+__global__ __launch_bounds__(512, 2) void fp8_matmul_scaled_kernel(const MatArgs p)
+{
+    constexpr int BM = 128, BN = 256, WAVES = 8, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
+    __shared__ __attribute__((aligned(128))) uint8_t tile[2 * STAGE];
+    __shared__ __attribute__((aligned(16))) float scale[4][WAVES * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tm, tn;
+    tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
+    const int m0 = min(tm * BM, p.M - BM), n0 = min(tn * BN, (p.N + 31) / 32 * 32 - BN);
+    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK, kround = (p.K + 15) & ~15, whole = p.K / FP8_BLK;
+
+    const int chunk = ((lane & 7) ^ (4 * (wave & 1) + (lane >> 4))) * 16;
+    const uint32_t aoff = (uint32_t)(lane >> 3) * (uint32_t)p.lda;
+    const uint8_t *abase = p.a + (long long)(m0 + wave * 8) * p.lda, *bbase = p.b + (long long)n0 * p.ldb;
+    const int brow = wave * 8 + (lane >> 3), blast = p.N - 1 - n0;
+    const uint32_t lds0 = lds_address(tile) + wave * 1024;
+    auto fetch = [&](int i, int kb, int stage) {
+        const int k = kb * FP8_BLK, r = i * WAVES * 8;
+        const uint32_t c = k + chunk < kround ? chunk : 0;
+        if (r < BM) load_to_lds(lds0 + stage * STAGE + r * FP8_BLK, aoff + c, abase + (long long)r * p.lda + k);
+        else load_to_lds(lds0 + stage * STAGE + r * FP8_BLK, (uint32_t)min(r - BM + brow, blast) * (uint32_t)p.ldb + c, bbase + k);
+    };
+    // 64 scales for each of the first six wavefronts (the others load some again, to a place that nobody reads)
+    const int srow = min(wave * 64, BM + BN - 64);
+    const int sfirst = srow < BM ? m0 + srow : n0 + srow - BM, sshift = srow < BM ? p.ashift : p.bshift;
+    const long long sld = srow < BM ? p.ldas : p.ldbs;
+    const int slast = (srow < BM ? p.M : p.N) - 1;
+    const uint8_t *sbase = reinterpret_cast<const uint8_t *>(static_cast<const float *>(srow < BM ? p.as : p.bs) + (long long)(min(sfirst, slast) >> sshift) * sld);
+    const uint32_t soff = (uint32_t)((min(sfirst + lane, slast) >> sshift) - (min(sfirst, slast) >> sshift)) * (uint32_t)sld * 4;
+    const uint32_t slds0 = lds_address(&scale[0][0]) + wave * 256;
+    auto fetch_scales = [&](int kb) { load_word_to_lds(slds0 + (kb & 3) * WAVES * 256, soff, sbase + (long long)min(kb, nkb - 1) * 4); };
+    f16_t acc[2][2], sum[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = sum[i][j][e] = 0.0f;
+    const int row = lane & 31, gg = lane >> 5;
+    const uint32_t o = row * FP8_BLK + ((gg ^ (row >> 1 & 7)) * 16);
+    const uint32_t aread = lds_address(tile) + wm * FP8_BLK + o, bread = lds_address(tile) + (BM + wn) * FP8_BLK + o;
+    typedef const __attribute__((address_space(3))) i4_t *lds_i4;
+    auto read = [&](uint32_t base, int f, int stage, int h) {
+        uint32_t p0 = base, p1;
+        if (h) asm volatile("v_xor_b32 %0, 64, %1" : "=v"(p0) : "v"(base));
+        if (h) asm volatile("v_xor_b32 %0, 0x60, %1" : "=v"(p1) : "v"(base));
+        else asm volatile("v_xor_b32 %0, 32, %1" : "=v"(p1) : "v"(base));
+        const i4_t lo = *(lds_i4)(p0 + stage * STAGE + f * 4096), hi = *(lds_i4)(p1 + stage * STAGE + f * 4096);
+        return i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    // scales of the block whose sums wait: of this lane's rows m, and (BTILE) of the fragments' columns; before the first block zeros
+    float sa[2] = {0.f, 0.f}, sb[2] = {0.f, 0.f};
+    if (!BTILE) scale[3][tid] = 0.0f;
+    auto read_scales = [&](int kb) {
+        const float *sc = scale[kb & 3];
+        sa[0] = sc[wm + row], sa[1] = sc[wm + 32 + row];
+        if (BTILE) sb[0] = sc[BM + wn], sb[1] = sc[BM + wn + 32];
+    };
+    // sums of block kb into the accumulators
+    auto scale_in = [&](int i, int j, int kb) {
+        if (BTILE) {
+            const float s = sa[i] * sb[j];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(sum[i][j][e], s, acc[i][j][e]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f4_t v = *reinterpret_cast<const f4_t *>(&scale[kb & 3][BM + wn + 32 * j + 8 * q + 4 * gg]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = __builtin_fmaf(sum[i][j][4 * q + e], sa[i] * v[e], acc[i][j][4 * q + e]);
+            }
+        }
+    };
+    i8_t a0[2], a1[2], b[2];
+    auto block = [&](int kb, int stage) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int i = t & 1, j = t >> 1;
+            scale_in(i, j, kb - 1);
+            sum[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a0[i], f16_t{}, 0, 0, 0, 127, 0, 127);
+            if (t < 2) a1[t] = read(aread, t, stage, 1);
+            if (i == 1) b[j] = read(bread, j, stage, 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int i = t & 1, j = t >> 1;
+            sum[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a1[i], sum[i][j], 0, 0, 0, 127, 0, 127);
+            if (t == 0) read_scales(kb);
+            if (t < 2) a0[t] = read(aread, t, stage ^ 1, 0);
+            if (i == 1) b[j] = read(bread, j, stage ^ 1, 0);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (2 * t + e < LOADS) fetch(2 * t + e, min(kb + 2, nkb - 1), stage);
+            if (t == 3) fetch_scales(kb + 2);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) fetch(i, min(s, nkb - 1), s);
+        fetch_scales(s);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    auto begin = [&](int stage) {
+#pragma unroll
+        for (int f = 0; f < 2; ++f) a0[f] = read(aread, f, stage, 0), b[f] = read(bread, f, stage, 0);
+    };
+    // zeros for what lies at K or behind it in the last block, whose first half is then read again
+    auto cut = [&](int kb, int stage) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        for (int t = tid; t < (BM + BN) * 8; t += WAVES * 64) {
+            const int r = t >> 3, c = t & 7, k = kb * FP8_BLK + 16 * c;
+            if (k + 16 <= p.K) continue;
+            i4_t *at = reinterpret_cast<i4_t *>(tile + stage * STAGE + r * FP8_BLK + (c ^ (r >> 1 & 7)) * 16);
+            *at = mask16(*at, k, p.K);
+        }
+        __syncthreads();
+        begin(stage);
+    };
+    begin(0);
+    int kb = 0;
+    for (; kb + 2 <= whole; kb += 2) {
+        block(kb, 0);
+        block(kb + 1, 1);
+    }
+    if (kb < nkb) {
+        if (kb >= whole) cut(kb, 0);
+        block(kb, 0);
+    }
+    if (kb + 1 < nkb) {
+        cut(kb + 1, 1);
+        block(kb + 1, 1);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < 4; ++t) scale_in(t & 1, t >> 1, nkb - 1);
+    T *y = static_cast<T *>(p.y);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int n = n0 + wn + 32 * j + 8 * q + 4 * gg;
+            f4_t bias = {0.f, 0.f, 0.f, 0.f};
+            if (p.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < p.N) bias[e] = p.bias[n + e];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                store4(y + (long long)(m0 + wm + 32 * i + row) * p.ldy + n, p.N - n,
+                       f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]} + bias);
         }
 }
 
@@ -838,14 +985,12 @@ template <int MODE, typename T> static void launch_block(MatArgs p, hipStream_t 
     p.tiles_n = (p.N + 255) / 256;
     const dim3 g(p.tiles_m * p.tiles_n), b(512);
     if constexpr (MODE == EXACT) {
-        if (!p.scale_f32) {
-            hipLaunchKernelGGL(fp8_matmul_wide_kernel, g, b, 0, st, p);
-            return;
-        }
+        if (p.scale_f32) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4>), g, b, 0, st, p);
+        else hipLaunchKernelGGL(fp8_matmul_wide_kernel, g, b, 0, st, p);
+    } else {
+        if (p.bshift) hipLaunchKernelGGL((fp8_matmul_scaled_kernel<true, T>), g, b, 0, st, p);
+        else hipLaunchKernelGGL((fp8_matmul_scaled_kernel<false, T>), g, b, 0, st, p);
     }
-    // (the last tile of a row may start at any multiple of N's factors: only at a multiple of 32 a fragment's columns have one scale)
-    if (p.bshift && p.N % 32 == 0) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, true, T>), g, b, 0, st, p);
-    else hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4, MODE, false, T>), g, b, 0, st, p);
 }
 
 template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t st)
@@ -889,6 +1034,7 @@ int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long lda
     if (M == 0 || N == 0) return 0;
     AQ_REQUIRE(a && as && b && bs && y, -EFAULT, "aq_fp8_matmul: NULL pointer");
     const long long nkb = (K + FP8_BLK - 1) / FP8_BLK;
+    AQ_REQUIRE(lda < (1LL << 23) * 16 && ldb < (1LL << 23) * 16, -E2BIG, "aq_fp8_matmul: a pitch of %lld bytes is too large", std::max(lda, ldb));
     AQ_REQUIRE(lda >= K && ldb >= K && ldas >= nkb && ldbs >= nkb && ldy >= N, -EINVAL, "aq_fp8_matmul: a pitch is smaller than its row");
     AQ_REQUIRE(((uintptr_t)a & 15) == 0 && ((uintptr_t)b & 15) == 0 && lda % 16 == 0 && ldb % 16 == 0, -EINVAL,
                "aq_fp8_matmul: codes and their pitches (%lld, %lld) have to be multiples of 16 bytes", lda, ldb);
