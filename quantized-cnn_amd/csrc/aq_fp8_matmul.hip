@@ -69,6 +69,7 @@ __device__ inline b8_t codes_to_bf16(int lo, int hi, float scale)
     return b8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// MODE: POW2, or the block's own sum (FP32S, EXACT)
 template <int MODE> __device__ inline f4_t block_product(const i8_t &b, const i8_t &a, f4_t acc, int sb, int sa)
 {
     if (MODE == POW2) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, acc, 0, 0, 0, sb, 0, sa);
@@ -484,16 +485,16 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
         }
 }
 
-// Large products with scales of any value and 16-bit outputs: tiles of 128 x 256, eight wavefronts with 64 x 64 each, LDS, loads and reads
-// as in fp8_matmul_large_kernel.  A block's sums start from zero in half 0 and are complete after half 1; they are scaled into the
+// Large products with scales of any value and 16-bit outputs: tiles of 128 x 256, eight wavefronts with 64 x 64 each, loads and reads
+// as in fp8_matmul_large_kernel with three stages of LDS.  A block's sums start from zero in half 0 and are complete after half 1; they are scaled into the
 // accumulators in half 0 of the next block, each right before its registers are needed again, while the matrix instruction of
 // the one before runs.  BTILE: B's scales are of 128 x 128 tiles, one for the 32 columns of a fragment (tiles start at multiples of 32
 // columns: the last one of a row reaches past N, reads row N - 1 there and stores nothing).
 template <bool BTILE, typename T>
 __global__ __launch_bounds__(512, 2) void fp8_matmul_scaled_kernel(const MatArgs p)
 {
-    constexpr int BM = 128, BN = 256, WAVES = 8, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
-    __shared__ __attribute__((aligned(128))) uint8_t tile[2 * STAGE];
+    constexpr int BM = 128, BN = 256, WAVES = 8, NS = 3, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
+    __shared__ __attribute__((aligned(128))) uint8_t tile[NS * STAGE];
     __shared__ __attribute__((aligned(16))) float scale[4][WAVES * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int tm, tn;
@@ -575,7 +576,7 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_scaled_kernel(const MatArgs
             if (i == 1) b[j] = read(bread, j, stage, 1);
             __builtin_amdgcn_sched_barrier(0);
         }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * (LOADS + 1)) : "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -583,23 +584,23 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_scaled_kernel(const MatArgs
             const int i = t & 1, j = t >> 1;
             sum[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a1[i], sum[i][j], 0, 0, 0, 127, 0, 127);
             if (t == 0) read_scales(kb);
-            if (t < 2) a0[t] = read(aread, t, stage ^ 1, 0);
-            if (i == 1) b[j] = read(bread, j, stage ^ 1, 0);
+            if (t < 2) a0[t] = read(aread, t, (stage + 1) % NS, 0);
+            if (i == 1) b[j] = read(bread, j, (stage + 1) % NS, 0);
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                if (2 * t + e < LOADS) fetch(2 * t + e, min(kb + 2, nkb - 1), stage);
-            if (t == 3) fetch_scales(kb + 2);
+                if (2 * t + e < LOADS) fetch(2 * t + e, min(kb + NS, nkb - 1), stage);
+            if (t == 3) fetch_scales(kb + NS);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
 
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NS; ++s) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) fetch(i, min(s, nkb - 1), s);
         fetch_scales(s);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * (LOADS + 1)) : "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     auto begin = [&](int stage) {
@@ -622,18 +623,16 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_scaled_kernel(const MatArgs
     };
     begin(0);
     int kb = 0;
-    for (; kb + 2 <= whole; kb += 2) {
-        block(kb, 0);
-        block(kb + 1, 1);
+    for (; kb + NS <= whole; kb += NS) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) block(kb + s, s);
     }
-    if (kb < nkb) {
-        if (kb >= whole) cut(kb, 0);
-        block(kb, 0);
-    }
-    if (kb + 1 < nkb) {
-        cut(kb + 1, 1);
-        block(kb + 1, 1);
-    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+        if (kb + s < nkb) {
+            if (kb + s >= whole) cut(kb + s, s);
+            block(kb + s, s);
+        }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int t = 0; t < 4; ++t) scale_in(t & 1, t >> 1, nkb - 1);
@@ -659,12 +658,12 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_scaled_kernel(const MatArgs
 // 64; three things go on at once, one behind each of the 16 matrix instructions of a half:
 //   the matrix instructions of half s;  the conversion to bf16 of half s + 1, four codes' pairs at a time;  the LDS reads of half s + 2,
 //   into the registers that the conversion has emptied.
-// At the start of block b, block b + 1 is in LDS, everybody has read b, and the load of b + 2 takes its place.
+// At the start of block b, block b + 1 is in LDS, everybody has read b, and the load of b + 3 takes its place.
 __global__ __launch_bounds__(512, 2) void fp8_matmul_wide_kernel(const MatArgs p)
 {
-    constexpr int BM = 128, BN = 256, WAVES = 8, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
-    __shared__ __attribute__((aligned(128))) uint8_t tile[2 * STAGE];
-    __shared__ uint32_t scale[2][WAVES * 64];
+    constexpr int BM = 128, BN = 256, WAVES = 8, NS = 3, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
+    __shared__ __attribute__((aligned(128))) uint8_t tile[NS * STAGE];
+    __shared__ uint32_t scale[NS][WAVES * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int tm, tn;
     tile_of(blockIdx.x, p.tiles_m, p.tiles_n, tm, tn);
@@ -719,7 +718,7 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_wide_kernel(const MatArgs p
     // fragments: 0, 1 of A, 2, 3 of B
     i4_t raw[4][2];
     b8_t even[4][4], odd[4][4];
-    uint32_t sc[2][4];
+    uint32_t sc[NS][4];
     auto read_raw = [&](int f, int stage, int h) {
         const uint32_t base = f < 2 ? aread : bread;
         uint32_t p0 = base, p1;  // (turned at the read: there are no registers to keep the four addresses)
@@ -743,28 +742,28 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_wide_kernel(const MatArgs p
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now[2 + j][w], now[i][w], acc[i][j], 0, 0, 0);
             convert(next, t >> 2, t & 3, s[t >> 2]);
             if ((t & 3) == 3) read_raw(t >> 2, rstage, h);
-            if (h == 0 && t < LOADS) fetch(t, min(kb + 2, nkb - 1), fstage);
-            if (h == 0 && t == LOADS) fetch_scales(min(kb + 2, nkb - 1), fstage);
+            if (h == 0 && t < LOADS) fetch(t, min(kb + NS, nkb - 1), fstage);
+            if (h == 0 && t == LOADS) fetch_scales(min(kb + NS, nkb - 1), fstage);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     auto block = [&](int kb, int stage) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * (LOADS + 1)) : "memory");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        if (kb + 1 == whole && whole < nkb) cut(kb + 1, stage ^ 1);
-        read_scales(stage ^ 1);
-        half(even, odd, sc[stage], stage ^ 1, 0, kb, stage);
-        half(odd, even, sc[stage ^ 1], stage ^ 1, 1, kb, stage);
+        if (kb + 1 == whole && whole < nkb) cut(kb + 1, (stage + 1) % NS);
+        read_scales((stage + 1) % NS);
+        half(even, odd, sc[stage], (stage + 1) % NS, 0, kb, stage);
+        half(odd, even, sc[(stage + 1) % NS], (stage + 1) % NS, 1, kb, stage);
     };
 
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NS; ++s) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) fetch(i, min(s, nkb - 1), s);
         fetch_scales(min(s, nkb - 1), s);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * (LOADS + 1)) : "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     if (whole == 0) cut(0, 0);
@@ -776,9 +775,10 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_wide_kernel(const MatArgs p
         for (int w = 0; w < 4; ++w) convert(even, f, w, sc[0][f]);
         read_raw(f, 0, 1);
     }
-    for (int kb = 0; kb < nkb; kb += 2) {
-        block(kb, 0);
-        if (kb + 1 < nkb) block(kb + 1, 1);
+    for (int kb = 0; kb < nkb; kb += NS) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+            if (kb + s < nkb) block(kb + s, s);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     float *y = static_cast<float *>(p.y);
@@ -1028,13 +1028,12 @@ int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long lda
     AQ_REQUIRE((a_block_rows == 1 || a_block_rows == FP8_BLK) && (b_block_rows == 1 || b_block_rows == FP8_BLK), -EINVAL,
                "aq_fp8_matmul: blocks of %d and %d rows: 1 or %d", a_block_rows, b_block_rows, FP8_BLK);
     AQ_REQUIRE(M >= 0 && N >= 0 && K >= 1, -EINVAL, "aq_fp8_matmul: bad sizes M=%lld N=%lld K=%lld", M, N, K);
-    // a launch holds fewer than 2^32 threads, row and column numbers stay below 2^31
-    AQ_REQUIRE(M < (1LL << 30) && N < (1LL << 30) && K < (1LL << 30) && ((M + 63) / 64) * ((N + 15) / 16) < (1LL << 23), -E2BIG,
-               "aq_fp8_matmul: M=%lld N=%lld K=%lld is too large for one call", M, N, K);
+    // a launch holds fewer than 2^32 threads; offsets within a tile have 32 bits
+    AQ_REQUIRE(M < (1LL << 26) && N < (1LL << 26) && M * N < (1LL << 38), -E2BIG, "aq_fp8_matmul: M=%lld N=%lld K=%lld is too large for one call", M, N, K);
+    AQ_REQUIRE(lda < (1LL << 24) && ldb < (1LL << 24), -E2BIG, "aq_fp8_matmul: a pitch of %lld bytes is too large", std::max(lda, ldb));
     if (M == 0 || N == 0) return 0;
     AQ_REQUIRE(a && as && b && bs && y, -EFAULT, "aq_fp8_matmul: NULL pointer");
     const long long nkb = (K + FP8_BLK - 1) / FP8_BLK;
-    AQ_REQUIRE(lda < (1LL << 23) * 16 && ldb < (1LL << 23) * 16, -E2BIG, "aq_fp8_matmul: a pitch of %lld bytes is too large", std::max(lda, ldb));
     AQ_REQUIRE(lda >= K && ldb >= K && ldas >= nkb && ldbs >= nkb && ldy >= N, -EINVAL, "aq_fp8_matmul: a pitch is smaller than its row");
     AQ_REQUIRE(((uintptr_t)a & 15) == 0 && ((uintptr_t)b & 15) == 0 && lda % 16 == 0 && ldb % 16 == 0, -EINVAL,
                "aq_fp8_matmul: codes and their pitches (%lld, %lld) have to be multiples of 16 bytes", lda, ldb);

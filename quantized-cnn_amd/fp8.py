@@ -131,7 +131,7 @@ def linear(x, weight, bias=None, out_dtype=None):
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight over the last axis -> (y, h), or y alone without residual."""
-    out = _RmsNorm.apply(_flat(x), weight, _flat(residual) if residual is not None else None, eps)
+    out = _RmsNorm.apply(_flat(x), weight.float(), _flat(residual) if residual is not None else None, eps)
     if residual is None:
         return out.view(x.shape)
     return out[0].view(x.shape), out[1].view(x.shape)
@@ -142,7 +142,7 @@ def norm_linear(x, norm_weight, weight, bias=None, residual=None, eps=1e-6, out_
     without residual."""
     if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
         raise ValueError("fp8.norm_linear: x %s / weight %s: need (..., in) and (in, out)" % (tuple(x.shape), tuple(weight.shape)))
-    out = _NormLinear.apply(_flat(x), norm_weight, weight, bias, _flat(residual) if residual is not None else None, eps, out_dtype or x.dtype)
+    out = _NormLinear.apply(_flat(x), norm_weight.float(), weight, bias, _flat(residual) if residual is not None else None, eps, out_dtype or x.dtype)
     y, h = out if residual is not None else (out, None)
     y = y.view(x.shape[:-1] + (y.shape[1],))
     return y if residual is None else (y, h.view(x.shape))

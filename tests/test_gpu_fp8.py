@@ -243,7 +243,8 @@ def test_product_other_forms(pow2):
     check_product(operand(7, 300, 128, pow2, 1), operand(260, 300, 1, pow2, 2), torch.randn(260, device=DEV), torch.float16)
 
 
-@pytest.mark.parametrize("m,n,k", [(1024, 1024, 512), (1030, 1300, 700), (1100, 1025, 1029), (1281, 1150, 576), (1024, 1400, 650)])
+@pytest.mark.parametrize("m,n,k", [(1024, 1024, 512), (1030, 1300, 700), (1100, 1025, 1029), (1281, 1150, 576), (1024, 1400, 650), (2100, 2100, 520),
+                                   (1700, 1400, 385), (3600, 3700, 260), (2304, 8192, 129)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("pow2", [True, False])
 def test_large_product(m, n, k, dtype, pow2):
@@ -288,21 +289,44 @@ def test_product_ignores_what_lies_behind_its_rows(m, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("m", [2, 40, 140])
-def test_product_special_values(m, dtype):
-    """A NaN code spoils its row (or column) and nothing else; extreme scales."""
-    a, b = operand(m, 300, 1, True, 1), operand(150, 300, 1, True, 2)
+@pytest.mark.parametrize("m,n", [(2, 150), (40, 150), (140, 150), (300, 900), (1100, 1300), (3600, 3700)])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_product_special_values(m, n, dtype, pow2):
+    """A NaN code or scale spoils its row (or column) and nothing else; extreme scales."""
+    k = 300
+    a, b = operand(m, k, 1, pow2, 1), operand(n, k, 1, pow2, 2)
     clean = ops.fp8_matmul(a, b, out_dtype=dtype)
     a.data[1, 250] = float("nan")
     b.data[77, 3] = float("nan")
+    b.scale[140, 2] = float("nan")
     y = ops.fp8_matmul(a, b, out_dtype=dtype)
     bad = torch.zeros_like(y, dtype=torch.bool)
-    bad[1], bad[:, 77] = True, True
+    bad[1], bad[:, 77], bad[:, 140] = True, True, True
     assert torch.equal(torch.isnan(y), bad) and torch.equal(y[~bad], clean[~bad])
-    z = operand(m, 300, 1, True, 1)
+    a.data[1, 250] = float("inf")  # (the type has no infinity: a NaN again)
+    assert bool(torch.isnan(ops.fp8_matmul(a, b, out_dtype=dtype)[1]).all())
+    z = operand(m, k, 1, pow2, 1)
     z.scale[0, 1] = 2.0 ** -127
     z.scale[1, 0] = 2.0 ** 100
-    check_product(z, operand(150, 300, 1, True, 2), None, dtype)
+    check_product(z, operand(n, k, 1, pow2, 2), None, dtype)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_product_of_drawn_sizes(seed):
+    rs = np.random.RandomState(seed)
+    m, n, k = (int(np.exp(rs.uniform(0, np.log(t)))) for t in (1500, 2000, 6000))
+    pow2, dtype = bool(rs.randint(2)), TYPES[rs.randint(3)]
+    a = operand(m, k, 1 if rs.randint(3) else 128, pow2, seed, False)
+    b = operand(n, k, 1 if rs.randint(3) == 0 else 128, pow2, seed + 1, False)
+    check_product(a, b, torch.randn(n, device=DEV) if rs.randint(2) else None, dtype)
+
+
+def test_product_of_tiny_blocks_in_fp32():
+    """Scales down to 2^-117 take part in full: results near 1e-33."""
+    a, b = operand(700, 400, 1, True, 1, False), operand(900, 400, 1, True, 2, False)
+    want = ops.fp8_matmul(a, b, out_dtype=torch.float32)
+    a.scale.copy_((a.scale.float() * 2.0 ** -110).to(E8))
+    assert torch.equal(ops.fp8_matmul(a, b, out_dtype=torch.float32), want * 2.0 ** -110)
 
 
 @pytest.mark.parametrize("shape", [(1, 512, 4096), (24, 1000, 4096), (300, 700, 1024), (100, 300, 4096), (1000, 1100, 600)])
@@ -623,6 +647,25 @@ def test_packed_layer_serves_the_same():
     assert layer._packed is None
     with pytest.raises(ValueError, match="need"):
         fp8.linear(x, torch.zeros(301, 5, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layers_with_16_bit_weights(dtype):
+    norm, lin = fp8.RMSNorm(130).to(DEV, dtype), fp8.Fp8Linear(130, 20).to(DEV, dtype)
+    x = torch.randn(6, 3, 130, device=DEV).to(dtype)
+    y, h = norm(x, x)
+    out = lin(y)
+    assert out.shape == (6, 3, 20) and out.dtype == dtype and h.dtype == dtype
+    out.float().square().sum().backward()
+    assert norm.weight.grad.dtype == dtype and lin.weight.grad.dtype == dtype and lin.bias.grad.dtype == dtype
+    n32 = norm.weight.detach().float()
+    assert torch.equal(y.view(18, 130), ops.rms_norm_forward(x.view(18, 130), n32, residual=x.view(18, 130))[0])
+    o = fp8.norm_linear(x, norm.weight, lin.weight, lin.bias)
+    assert o.shape == (6, 3, 20)
+    e = fp8.norm_linear(x[:0], norm.weight, lin.weight, lin.bias)  # no tokens
+    assert e.shape == (0, 3, 20)
+    g = torch.autograd.grad(fp8.linear(x[:0], lin.weight, lin.bias), (lin.weight, lin.bias), torch.zeros(0, 3, 20, device=DEV, dtype=dtype))
+    assert all(bool((t == 0).all()) for t in g)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
