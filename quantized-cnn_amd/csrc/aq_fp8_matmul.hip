@@ -13,6 +13,10 @@
 //   WIDE:  the same for large products with power-of-two scales: code * scale is exact in bf16 (for scales of 2^-117 and more; below,
 //          a code's last bits fall under bf16's smallest step), so the scales go into the conversion, the blocks' sums into
 //          one accumulator through the bf16 instruction, and the fp32 multiplications per block are saved.
+//
+// What bounds them, measured: 8192^3 to bf16 0.46 ms, 2.4 PFLOP/s: the power limit (the matrix units are busy 77 % of the cycles at
+// 1.5 GHz; a loop of nothing but these instructions on random codes reaches 3.8 PFLOP/s).  4096^3 to fp32 0.117 ms, 1.18 PFLOP/s
+// (a library product of bf16 matrices: 1.23).  Few rows: the reading of B, 8192 x 8192 for one row in 14.8 us, 4.5 TB/s.
 #include <algorithm>
 
 #include "aq_fp8.h"
@@ -485,15 +489,15 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
         }
 }
 
-// Large products with scales of any value and 16-bit outputs: tiles of 128 x 256, eight wavefronts with 64 x 64 each, loads and reads
-// as in fp8_matmul_large_kernel with three stages of LDS.  A block's sums start from zero in half 0 and are complete after half 1; they are scaled into the
+// Large products with scales of any value and 16-bit outputs: tiles of 128 x BN, wavefronts with 64 x 64 each, loads and reads
+// as in fp8_matmul_large_kernel with NS stages of LDS.  A block's sums start from zero in half 0 and are complete after half 1; they are scaled into the
 // accumulators in half 0 of the next block, each right before its registers are needed again, while the matrix instruction of
 // the one before runs.  BTILE: B's scales are of 128 x 128 tiles, one for the 32 columns of a fragment (tiles start at multiples of 32
 // columns: the last one of a row reaches past N, reads row N - 1 there and stores nothing).
-template <bool BTILE, typename T>
-__global__ __launch_bounds__(512, 2) void fp8_matmul_scaled_kernel(const MatArgs p)
+template <int BN, int NS, bool BTILE, typename T>
+__global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_scaled_kernel(const MatArgs p)
 {
-    constexpr int BM = 128, BN = 256, WAVES = 8, NS = 3, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
+    constexpr int BM = 128, WAVES = BN / 32, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
     __shared__ __attribute__((aligned(128))) uint8_t tile[NS * STAGE];
     __shared__ __attribute__((aligned(16))) float scale[4][WAVES * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -654,14 +658,15 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_scaled_kernel(const MatArgs
         }
 }
 
-// Large products with power-of-two scales and fp32 outputs: tiles of 128 x 256, eight wavefronts with 64 x 64 each.  K in half blocks of
-// 64; three things go on at once, one behind each of the 16 matrix instructions of a half:
+// Large products with power-of-two scales and fp32 outputs: tiles of 128 x BN, wavefronts with 64 x 64 each.  K in half blocks of 64;
+// three things go on at once, one behind each of the 16 matrix instructions of a half:
 //   the matrix instructions of half s;  the conversion to bf16 of half s + 1, four codes' pairs at a time;  the LDS reads of half s + 2,
 //   into the registers that the conversion has emptied.
-// At the start of block b, block b + 1 is in LDS, everybody has read b, and the load of b + 3 takes its place.
-__global__ __launch_bounds__(512, 2) void fp8_matmul_wide_kernel(const MatArgs p)
+// At the start of block b, block b + 1 is in LDS, everybody has read b, and the load of b + NS takes its place.
+template <int BN, int NS>
+__global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_wide_kernel(const MatArgs p)
 {
-    constexpr int BM = 128, BN = 256, WAVES = 8, NS = 3, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
+    constexpr int BM = 128, WAVES = BN / 32, LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
     __shared__ __attribute__((aligned(128))) uint8_t tile[NS * STAGE];
     __shared__ uint32_t scale[NS][WAVES * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -960,6 +965,11 @@ static int matmul_splits(long long M, long long N, long long K)
     return (int)std::max(1LL, std::min(256 / tiles, nkb / 4));
 }
 
+// Tiles by how many of them there are for the 256 compute units (times at 4096-long rows unless stated):
+//   256 x 256 from three quarters of a round on (4096 x 4096: 57 us against 75 us in 128 x 128; 2048 x 4096, half a round: 47 against 38);
+//   128 x 128 with two stages, two workgroups on a unit, for more than a round (1500 x 5000 x 2560: 25 us against 30 us with four stages);
+//   128 x 128 with four stages for up to a round (1024 x 4096: 22 against 28 us with two);
+//   64 x 128 for fewer (512 x 4096: 17 us; 1000 x 1000 x 1000: 8 against 11 us), K in parts for very few.
 template <typename T> static void launch_pow2(MatArgs p, hipStream_t st)
 {
     if (p.N < 128) return launch_rows<4, 2, 2, POW2, T>(p, st);
@@ -981,15 +991,23 @@ template <typename T> static void launch_pow2(MatArgs p, hipStream_t st)
 
 template <int MODE, typename T> static void launch_block(MatArgs p, hipStream_t st)
 {
+    // Two workgroups of 128 x 128 on a compute unit run past each other's barriers (fp32 output 512 x 4096 x 4096: 30 us against 46 us for one
+    // of 128 x 256, any scales 28 against 34 us); with scales in fp32 arithmetic the larger tile wins once there are two
+    // rounds of it (4096^3: 16-bit output 82 against 86 us, fp32 output 147 against 191 us).
+    const bool wide = p.scale_f32 && p.N >= 256 && tiles_of(p.M, p.N, 128, 256) >= 512;
     p.tiles_m = (p.M + 127) / 128;
-    p.tiles_n = (p.N + 255) / 256;
-    const dim3 g(p.tiles_m * p.tiles_n), b(512);
+    p.tiles_n = wide ? (p.N + 255) / 256 : (p.N + 127) / 128;
+    const dim3 g(p.tiles_m * p.tiles_n);
     if constexpr (MODE == EXACT) {
-        if (p.scale_f32) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4>), g, b, 0, st, p);
-        else hipLaunchKernelGGL(fp8_matmul_wide_kernel, g, b, 0, st, p);
+        if (wide) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 256, 2, 4>), g, dim3(512), 0, st, p);
+        else if (p.scale_f32) hipLaunchKernelGGL((fp8_matmul_block_kernel<128, 128, 2, 2>), g, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((fp8_matmul_wide_kernel<128, 2>), g, dim3(256), 0, st, p);
+    } else if (wide) {
+        if (p.bshift) hipLaunchKernelGGL((fp8_matmul_scaled_kernel<256, 3, true, T>), g, dim3(512), 0, st, p);
+        else hipLaunchKernelGGL((fp8_matmul_scaled_kernel<256, 3, false, T>), g, dim3(512), 0, st, p);
     } else {
-        if (p.bshift) hipLaunchKernelGGL((fp8_matmul_scaled_kernel<true, T>), g, b, 0, st, p);
-        else hipLaunchKernelGGL((fp8_matmul_scaled_kernel<false, T>), g, b, 0, st, p);
+        if (p.bshift) hipLaunchKernelGGL((fp8_matmul_scaled_kernel<128, 2, true, T>), g, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((fp8_matmul_scaled_kernel<128, 2, false, T>), g, dim3(256), 0, st, p);
     }
 }
 
@@ -1001,8 +1019,11 @@ template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t
     if constexpr (MODE == POW2) {
         launch_pow2<T>(p, st);
     } else {
+        // Streamed fragments while their workgroups fit the compute units about once (512 x 1024 x 4096: 19 against 28 us on tiles;
+        // 512 x 2048 x 4096: 35 against 28 us); fp32 outputs with any scales, whose tiles are the slowest, twice (36 against 48 us).
         if (tiles_of(p.M, p.N, 64, 16) <= 256) return launch_rows<4, 1, 2, MODE, T>(p, st);
-        if (p.M < 128 || p.N < 256 || tiles_of(p.M, p.N, 64, 32) <= 512) return launch_rows<4, 2, 2, MODE, T>(p, st);
+        const long long few = MODE == EXACT && p.scale_f32 ? 512 : 256;
+        if (p.M < 128 || p.N < 128 || tiles_of(p.M, p.N, 64, 32) <= few) return launch_rows<4, 2, 2, MODE, T>(p, st);
         launch_block<MODE, T>(p, st);
     }
 }

@@ -2,6 +2,8 @@
 // their rows, along their columns (the transpose, for the products of a backward pass) or both from one read, turned round, and
 // read back.  Per block: amax over the finite magnitudes, scale 2^e with the smallest e that brings amax to 448 or less, codes
 // x * 2^-e rounded to nearest even.  Scaling by a power of two is exact, so the code's rounding is the only one.
+// All are bound by memory bandwidth: 8192 x 8192 bf16 to codes along both axes 56 us (268 MB, 4.7 TB/s; a copy of 1 GiB runs at
+// 5.1 TB/s), codes to bf16 values 38 us (201 MB, 5.2 TB/s).
 #include "aq_fp8.h"
 
 namespace aq {

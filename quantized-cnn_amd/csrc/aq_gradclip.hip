@@ -2,7 +2,9 @@
 // Squares are formed and summed in double (no overflow for large fp32 gradients, and the order does not show in the result's
 // fp32 digits).  A tensor is cut into chunks and the chunks of all tensors are dealt to at most GRAD_PARTS workgroups, each of
 // which leaves one partial sum.  The scaling launch adds the partial sums up again in every workgroup, in the same order
-// everywhere: two launches for 64 tensors, no atomics, no host round trip.  Both passes are bound by memory bandwidth.
+// everywhere: two launches for 64 tensors, no atomics, no host round trip.  Both passes are bound by memory bandwidth: 400 M fp32
+// elements 246 us (1.6 GB, 6.5 TB/s) and 594 us (3.2 GB, 5.4 TB/s).  16-byte accesses that are neighbours across the lanes matter
+// there: with two per lane side by side the streaming stores took 693 us.
 #include <algorithm>
 
 #include "aq_fp8.h"

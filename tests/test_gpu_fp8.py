@@ -244,7 +244,8 @@ def test_product_other_forms(pow2):
 
 
 @pytest.mark.parametrize("m,n,k", [(1024, 1024, 512), (1030, 1300, 700), (1100, 1025, 1029), (1281, 1150, 576), (1024, 1400, 650), (2100, 2100, 520),
-                                   (1700, 1400, 385), (3600, 3700, 260), (2304, 8192, 129)])
+                                   (1700, 1400, 385), (3600, 3700, 260), (2304, 8192, 129),
+                                   (4097, 4225, 200)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("pow2", [True, False])
 def test_large_product(m, n, k, dtype, pow2):
