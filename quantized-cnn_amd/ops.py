@@ -5,7 +5,6 @@ torch's caching allocator (so calls are capturable in a HIP graph), and never sy
 """
 import array
 import ctypes as C
-import functools
 
 import torch
 
@@ -909,16 +908,8 @@ FP8_BLOCK = 128
 _SCALE_TYPES = {torch.float8_e8m0fnu: _lib.SCALE_POW2, torch.float32: _lib.SCALE_F32}
 
 
-def _on_device(f):
-    """Runs f on the device of its first argument (a tensor, Fp8Blocks, or a list of tensors), whichever is current."""
-    @functools.wraps(f)
-    def call(first, *args, **kw):
-        d = first.device if isinstance(first, (torch.Tensor, Fp8Blocks)) else first[0].device if len(first) else None
-        if d is None or d.type != "cuda" or d.index == torch._C._cuda_getDevice():
-            return f(first, *args, **kw)
-        with torch.cuda.device(d):
-            return f(first, *args, **kw)
-    return call
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _hip(t, name, device=None):
@@ -933,7 +924,8 @@ def _matrix(t, name, device=None, dtype=None, shape=None):
     """Checks of a 2-D operand whose rows may lie apart; returns its pitch in elements."""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise ValueError("%s: expected a 2-D tensor" % name)
-    _hip(t, name, device)
+    if not t.is_cuda or (device is not None and t.device != device):
+        _hip(t, name, device)
     if t.dtype not in _lib.ELEMENT_TYPES or (dtype is not None and t.dtype != dtype):
         raise ValueError("%s: dtype %s, expected %s" % (name, t.dtype, dtype or "float32, bfloat16 or float16"))
     if shape is not None and t.shape != shape:
@@ -943,10 +935,12 @@ def _matrix(t, name, device=None, dtype=None, shape=None):
 
 def _pitch(t, name):
     rows, cols = t.shape
-    ld = t.stride(0) if rows > 1 else cols
-    if (cols > 1 and t.stride(1) != 1) or (ld < cols and rows and cols):
+    s0, s1 = t.stride()
+    if rows <= 1:
+        s0 = cols
+    if (cols > 1 and s1 != 1) or (s0 < cols and rows):
         raise ValueError("%s: strides %s: the elements of a row have to be neighbours, and rows must not overlap" % (name, t.stride()))
-    return max(ld, cols)
+    return s0 if s0 > cols else cols
 
 
 class Fp8Blocks:
@@ -964,19 +958,21 @@ class Fp8Blocks:
     def __init__(self, data, scale, block_rows=1):
         if not isinstance(data, torch.Tensor) or not isinstance(scale, torch.Tensor) or data.dim() != 2 or scale.dim() != 2:
             raise ValueError("Fp8Blocks: data and scale have to be 2-D tensors")
-        _hip(data, "data")
-        _hip(scale, "scale", data.device)
-        if data.dtype != torch.float8_e4m3fn or scale.dtype not in _SCALE_TYPES:
+        dev = data.device
+        if not data.is_cuda or scale.device != dev:
+            _hip(data, "data")
+            _hip(scale, "scale", dev)
+        st = _SCALE_TYPES.get(scale.dtype)
+        if data.dtype != torch.float8_e4m3fn or st is None:
             raise ValueError("Fp8Blocks: data %s / scale %s, expected float8_e4m3fn and float8_e8m0fnu or float32" % (data.dtype, scale.dtype))
-        if block_rows not in (1, FP8_BLOCK):
+        if block_rows != 1 and block_rows != FP8_BLOCK:
             raise ValueError("Fp8Blocks: block_rows %r, expected 1 or %d" % (block_rows, FP8_BLOCK))
-        rows, cols = data.shape
-        if scale.shape != (-(-rows // block_rows), -(-cols // FP8_BLOCK)):
+        rows, cols = shape = data.shape
+        if scale.shape != (-(-rows // block_rows), (cols + 127) >> 7):
             raise ValueError("Fp8Blocks: scale %s does not belong to data %s in blocks of %d x %d" % (
                 tuple(scale.shape), (rows, cols), block_rows, FP8_BLOCK))
-        self._data, self._scale, self._buf, self.block_rows, self.shape, self.device = data, scale, None, block_rows, (rows, cols), data.device
+        self._data, self._scale, self._buf, self.block_rows, self.shape, self.device, self._scale_type = data, scale, None, block_rows, shape, dev, st
         self._ld, self._lds = _pitch(data, "data"), _pitch(scale, "scale")
-        self._scale_type = _SCALE_TYPES[scale.dtype]
 
     @property
     def scale_dtype(self):
@@ -1034,17 +1030,12 @@ def _new_blocks(rows, cols, block_rows, scale_type, device):
     return b
 
 
-def _stream_of(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
 def _scale_dtype(scale_dtype):
     if scale_dtype not in _SCALE_TYPES:
         raise ValueError("scale_dtype %s, expected float8_e8m0fnu or float32" % (scale_dtype,))
     return _SCALE_TYPES[scale_dtype]
 
 
-@_on_device
 def fp8_quantize(x, forms="rows", block_rows=1, scale_dtype=torch.float8_e8m0fnu, colsum=False):
     """x (rows, cols), fp32 / bf16 / fp16 -> Fp8Blocks: per block the smallest power of two that brings its largest finite
     magnitude to 448 or less, codes rounded to nearest even; NaN and infinities become NaN codes.
@@ -1060,6 +1051,9 @@ def fp8_quantize(x, forms="rows", block_rows=1, scale_dtype=torch.float8_e8m0fnu
         raise ValueError("fp8_quantize: column sums come with the transposed form in 1 x 128 blocks only")
     rows, cols = x.shape
     dev = x.device
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return fp8_quantize(x, forms, block_rows, scale_dtype, colsum)
     q = _new_blocks(rows, cols, block_rows, st, dev) if forms != "cols" else None
     qt = _new_blocks(cols, rows, block_rows, st, dev) if forms != "rows" else None
     sums = ws = None
@@ -1073,41 +1067,44 @@ def fp8_quantize(x, forms="rows", block_rows=1, scale_dtype=torch.float8_e8m0fnu
         pt, pts = qt._ptrs() if qt is not None else (None, None)
         _lib.check(_lib.lib().aq_fp8_quantize(
             x.data_ptr(), _lib.ELEMENT_TYPES[x.dtype], rows, cols, ldx, pq, q._ld if pq else 0, ps, q._lds if pq else 0, pt, qt._ld if pt else 0, pts,
-            qt._lds if pt else 0, block_rows, st, sums.data_ptr() if colsum else None, ws.data_ptr() if colsum else None, nbytes, _stream_of(dev)))
+            qt._lds if pt else 0, block_rows, st, sums.data_ptr() if colsum else None, ws.data_ptr() if colsum else None, nbytes, _current_stream(dev.index)))
     out = (q,) if forms == "rows" else (qt,) if forms == "cols" else (q, qt)
     if colsum:
         out += (sums,)
     return out[0] if len(out) == 1 else out
 
 
-@_on_device
 def fp8_transpose(q):
     """Fp8Blocks of the transposed matrix.  Tiles of 128 x 128 keep their codes; 1 x 128 blocks are formed anew along the other axis
     (exact but for values below the new block's smallest subnormal step)."""
+    if q.device.index != _current_device():
+        with torch.cuda.device(q.device):
+            return fp8_transpose(q)
     rows, cols = q.shape
     t = _new_blocks(cols, rows, q.block_rows, q._scale_type, q.device)
     if rows and cols:
         pq, ps = q._ptrs()
         pt, pts = t._ptrs()
-        _lib.check(_lib.lib().aq_fp8_transpose(pq, q._ld, ps, q._lds, rows, cols, pt, t._ld, pts, t._lds, q.block_rows, q._scale_type, _stream_of(q.device)))
+        _lib.check(_lib.lib().aq_fp8_transpose(pq, q._ld, ps, q._lds, rows, cols, pt, t._ld, pts, t._lds, q.block_rows, q._scale_type, _current_stream(q.device.index)))
     return t
 
 
-@_on_device
 def fp8_dequantize(q, dtype=torch.bfloat16):
     """The values of Fp8Blocks as a plain tensor (in bf16 and fp32 exact where the scales are powers of two and the values in range)."""
+    if q.device.index != _current_device():
+        with torch.cuda.device(q.device):
+            return fp8_dequantize(q, dtype)
     if dtype not in _lib.ELEMENT_TYPES:
         raise ValueError("fp8_dequantize: dtype %s, expected float32, bfloat16 or float16" % (dtype,))
     rows, cols = q.shape
-    y = torch.empty((rows, cols), dtype=dtype, device=q.device)
+    y = torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=q.device)
     if rows and cols:
         pq, ps = q._ptrs()
         _lib.check(_lib.lib().aq_fp8_dequantize(pq, q._ld, ps, q._lds, rows, cols, q.block_rows, q._scale_type, y.data_ptr(), _lib.ELEMENT_TYPES[dtype],
-                                                cols, _stream_of(q.device)))
+                                                cols, _current_stream(q.device.index)))
     return y
 
 
-@_on_device
 def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     """a (M, K) @ b (N, K)^T + bias (N,) of two Fp8Blocks with scales of one type -> (M, N).  fp32 outputs keep fp32 sums; bf16 and
     fp16 outputs run on the 8-bit matrix instructions (error of a sum up to 2^-13 of the sum of its terms' magnitudes)."""
@@ -1116,6 +1113,9 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     M, K = a.shape
     N = b.shape[0]
     dev = a.device
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return fp8_matmul(a, b, bias, out_dtype)
     if b.shape[1] != K or b.device != dev or a._scale_type != b._scale_type:
         raise ValueError("fp8_matmul: a %s with %s scales on %s, b %s with %s scales on %s" % (
             a.shape, a.scale_dtype, dev, b.shape, b.scale_dtype, b.device))
@@ -1128,17 +1128,17 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     if K == 0:
         y = torch.zeros((M, N), dtype=out_dtype, device=dev)
         return y if bias is None else y + bias.to(out_dtype)
-    y = torch.empty((M, N), dtype=out_dtype, device=dev)
+    y = torch.empty_strided((M, N), (N, 1), dtype=out_dtype, device=dev)
     if M == 0 or N == 0:
         return y
     L = _lib.lib()
     da, pa, lda = a._by16()
     db, pb, ldb = b._by16()
-    nbytes = L.aq_fp8_matmul_workspace_bytes(M, N, K)
+    nbytes = L.aq_fp8_matmul_workspace_bytes(M, N, K) if M > 64 else 0  # (64 rows and fewer need none)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.check(L.aq_fp8_matmul(pa, lda, a._ptrs()[1], a._lds, a.block_rows, pb, ldb, b._ptrs()[1], b._lds, b.block_rows, M, N, K,
                                a._scale_type, bias.data_ptr() if bias is not None else None, y.data_ptr(), _lib.ELEMENT_TYPES[out_dtype], N,
-                               ws.data_ptr() if nbytes else None, nbytes, _stream_of(dev)))
+                               ws.data_ptr() if nbytes else None, nbytes, _current_stream(dev.index)))
     return y
 
 
@@ -1151,7 +1151,6 @@ def _norm_vector(t, n, name, dev):
     return t.data_ptr()
 
 
-@_on_device
 def rms_norm_forward(x, weight, residual=None, eps=1e-6, quantize=False, scale_dtype=torch.float8_e8m0fnu):
     """h = x + residual (rounded to x's type; x itself without residual); y = h / sqrt(mean(h^2) + eps) * weight over the rows of
     x (rows, cols) -> (y, h, rstd): y of x's type, or Fp8Blocks of it (1 x 128 blocks) with quantize=True; rstd fp32 (rows,)."""
@@ -1160,22 +1159,24 @@ def rms_norm_forward(x, weight, residual=None, eps=1e-6, quantize=False, scale_d
     dev = x.device
     if cols == 0:
         raise ValueError("rms_norm_forward: x %s has no columns" % (tuple(x.shape),))
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return rms_norm_forward(x, weight, residual, eps, quantize, scale_dtype)
     ldr = _matrix(residual, "residual", dev, x.dtype, x.shape) if residual is not None else 0
     w = _norm_vector(weight, cols, "weight", dev)
     st = _scale_dtype(scale_dtype)
-    y = _new_blocks(rows, cols, 1, st, dev) if quantize else torch.empty((rows, cols), dtype=x.dtype, device=dev)
-    h = torch.empty((rows, cols), dtype=x.dtype, device=dev) if residual is not None else x
+    y = _new_blocks(rows, cols, 1, st, dev) if quantize else torch.empty_strided((rows, cols), (cols, 1), dtype=x.dtype, device=dev)
+    h = torch.empty_strided((rows, cols), (cols, 1), dtype=x.dtype, device=dev) if residual is not None else x
     rstd = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows:
         pq, ps = y._ptrs() if quantize else (None, None)
         _lib.check(_lib.lib().aq_rms_norm_fwd(
             x.data_ptr(), ldx, residual.data_ptr() if residual is not None else None, ldr, _lib.ELEMENT_TYPES[x.dtype], w, rows, cols, eps,
             None if quantize else y.data_ptr(), cols, pq, y._ld if quantize else 0, ps, y._lds if quantize else 0, st,
-            h.data_ptr() if residual is not None else None, cols, rstd.data_ptr(), _stream_of(dev)))
+            h.data_ptr() if residual is not None else None, cols, rstd.data_ptr(), _current_stream(dev.index)))
     return y, h, rstd
 
 
-@_on_device
 def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dx=True, need_dweight=True):
     """Gradients of rms_norm_forward from h and rstd as it returned them: -> (dx, dweight), dx (of h's type) for x and residual
     alike, dweight fp32; None where not needed.  dh: the gradient that arrives at h by itself (the residual path), added to dx."""
@@ -1186,6 +1187,9 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dx=True, need_dweight=T
     lddh = _matrix(dh, "dh", dev, dy.dtype, dy.shape) if dh is not None else 0
     if cols == 0:
         raise ValueError("rms_norm_backward: dy %s has no columns" % (tuple(dy.shape),))
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return rms_norm_backward(dy, h, weight, rstd, dh, need_dx, need_dweight)
     w = _norm_vector(weight, cols, "weight", dev)
     r = _norm_vector(rstd, rows, "rstd", dev)
     dx = torch.empty((rows, cols), dtype=dy.dtype, device=dev) if need_dx else None
@@ -1197,7 +1201,7 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dx=True, need_dweight=T
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _lib.check(L.aq_rms_norm_bwd(dy.data_ptr(), ldd, dh.data_ptr() if dh is not None else None, lddh, h.data_ptr(), ldh, _lib.ELEMENT_TYPES[dy.dtype],
                                  w, r, rows, cols, dx.data_ptr() if need_dx else None, cols, dw.data_ptr() if need_dweight else None,
-                                 ws.data_ptr() if nbytes else None, nbytes, _stream_of(dev)))
+                                 ws.data_ptr() if nbytes else None, nbytes, _current_stream(dev.index)))
     return dx, dw
 
 
@@ -1205,34 +1209,38 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dx=True, need_dweight=T
 
 def _grad_lists(tensors):
     """(addresses, sizes, types) of a list of gradients as arrays, and their device; checked in bulk, a training step has many."""
+    T = torch.Tensor
     dev = tensors[0].device
-    ptrs = array.array("q", [t.data_ptr() for t in tensors])
-    sizes = array.array("q", [t.numel() for t in tensors])
-    try:
-        types = array.array("i", [_lib.ELEMENT_TYPES[t.dtype] for t in tensors])
-    except KeyError:
-        types = None
-    if types is None or not all([t.is_contiguous() for t in tensors]) or len({t.get_device() for t in tensors}) != 1 or dev.type != "cuda":
+    ptrs = array.array("q", map(T.data_ptr, tensors))
+    sizes = array.array("q", map(T.numel, tensors))
+    kinds = {t.dtype for t in tensors}
+    if dev.type != "cuda" or not kinds <= _lib.ELEMENT_TYPES.keys() or not all(map(T.is_contiguous, tensors)) or len(set(map(T.get_device, tensors))) != 1:
         for i, t in enumerate(tensors):
             _hip(t, "tensor[%d]" % i)
             if t.device != dev or t.dtype not in _lib.ELEMENT_TYPES or not t.is_contiguous():
                 raise ValueError("tensor[%d]: %s on %s, strides %s: contiguous float32, bfloat16 or float16 tensors of one device are expected" % (
                     i, t.dtype, t.device, t.stride()))
+    if len(kinds) == 1:
+        types = array.array("i", [_lib.ELEMENT_TYPES[kinds.pop()]]) * len(ptrs)
+    else:
+        types = array.array("i", [_lib.ELEMENT_TYPES[t.dtype] for t in tensors])
     return ptrs, sizes, types, dev
 
 
 def _grad_norm(ptrs, outs, sizes, types, dev, max_norm):
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return _grad_norm(ptrs, outs, sizes, types, dev, max_norm)
     L = _lib.lib()
     norm = torch.empty((), dtype=torch.float32, device=dev)
     n, at = len(ptrs), sizes.buffer_info()[0]
     nbytes = L.aq_clip_grad_norm_workspace_bytes(at, n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.check(L.aq_clip_grad_norm(ptrs.buffer_info()[0], outs.buffer_info()[0] if outs is not None else None, at, types.buffer_info()[0], n, max_norm,
-                                   norm.data_ptr(), ws.data_ptr(), nbytes, _stream_of(dev)))
+                                   norm.data_ptr(), ws.data_ptr(), nbytes, _current_stream(dev.index)))
     return norm
 
 
-@_on_device
 def grad_norm(tensors):
     """sqrt(sum of squares of all elements of all tensors), fp32 0-dim device tensor (sums in double)."""
     if len(tensors) == 0:
@@ -1241,7 +1249,6 @@ def grad_norm(tensors):
     return _grad_norm(ptrs, None, sizes, types, dev, 0.0)
 
 
-@_on_device
 def clip_grad_norm(tensors, max_norm, out=None):
     """Scales all tensors by min(1, max_norm / (norm + 1e-6)), norm = sqrt(sum of squares of all their elements): in place, or into
     the tensors of `out` (as many elements, of the same types).  -> norm, fp32 0-dim device tensor.  The host does not wait; a NaN
