@@ -126,7 +126,9 @@ template <bool NT, typename T> __device__ inline void store8_any(T *p, const flo
     store_any<NT>(u4_t{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])}, reinterpret_cast<u4_any *>(p));
 }
 // Calls that move more than this many bytes (half the last-level cache, the rest being what other kernels have there) stream.
-// Measured at 134 + 134 MB of the quantiser: 66 us with plain accesses, 57 us streaming; at 34 + 34 MB no difference.
+// Measured at 134 + 134 MB of the quantiser: 66 us with plain accesses, 57 us streaming; at 34 + 34 MB no difference.  Rows that do
+// not start at multiples of 16 bytes never stream: their accesses share lines, which streaming fetches again (norm backward,
+// 4096 x 4097 bf16: 49 us streaming against 30).
 constexpr long long STREAM_BYTES = 128LL << 20;
 
 // the first n (0..8) of eight elements; the others read as zero and are not written
@@ -260,6 +262,8 @@ template <typename T> __device__ inline void column_amax8(const raw8<T> (&r)[8],
         m[j] = amax8(v);
     }
 }
+
+inline bool rows16(const void *p, long long ld, int size) { return !p || (((uintptr_t)p & 15) == 0 && ld * size % 16 == 0); }
 
 template <typename F> inline int by_type(int type, F f)
 {

@@ -236,7 +236,8 @@ static long long blocks_of(long long n, int b) { return (n + b - 1) / b; }
 template <typename T> static void launch_tiles(const TileArgs &a, long long tiles, bool square, hipStream_t st)
 {
     const dim3 g((unsigned)tiles), b(256);
-    const bool stream = a.rows * a.cols * (long long)(sizeof(T) + (a.q ? 1 : 0) + (a.qt ? 1 : 0)) > STREAM_BYTES;
+    const bool stream = a.rows * a.cols * (long long)(sizeof(T) + (a.q ? 1 : 0) + (a.qt ? 1 : 0)) > STREAM_BYTES && rows16(a.x, a.ldx, sizeof(T)) &&
+                        rows16(a.q, a.ldq, 1) && rows16(a.qt, a.ldqt, 1);
     if (square) hipLaunchKernelGGL((fp8_tile_kernel<T, true, false>), g, b, 0, st, a);  // weights: the codes are read soon
     else if (stream) hipLaunchKernelGGL((fp8_tile_kernel<T, false, true>), g, b, 0, st, a);
     else hipLaunchKernelGGL((fp8_tile_kernel<T, false, false>), g, b, 0, st, a);
@@ -282,7 +283,7 @@ int aq_fp8_quantize(const void *x, int xtype, long long rows, long long cols, lo
             const dim3 g((unsigned)blocks_of(total, 64)), b(256);
             by_type(xtype, [&](auto *t) {
                 using T = std::remove_pointer_t<decltype(t)>;
-                if (rows * cols * (long long)(sizeof(T) + 1) > STREAM_BYTES)
+                if (rows * cols * (long long)(sizeof(T) + 1) > STREAM_BYTES && rows16(x, ldx, sizeof(T)) && rows16(q, ldq, 1))
                     hipLaunchKernelGGL((fp8_rows_kernel<T, true>), g, b, 0, st, static_cast<const T *>(x), ldx, q, ldq, qs, ldqs, (uint32_t)nblk, (uint32_t)total,
                                        (int)cols, scale_f32);
                 else
@@ -343,7 +344,7 @@ int aq_fp8_dequantize(const uint8_t *q, long long ldq, const void *qs, long long
     hipStream_t st = static_cast<hipStream_t>(stream);
     by_type(ytype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (rows * cols * (long long)(1 + sizeof(T)) > STREAM_BYTES)
+        if (rows * cols * (long long)(1 + sizeof(T)) > STREAM_BYTES && rows16(q, ldq, 1) && rows16(y, ldy, sizeof(T)))
             hipLaunchKernelGGL((fp8_values_kernel<T, true>), g, b, 0, st, q, ldq, qs, ldqs, (uint32_t)rows, (int)cols, (uint32_t)chunks, shift, scale_f32,
                                static_cast<T *>(y), ldy);
         else

@@ -257,22 +257,24 @@ __global__ __launch_bounds__(256) void rms_norm_dw_long_kernel(const NormBwdArgs
     a.part[(long long)slice * a.cols + c] = s;
 }
 
-// dw: 64 columns and 16 runs of the partial rows a workgroup, summed in double in a fixed order
+// dw: 16 columns and 64 runs of the partial rows a workgroup, summed in double in a fixed order
 __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float *__restrict__ part, int n, long long cols, float *__restrict__ dw)
 {
-    __shared__ double sh[16][64];
-    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
-    const long long c = (long long)blockIdx.x * 64 + lane;
+    __shared__ double sh[64][16];
+    const int lane = threadIdx.x & 15, run = threadIdx.x >> 4;
+    const long long c = (long long)blockIdx.x * 16 + lane;
     double s = 0.0;
     if (c < cols) {
 #pragma unroll 4
-        for (int i = run; i < n; i += 16) s += (double)part[i * cols + c];
+        for (int i = run; i < n; i += 64) s += (double)part[i * cols + c];
     }
     sh[run][lane] = s;
     __syncthreads();
-    if (run || c >= cols) return;
-    for (int i = 1; i < 16; ++i) s += sh[i][lane];
-    dw[c] = (float)s;
+    for (int half = 32; half >= 1; half >>= 1) {
+        if (run < half) sh[run][lane] += sh[run + half][lane];
+        __syncthreads();
+    }
+    if (run == 0 && c < cols) dw[c] = (float)sh[0][lane];
 }
 
 constexpr long long NORM_LONG = 1024 * 4 * 8, NORM_BWD_LONG = 1024 * 2 * 8;  // columns that fit the registers of a workgroup
@@ -309,7 +311,8 @@ int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldr
         }
         // few chunks a thread while a workgroup stays small enough to have several of them on a compute unit
         const long long each = cols * type_size(type);
-        const bool stream = rows * (each + (res ? each : 0) + (h ? each : 0) + (y ? each : 0) + (q ? cols : 0)) > STREAM_BYTES;
+        const bool stream = rows * (each + (res ? each : 0) + (h ? each : 0) + (y ? each : 0) + (q ? cols : 0)) > STREAM_BYTES &&
+                            rows16(x, ldx, sizeof(T)) && rows16(res, ldres, sizeof(T)) && rows16(y, ldy, sizeof(T)) && rows16(h, ldh, sizeof(T)) && rows16(q, ldq, 1);
         const dim3 g((unsigned)rows);
         auto launch = [&](auto v) {
             constexpr int V = decltype(v)::value;
@@ -357,7 +360,8 @@ int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long ld
                 return 0;
             }
             const long long each = cols * type_size(type);
-            const bool stream = rows * (2 * each + (dh ? each : 0) + (dx ? each : 0)) > STREAM_BYTES;
+            const bool stream = rows * (2 * each + (dh ? each : 0) + (dx ? each : 0)) > STREAM_BYTES && rows16(dy, lddy, sizeof(T)) &&
+                                rows16(h, ldh, sizeof(T)) && rows16(dh, lddh, sizeof(T)) && rows16(dx, lddx, sizeof(T));
             auto launch = [&](auto v) {
                 constexpr int V = decltype(v)::value;
                 if (stream) hipLaunchKernelGGL((rms_norm_bwd_kernel<T, V, true>), dim3((unsigned)parts), dim3(norm_threads(cols, V)), 0, st, a);
@@ -369,7 +373,7 @@ int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long ld
         });
         if (int rc = check_launch("aq_rms_norm_bwd")) return rc;
     }
-    if (dw) hipLaunchKernelGGL(rms_norm_dw_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, st, a.part, parts, cols, dw);
+    if (dw) hipLaunchKernelGGL(rms_norm_dw_kernel, dim3((unsigned)((cols + 15) / 16)), dim3(1024), 0, st, a.part, parts, cols, dw);
     return check_launch("aq_rms_norm_bwd");
 }
 
