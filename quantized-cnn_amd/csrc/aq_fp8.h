@@ -107,6 +107,33 @@ template <typename T> __device__ inline raw8<T> load_raw_n(const T *p, int n)
         if (i < n) r.a[i / PER] |= (uint32_t)p[i].b << 32 / PER * (i % PER);
     return r;
 }
+// A row's eight elements from column c, for rows of eight elements or more, whose end may lie within them or before them: the eight are
+// read from where the row's last eight begin at the latest, so every lane has one whole access in flight and waits at its use,
+// where row_chunk() moves the elements to their places and puts zeros behind the row's end.
+template <bool NT, typename T> __device__ inline raw8<T> load_row_chunk(const T *row, long long c, long long cols)
+{
+    return load_raw<NT>(row + (c < cols - 8 ? c : cols - 8));
+}
+template <typename T> __device__ inline raw8<T> row_chunk(raw8<T> r, long long c, long long cols)
+{
+    const long long over = c - (cols - 8);
+    if (over <= 0) return r;
+    constexpr int N = 2 * sizeof(T);  // 32-bit words
+    uint32_t w[N];
+    __builtin_memcpy(w, &r, sizeof(w));
+    const int bytes = over >= 8 ? 8 * (int)sizeof(T) : (int)over * (int)sizeof(T);
+#pragma unroll
+    for (int step = N; step >= 1; step >>= 1)
+        if (bytes & 4 * step) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = i + step < N ? w[i + step < N ? i + step : 0] : 0;
+        }
+    const int bits = (bytes & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_alignbit(i + 1 < N ? w[i + 1 < N ? i + 1 : 0] : 0, w[i], bits);
+    __builtin_memcpy(&r, w, sizeof(w));
+    return r;
+}
 __device__ inline float value(const raw8<float> &r, int i) { return i < 4 ? r.a[i & 3] : r.b[i & 3]; }
 __device__ inline float value(const raw8<bf16_el> &r, int i) { return __uint_as_float(i & 1 ? r.a[i >> 1] & 0xffff0000u : r.a[i >> 1] << 16); }
 __device__ inline float value(const raw8<f16_el> &r, int i) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(r.a[i >> 1] >> 16 * (i & 1))); }

@@ -30,6 +30,12 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T *__restrict__ x, 
     if (cols % FP8_BLK == 0 && (blockIdx.x + 1) * (16 * U) <= total) {
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = load_raw<NT>(x + (long long)row[u] * ldx + blk[u] * FP8_BLK + c0);
+    } else if (cols >= 8) {
+        const uint32_t last = (total - 1) / nblk;
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load_row_chunk<NT>(x + (long long)min(row[u], last) * ldx, blk[u] * FP8_BLK + c0, cols);
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = row_chunk(v[u], n[u] > 0 ? blk[u] * FP8_BLK + c0 : cols, cols);
     } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = load_raw_n(x + (long long)row[u] * ldx + blk[u] * FP8_BLK + c0, n[u]);
@@ -83,6 +89,12 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const TileArgs a)
     if (r0 + FP8_BLK <= a.rows && cbase + FP8_BLK <= a.cols) {  // the same in all lanes: all loads in flight at once
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = load_raw<NT>(p + i * a.ldx);
+    } else if (a.cols >= 8) {
+        const T *first = static_cast<const T *>(a.x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = load_row_chunk<NT>(first + min(r0 + 8 * rg + i, a.rows - 1) * a.ldx, c0, a.cols);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = row_chunk(x[i], r0 + 8 * rg + i < a.rows ? c0 : a.cols, a.cols);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = load_raw_n(p + i * a.ldx, r0 + 8 * rg + i < a.rows ? ncol : 0);

@@ -43,12 +43,12 @@ struct NormArgs {
     int scale_f32;
 };
 
-template <bool NT, typename T> __device__ inline void norm_outputs(const NormArgs &a, long long r, long long c, int n, const float (&hv)[8], float rs)
+template <bool NT, typename T>
+__device__ inline void norm_outputs(const NormArgs &a, long long r, long long c, int n, const float (&hv)[8], const raw8<float> &w, float rs)
 {
-    float wv[8], o[8];
-    load_n(a.w + c, n, wv);
+    float o[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = (hv[j] * rs) * wv[j];
+    for (int j = 0; j < 8; ++j) o[j] = (hv[j] * rs) * value(w, j);
     if (a.y) store_n<NT>(static_cast<T *>(a.y) + r * a.ldy + c, n, o);
     if (a.q) {
         const int e = scale_exponent(max16(amax8(o)));  // 16 lanes with 8 elements each: one block
@@ -66,18 +66,28 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_kernel(const NormArgs a)
     const int T0 = (int)blockDim.x;
     const T *x = static_cast<const T *>(a.x) + r * a.ldx, *res = static_cast<const T *>(a.res) + r * a.ldres;
     raw8<T> xv[V], rv[V];
-    if (a.cols == T0 * V * 8) {  // the same in all lanes: all loads in flight at once
+    raw8<float> wv[V];
+    if (a.cols >= 8) {  // the same in all lanes: all loads in flight at once
 #pragma unroll
-        for (int i = 0; i < V; ++i) xv[i] = load_raw<NT>(x + (i * T0 + threadIdx.x) * 8);
+        for (int i = 0; i < V; ++i) xv[i] = load_row_chunk<NT>(x, (i * T0 + threadIdx.x) * 8, a.cols);
         if (a.res)
 #pragma unroll
-            for (int i = 0; i < V; ++i) rv[i] = load_raw<NT>(res + (i * T0 + threadIdx.x) * 8);
+            for (int i = 0; i < V; ++i) rv[i] = load_row_chunk<NT>(res, (i * T0 + threadIdx.x) * 8, a.cols);
+#pragma unroll
+        for (int i = 0; i < V; ++i) wv[i] = load_row_chunk<false>(a.w, (i * T0 + threadIdx.x) * 8, a.cols);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = (i * T0 + threadIdx.x) * 8;
+            xv[i] = row_chunk(xv[i], c, a.cols);
+            if (a.res) rv[i] = row_chunk(rv[i], c, a.cols);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = (i * T0 + threadIdx.x) * 8, n = (int)min(8LL, a.cols - c);
             xv[i] = load_raw_n(x + c, n);
             if (a.res) rv[i] = load_raw_n(res + c, n);
+            wv[i] = load_raw_n(a.w + c, n);
         }
     }
     float hv[V][8];
@@ -97,7 +107,7 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_kernel(const NormArgs a)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = (i * T0 + threadIdx.x) * 8;
-        norm_outputs<NT, T>(a, r, c, (int)max(0LL, min(8LL, a.cols - c)), hv[i], rs);
+        norm_outputs<NT, T>(a, r, c, (int)max(0LL, min(8LL, a.cols - c)), hv[i], a.cols >= 8 ? row_chunk(wv[i], c, a.cols) : wv[i], rs);
     }
 }
 
@@ -136,7 +146,7 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_long_kernel(const NormArgs 
         float hv[8];
         if (a.h) load_n(static_cast<const T *>(h) + c, n, hv);  // (its own store: h may be x or res itself)
         else row_chunk(c, n, hv);
-        norm_outputs<false, T>(a, r, c, n, hv, rs);
+        norm_outputs<false, T>(a, r, c, n, hv, load_raw_n(a.w + c, n), rs);
     }
 }
 
@@ -155,7 +165,6 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
 {
     __shared__ float sh[16];
     const int T0 = (int)blockDim.x;
-    const bool whole = a.cols == T0 * V * 8;
     float wv[V][8], acc[V][8];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -171,13 +180,13 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
         const T *dy = static_cast<const T *>(a.dy) + r * a.lddy, *h = static_cast<const T *>(a.h) + r * a.ldh;
         const T *dh = static_cast<const T *>(a.dh) + r * a.lddh;
         rsn = a.rstd[r];
-        if (whole) {
+        if (a.cols >= 8) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int c = (i * T0 + threadIdx.x) * 8;
-                dyn[i] = load_raw<NT>(dy + c);
-                hn[i] = load_raw<NT>(h + c);
-                if (a.dh && a.dx) dhn[i] = load_raw<NT>(dh + c);
+                dyn[i] = load_row_chunk<NT>(dy, c, a.cols);
+                hn[i] = load_row_chunk<NT>(h, c, a.cols);
+                if (a.dh && a.dx) dhn[i] = load_row_chunk<NT>(dh, c, a.cols);
             }
         } else {
 #pragma unroll
@@ -195,7 +204,12 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
         if (V > 1) load(r);
         const float rs = rsn;
 #pragma unroll
-        for (int i = 0; i < V; ++i) dyv[i] = dyn[i], hv[i] = hn[i], dhv[i] = dhn[i];
+        for (int i = 0; i < V; ++i) {
+            const int c = (i * T0 + threadIdx.x) * 8;
+            dyv[i] = a.cols >= 8 ? row_chunk(dyn[i], c, a.cols) : dyn[i];
+            hv[i] = a.cols >= 8 ? row_chunk(hn[i], c, a.cols) : hn[i];
+            if (a.dh && a.dx) dhv[i] = a.cols >= 8 ? row_chunk(dhn[i], c, a.cols) : dhn[i];
+        }
         if (V == 1 && r + gridDim.x < a.rows) load(r + gridDim.x);
         float s = 0.0f;
 #pragma unroll
