@@ -173,6 +173,7 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
     }
+    const bool shifted = V == 1 && a.cols >= 8;  // two chunks shifted, or two of dh read early, do not fit the 128 registers of a thread
     const float inv = 1.0f / (float)a.cols;
     raw8<T> dyn[V], hn[V], dhn[V];
     float rsn = 0.0f;
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
         const T *dy = static_cast<const T *>(a.dy) + r * a.lddy, *h = static_cast<const T *>(a.h) + r * a.ldh;
         const T *dh = static_cast<const T *>(a.dh) + r * a.lddh;
         rsn = a.rstd[r];
-        if (a.cols >= 8) {
+        if (shifted) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int c = (i * T0 + threadIdx.x) * 8;
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
                 const int c = (i * T0 + threadIdx.x) * 8, k = (int)max(0LL, min(8LL, a.cols - c));
                 dyn[i] = load_raw_n(dy + c, k);
                 hn[i] = load_raw_n(h + c, k);
-                if (a.dh && a.dx) dhn[i] = load_raw_n(dh + c, k);
+                if (V == 1 && a.dh && a.dx) dhn[i] = load_raw_n(dh + c, k);
             }
         }
     };
@@ -206,9 +207,9 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = (i * T0 + threadIdx.x) * 8;
-            dyv[i] = a.cols >= 8 ? row_chunk(dyn[i], c, a.cols) : dyn[i];
-            hv[i] = a.cols >= 8 ? row_chunk(hn[i], c, a.cols) : hn[i];
-            if (a.dh && a.dx) dhv[i] = a.cols >= 8 ? row_chunk(dhn[i], c, a.cols) : dhn[i];
+            dyv[i] = shifted ? row_chunk(dyn[i], c, a.cols) : dyn[i];
+            hv[i] = shifted ? row_chunk(hn[i], c, a.cols) : hn[i];
+            if (V == 1 && a.dh && a.dx) dhv[i] = shifted ? row_chunk(dhn[i], c, a.cols) : dhn[i];
         }
         if (V == 1 && r + gridDim.x < a.rows) load(r + gridDim.x);
         float s = 0.0f;
@@ -225,13 +226,15 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int c = (i * T0 + threadIdx.x) * 8;
+            const int k = (int)max(0LL, min(8LL, a.cols - c));
+            if (V > 1 && a.dh) dhv[i] = load_raw_n(static_cast<const T *>(a.dh) + r * a.lddh + c, k);
             float o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float d = rs * __builtin_fmaf(-(value(hv[i], j) * rs), m, value(dyv[i], j) * wv[i][j]);
                 o[j] = a.dh ? d + value(dhv[i], j) : d;
             }
-            store_n<NT>(static_cast<T *>(a.dx) + r * a.lddx + c, (int)max(0LL, min(8LL, a.cols - c)), o);
+            store_n<NT>(static_cast<T *>(a.dx) + r * a.lddx + c, k, o);
         }
     }
     if (!a.part) return;
