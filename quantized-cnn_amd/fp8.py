@@ -19,8 +19,10 @@ from . import ops
 
 
 def _flat(t):
-    """(..., n) -> (rows, n), a view where the strides allow it."""
-    return t if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1) else t.reshape(-1, t.shape[-1]).contiguous()
+    """(..., n) -> (rows, n), a view where the strides allow it (rows that share memory, as a broadcast gradient's do, are copied)."""
+    if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] <= 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
+        return t
+    return t.reshape(-1, t.shape[-1]).contiguous()
 
 
 def _weight_forms(weight, need_dx):

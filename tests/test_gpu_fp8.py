@@ -772,3 +772,26 @@ def test_train_step_clips():
         l1, l2 = float(s1(x, y)), float(s2(x, y))
         assert abs(l1 - l2) <= 1e-4 * abs(l1)
         assert float(s1.grad_norm) > 0.1 and abs(float(s1.grad_norm) - float(s2.grad_norm)) <= 1e-2 * float(s1.grad_norm)
+
+
+def test_gradients_and_inputs_whose_rows_share_memory():
+    x, w, b = torch.randn(20, 130, device=DEV), torch.randn(130, 40, device=DEV), torch.randn(40, device=DEV)
+    v, nw = torch.randn(40, device=DEV), torch.rand(130, device=DEV) + 0.5
+    leaves = [t.requires_grad_(True) for t in (x, nw, w, b)]
+    r = torch.randn(130, device=DEV)
+
+    def grads_of(call, reduce):
+        return torch.autograd.grad(reduce(call()), leaves, allow_unused=True)
+    for call in (lambda: fp8.linear(x, w, b), lambda: fp8.norm_linear(x, nw, w, b), lambda: fp8.norm_linear(x, nw, w, b, residual=r.expand(20, 130))[0],
+                 lambda: fp8.linear(fp8.rms_norm(x, nw, residual=r.expand(20, 130))[0], w, b)):
+        want = grads_of(call, lambda y: (y * v.repeat(20, 1)).sum())  # a gradient with rows of its own
+        got = grads_of(call, lambda y: (y.sum(0) * v).sum())          # one row for all
+        assert all(a is None and c is None or torch.equal(a, c) for a, c in zip(got, want))
+        assert all(a is None or bool(torch.isfinite(a).all()) for a in got)
+    with torch.no_grad():
+        assert torch.equal(fp8.linear(x[:1].expand(20, 130), w, b), fp8.linear(x[:1], w, b).expand(20, 40))
+        h = fp8.rms_norm(x, nw, residual=r.expand(20, 130))[1]
+        assert torch.equal(h, x + r)
+    # h's own gradient, one row for all
+    g = torch.autograd.grad((fp8.rms_norm(x, nw, residual=r.expand(20, 130))[1].sum(0) * r).sum(), (x,))[0]
+    assert torch.equal(g, r.expand(20, 130))
