@@ -115,6 +115,11 @@ class _NormLinear(torch.autograd.Function):
         return dx, dnw, dw, db.to(btype) if need_db else None, dx if ctx.both else None, None, None
 
 
+def _check_residual(name, x, residual):
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError("fp8.%s: residual %s, expected x's shape %s" % (name, tuple(residual.shape), tuple(x.shape)))
+
+
 def linear(x, weight, bias=None, out_dtype=None):
     """x (..., in) @ weight + bias in 8-bit floating point; out_dtype defaults to x's.  weight: (in, out) tensor, quantised in
     this call, or Fp8Blocks (out, in) made before (no gradient of the weight then, and none of x)."""
@@ -133,6 +138,7 @@ def linear(x, weight, bias=None, out_dtype=None):
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight over the last axis -> (y, h), or y alone without residual."""
+    _check_residual("rms_norm", x, residual)
     out = _RmsNorm.apply(_flat(x), weight.float(), _flat(residual) if residual is not None else None, eps)
     if residual is None:
         return out.view(x.shape)
@@ -144,6 +150,7 @@ def norm_linear(x, norm_weight, weight, bias=None, residual=None, eps=1e-6, out_
     without residual."""
     if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
         raise ValueError("fp8.norm_linear: x %s / weight %s: need (..., in) and (in, out)" % (tuple(x.shape), tuple(weight.shape)))
+    _check_residual("norm_linear", x, residual)
     out = _NormLinear.apply(_flat(x), norm_weight.float(), weight, bias, _flat(residual) if residual is not None else None, eps, out_dtype or x.dtype)
     y, h = out if residual is not None else (out, None)
     y = y.view(x.shape[:-1] + (y.shape[1],))

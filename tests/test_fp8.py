@@ -110,3 +110,13 @@ def test_training_steps_check_max_norm():
     for bad in (0, -1.0, float("nan")):
         with pytest.raises(ValueError, match="max_norm"):
             train.CapturedStep(m, torch.optim.SGD(m.parameters(), 0.1), torch.nn.functional.mse_loss, max_norm=bad)
+
+
+def test_a_residual_of_another_shape_is_refused():
+    from quantized_cnn_amd import fp8
+    x, w = torch.randn(4, 6, 128), torch.ones(128)
+    for r in (torch.randn(6, 4, 128), torch.randn(24, 128), torch.randn(128)):  # as many elements, or fewer
+        with pytest.raises(ValueError, match="residual"):
+            fp8.rms_norm(x, w, residual=r)
+        with pytest.raises(ValueError, match="residual"):
+            fp8.norm_linear(x, w, torch.randn(128, 8), residual=r)
