@@ -1052,6 +1052,7 @@ int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long lda
     // a launch holds fewer than 2^32 threads; offsets within a tile have 32 bits
     AQ_REQUIRE(M < (1LL << 26) && N < (1LL << 26) && M * N < (1LL << 38), -E2BIG, "aq_fp8_matmul: M=%lld N=%lld K=%lld is too large for one call", M, N, K);
     AQ_REQUIRE(lda < (1LL << 24) && ldb < (1LL << 24), -E2BIG, "aq_fp8_matmul: a pitch of %lld bytes is too large", std::max(lda, ldb));
+    AQ_REQUIRE(ldas < (1LL << 24) && ldbs < (1LL << 24), -E2BIG, "aq_fp8_matmul: a pitch of %lld scales is too large", std::max(ldas, ldbs));
     if (M == 0 || N == 0) return 0;
     AQ_REQUIRE(a && as && b && bs && y, -EFAULT, "aq_fp8_matmul: NULL pointer");
     const long long nkb = (K + FP8_BLK - 1) / FP8_BLK;

@@ -120,3 +120,10 @@ def test_a_residual_of_another_shape_is_refused():
             fp8.rms_norm(x, w, residual=r)
         with pytest.raises(ValueError, match="residual"):
             fp8.norm_linear(x, w, torch.randn(128, 8), residual=r)
+
+
+@pytest.mark.parametrize("ldas,ldbs", [(1 << 24, 1), (1, 1 << 30)])
+def test_matmul_refuses_scales_too_far_apart(ldas, ldbs):
+    """(the offsets of a tile's scales have 32 bits)"""
+    rc, err = _rc("aq_fp8_matmul", P, 128, P, ldas, 1, P, 128, P, ldbs, 1, 256, 256, 128, 0, None, P, 1, 256, None, 0, None)
+    assert rc < 0 and "pitch" in err and "scales" in err
