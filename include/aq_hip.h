@@ -486,7 +486,8 @@ int aq_fp8_dequantize(const uint8_t *q, long long ldq, const void *qs, long long
  * the next multiple of 16 bytes (what lies behind K does not matter).  Sums in fp32.  bf16 / fp16 outputs: the 8-bit matrix
  * instructions, which align the products of a group of 8 to the largest of them and drop what lies 2^-14 below it; fp32
  * output: the codes as fp16 through the 16-bit instructions, whose sums keep fp32.  workspace:
- * aq_fp8_matmul_workspace_bytes(M, N, K) bytes, 16-byte aligned (partial sums of products with few tiles and long rows). */
+ * aq_fp8_matmul_workspace_bytes(M, N, K) bytes, 16-byte aligned (partial sums of products with few tiles and long rows).
+ * One call takes M and N below 2^26, M * N below 2^38, pitches of codes and scales below 2^24. */
 size_t aq_fp8_matmul_workspace_bytes(long long M, long long N, long long K);
 int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long ldas, int a_block_rows, const uint8_t *b, long long ldb,
                   const void *bs, long long ldbs, int b_block_rows, long long M, long long N, long long K, int scale_type,
@@ -495,7 +496,7 @@ int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long lda
 /* ---- root-mean-square norm over rows, with the residual's addition ---------------------------------------------------
  * h = round(x + res) (h = x without res), rstd = 1 / sqrt(mean(h^2) + eps), y = (h * rstd) * w; x, res, h, y of one type, w and
  * rstd fp32.  Outputs that are not wanted are NULL.  q / qs: y in blocks of 1 x 128 as aq_fp8_quantize makes them, instead
- * of or beside y.  h may be x or res itself (in place). */
+ * of or beside y.  h may be x or res itself (in place).  One call takes fewer than 2^22 rows, here and below. */
 int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldres, int type, const float *w, long long rows,
                     long long cols, double eps, void *y, long long ldy, uint8_t *q, long long ldq, void *qs, long long ldqs, int scale_type,
                     void *h, long long ldh, float *rstd, void *stream);

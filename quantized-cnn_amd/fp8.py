@@ -27,10 +27,31 @@ def _flat(t):
 
 def _weight_forms(weight, need_dx):
     """-> (codes of weight^T for the forward product, codes of weight for the input gradient or None)."""
+    if weight.stride(1) != 1 and weight.stride(0) == 1:  # a transposed view: tiles are square, so its transpose has the same codes
+        got = ops.fp8_quantize(_flat(weight.t()), forms="both" if need_dx else "rows", block_rows=ops.FP8_BLOCK)
+        return got if need_dx else (got, None)
     if need_dx:
-        rows, cols = ops.fp8_quantize(weight, forms="both", block_rows=ops.FP8_BLOCK)
+        rows, cols = ops.fp8_quantize(_flat(weight), forms="both", block_rows=ops.FP8_BLOCK)
         return cols, rows
-    return ops.fp8_quantize(weight, forms="cols", block_rows=ops.FP8_BLOCK), None
+    return ops.fp8_quantize(_flat(weight), forms="cols", block_rows=ops.FP8_BLOCK), None
+
+
+def _checked(out):
+    """out, the result of a Function's apply, after a check of the leaves among its arguments.  A leaf's gradient is accumulated on the stream
+    that was current when its first graph was made.  If that graph lives on and was made on the default stream, a backward pass in a
+    capture would make that stream wait for the capture, which ends the process: it is refused here, where nothing is lost yet."""
+    fn = (out[0] if isinstance(out, tuple) else out).grad_fn
+    if fn is not None:
+        capturing = torch.cuda.is_current_stream_capturing()
+        eager = not capturing and torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()) == 0
+        for node, _ in fn.next_functions:
+            if node is not None and type(node).__name__ == "AccumulateGrad":
+                if capturing and node.metadata.get("fp8_default_stream"):
+                    raise RuntimeError("fp8: a graph of the same parameters, made on the default stream, is still alive (a loss or an output is kept): "
+                                       "its gradients cannot be captured; delete or detach it before the capture")
+                if eager:
+                    node.metadata.setdefault("fp8_default_stream", True)
+    return out
 
 
 def _grad_forms(dy, need_dx, need_dw, need_db):
@@ -132,26 +153,28 @@ def linear(x, weight, bias=None, out_dtype=None):
     else:
         if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
             raise ValueError("fp8.linear: x %s / weight %s: need (..., in) and (in, out)" % (tuple(x.shape), tuple(weight.shape)))
-        y = _Linear.apply(x2, weight, bias, out_dtype)
+        y = _checked(_Linear.apply(x2, weight, bias, out_dtype))
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (y.shape[1],))
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight over the last axis -> (y, h), or y alone without residual."""
     _check_residual("rms_norm", x, residual)
-    out = _RmsNorm.apply(_flat(x), weight.float(), _flat(residual) if residual is not None else None, eps)
+    out = _checked(_RmsNorm.apply(_flat(x), weight.float(), _flat(residual) if residual is not None else None, eps))
     if residual is None:
         return out.view(x.shape)
     return out[0].view(x.shape), out[1].view(x.shape)
 
 
 def norm_linear(x, norm_weight, weight, bias=None, residual=None, eps=1e-6, out_dtype=None):
-    """linear(rms_norm(x, norm_weight, residual), weight, bias) with the norm's output kept as codes only -> (y, h), or y alone
+    """linear(rms_norm(x, norm_weight, residual), weight, bias) with the norm's output kept as codes only (made from
+    its fp32 values, without a rounding to x's type between) -> (y, h), or y alone
     without residual."""
     if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
         raise ValueError("fp8.norm_linear: x %s / weight %s: need (..., in) and (in, out)" % (tuple(x.shape), tuple(weight.shape)))
     _check_residual("norm_linear", x, residual)
-    out = _NormLinear.apply(_flat(x), norm_weight.float(), weight, bias, _flat(residual) if residual is not None else None, eps, out_dtype or x.dtype)
+    out = _checked(_NormLinear.apply(_flat(x), norm_weight.float(), weight, bias, _flat(residual) if residual is not None else None, eps,
+                                     out_dtype or x.dtype))
     y, h = out if residual is not None else (out, None)
     y = y.view(x.shape[:-1] + (y.shape[1],))
     return y if residual is None else (y, h.view(x.shape))
@@ -172,7 +195,7 @@ class Fp8Linear(nn.Module):
         """Quantises the weight once, for serving: forward() under no_grad in eval mode then reads the codes.  They are of the weight as
         it is now; train(), load_state_dict() and moving the module drop them."""
         with torch.no_grad():
-            self._packed = ops.fp8_quantize(self.weight, forms="cols", block_rows=ops.FP8_BLOCK)
+            self._packed = _weight_forms(self.weight, False)[0]
         return self
 
     def train(self, mode=True):

@@ -795,3 +795,53 @@ def test_gradients_and_inputs_whose_rows_share_memory():
     # h's own gradient, one row for all
     g = torch.autograd.grad((fp8.rms_norm(x, nw, residual=r.expand(20, 130))[1].sum(0) * r).sum(), (x,))[0]
     assert torch.equal(g, r.expand(20, 130))
+
+
+@pytest.mark.parametrize("n_in,n_out", [(130, 300), (256, 1), (1, 70)])
+def test_weights_that_are_transposed_views(n_in, n_out):
+    x, dy = torch.randn(9, n_in, device=DEV, requires_grad=True), torch.randn(9, n_out, device=DEV)
+    w = torch.randn(n_in, n_out, device=DEV)
+    wt = w.t().contiguous().requires_grad_(True)  # (out, in), as other layers keep it
+    w.requires_grad_(True)
+    y, yt = fp8.linear(x, w), fp8.linear(x, wt.t())
+    assert torch.equal(y, yt)
+    gx, gw = torch.autograd.grad(y, (x, w), dy)
+    hx, hw = torch.autograd.grad(yt, (x, wt), dy)
+    assert torch.equal(gx, hx) and torch.equal(gw, hw.t())
+    with torch.no_grad():
+        assert torch.equal(fp8.linear(x, wt.t()), y)
+        wide = torch.zeros(n_in, 2 * n_out, device=DEV)
+        wide[:, ::2] = w
+        assert torch.equal(fp8.linear(x, wide[:, ::2]), y)  # neither rows nor columns in one piece
+    layer = fp8.Fp8Linear(n_in, n_out, bias=False).to(DEV).eval()
+    layer.weight = torch.nn.Parameter(wt.detach().t())
+    layer.pack()
+    with torch.no_grad():
+        assert torch.equal(layer(x), y)
+
+
+def test_capture_beside_a_live_eager_graph_is_refused():
+    layer, norm = fp8.Fp8Linear(256, 64).to(DEV), fp8.RMSNorm(256).to(DEV)
+    x = torch.randn(32, 256, device=DEV)
+
+    def run():
+        return fp8.norm_linear(norm(x), norm.weight, layer.weight, layer.bias).square().sum()
+    kept = run()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(g):
+            run().backward()
+    torch.cuda.synchronize()
+    kept.backward()  # the eager graph is whole
+    want = [p.grad.clone() for p in (layer.weight, layer.bias, norm.weight)]
+    del kept
+    for p in (layer.weight, layer.bias, norm.weight):
+        p.grad = None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        run().backward()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p.grad, t) for p, t in zip((layer.weight, layer.bias, norm.weight), want))
+        run()  # eager work between the replays
