@@ -956,29 +956,35 @@ template <int BM, int BN, int WM, int WN, int NS, typename T> static void launch
 }
 
 static long long tiles_of(long long M, long long N, long long bm, long long bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); }
-// Parts of K for the 64 x 128 tiles: as many as bring the launch to 256 workgroups, none shorter than four blocks.  Joining them
-// costs about 8 us and a block of K about 0.4 us, so rows of 24 blocks and more only.
+// Parts of K for the 64 x 128 tiles: as many as bring the launch to 256 workgroups, none shorter than four blocks.  Writing and joining
+// them costs 8 to 10 us and a block of K 0.4 us, so they have to save 24 blocks (256 x 2048 x 8192, 64 tiles: 27 -> 16 us; 128 x 8192 x 8192,
+// 128 tiles: 28 -> 23 us; 256 x 4096 x 4096, 128 tiles: 17 us whole, 19 us in two parts).
 static int matmul_splits(long long M, long long N, long long K)
 {
     const long long tiles = tiles_of(M, N, 64, 128), nkb = (K + FP8_BLK - 1) / FP8_BLK;
-    if (M <= 64 || N < 128 || tiles > 32 || nkb < 24) return 1;
-    return (int)std::max(1LL, std::min(256 / tiles, nkb / 4));
+    if (M <= 64 || N < 128 || tiles > 128) return 1;
+    const long long parts = std::min(256 / tiles, nkb / 4);
+    return parts > 1 && nkb * (parts - 1) / parts >= 24 ? (int)parts : 1;
 }
 
 // Tiles by how many of them there are for the 256 compute units (times at 4096-long rows unless stated):
 //   256 x 256 from three quarters of a round on (4096 x 4096: 57 us against 75 us in 128 x 128; 2048 x 4096, half a round: 47 against 38);
 //   128 x 128 with two stages, two workgroups on a unit, for more than a round (1500 x 5000 x 2560: 25 us against 30 us with four stages);
 //   128 x 128 with four stages for up to a round (1024 x 4096: 22 against 28 us with two);
-//   64 x 128 for fewer (512 x 4096: 17 us; 1000 x 1000 x 1000: 8 against 11 us), K in parts for very few.
+//   64 x 128 for fewer (512 x 4096: 17 us; 1000 x 1000 x 1000: 8 against 11 us), K in parts for very few;
+//   32 x 32 from streamed fragments where that is one round and K one round of the wavefronts' loads (256 x 1024: 11.5 us, in 64 x 128 and
+//   parts of K 14 us; 100 x 1000 x 2048: 7.4 against 10.1 us; at K = 8192 the parts win, 512 x 512: 15.6 against 19 us, and so they do
+//   for half a round, 256 x 256: 9.6 against 11.2 us).
 template <typename T> static void launch_pow2(MatArgs p, hipStream_t st)
 {
     if (p.N < 128) return launch_rows<4, 2, 2, POW2, T>(p, st);
     if (p.M >= 256 && p.N >= 256 && tiles_of(p.M, p.N, 256, 256) >= 192) return launch_large<256, 256, 4, 2, 2, T>(p, st);
     if (p.M >= 128 && tiles_of(p.M, p.N, 128, 128) > 256) return launch_large<128, 128, 2, 2, 2, T>(p, st);
     if (p.M >= 128 && tiles_of(p.M, p.N, 64, 128) > 256) return launch_large<128, 128, 2, 2, 4, T>(p, st);
-    const int splits = matmul_splits(p.M, p.N, p.K);
+    const int splits = matmul_splits(p.M, p.N, p.K), nkb = (p.K + FP8_BLK - 1) / FP8_BLK;
+    const long long small = tiles_of(p.M, p.N, 32, 32);
+    if (small <= 256 && nkb <= 32 && (splits == 1 || small > 128)) return launch_rows<2, 2, 4, POW2, T>(p, st);
     if (splits == 1) return launch_large<64, 128, 1, 4, 4, T>(p, st);
-    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK;
     p.split_blocks = (nkb + splits - 1) / splits;
     p.splits = (nkb + p.split_blocks - 1) / p.split_blocks;
     p.tiles_m = (p.M + 63) / 64;
@@ -1019,9 +1025,10 @@ template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t
     if constexpr (MODE == POW2) {
         launch_pow2<T>(p, st);
     } else {
-        // Streamed fragments while their workgroups fit the compute units about once (512 x 1024 x 4096: 19 against 28 us on tiles;
-        // 512 x 2048 x 4096: 35 against 28 us); fp32 outputs with any scales, whose tiles are the slowest, twice (36 against 48 us).
-        if (tiles_of(p.M, p.N, 64, 16) <= 256) return launch_rows<4, 1, 2, MODE, T>(p, st);
+        // Streamed fragments while their workgroups fit the compute units once, in 32 x 32 (256 x 1024 x 4096: 13 us, in 64 x 32 19 us), then in
+        // 64 x 32 (512 x 1024 x 4096: 19 us, in 32 x 32 23 us, on tiles 28 us; 512 x 2048 x 4096: 35 us, on tiles 28 us); fp32 outputs with any
+        // scales, whose tiles are the slowest, for twice as many (36 against 48 us).
+        if (tiles_of(p.M, p.N, 32, 32) <= 256) return launch_rows<2, 2, 2, MODE, T>(p, st);
         const long long few = MODE == EXACT && p.scale_f32 ? 512 : 256;
         if (p.M < 128 || p.N < 128 || tiles_of(p.M, p.N, 64, 32) <= few) return launch_rows<4, 2, 2, MODE, T>(p, st);
         launch_block<MODE, T>(p, st);

@@ -845,3 +845,30 @@ def test_capture_beside_a_live_eager_graph_is_refused():
         torch.cuda.synchronize()
         assert all(torch.equal(p.grad, t) for p, t in zip((layer.weight, layer.bias, norm.weight), want))
         run()  # eager work between the replays
+
+
+@pytest.mark.parametrize("m,n,k", [(400, 700, 1300), (500, 1000, 4100), (130, 2050, 6200), (260, 1930, 6300), (65, 4000, 4200), (127, 2000, 4096), (250, 1020, 4097)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pow2", [True, False])
+def test_product_of_middle_sizes(m, n, k, dtype, pow2):
+    """Around the borders between streamed fragments, tiles of 64 x 128 and parts of K."""
+    check_product(operand(m, k, 1, pow2, m), operand(n, k, 128 if n % 20 else 1, pow2, k), torch.randn(n, device=DEV) if m % 4 else None, dtype)
+
+
+@pytest.mark.parametrize("m,n", [(500, 700), (1030, 1000)])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_special_values_in_middle_sizes(m, n, pow2):
+    for dtype in TYPES:
+        test_product_special_values(m, n, dtype, pow2)
+
+
+@pytest.mark.parametrize("m,n,k", [(500, 700, 200), (130, 1000, 4110), (300, 1000, 600), (1100, 1300, 333), (3600, 3700, 205)])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_larger_products_ignore_what_lies_behind_their_rows(m, n, k, pow2):
+    full = [torch.full((r + 1, k + 60 & ~15), float("nan"), device=DEV).to(torch.float8_e4m3fn) for r in (m, n)]
+    a0, b0 = operand(m, k, 1, pow2, 1, False), operand(n, k, 1, pow2, 2, False)
+    full[0][:m, :k], full[1][:n, :k] = a0.data, b0.data
+    a, b = ops.Fp8Blocks(full[0][:m, :k], a0.scale), ops.Fp8Blocks(full[1][:n, :k], b0.scale)
+    for dtype in TYPES:
+        y = ops.fp8_matmul(a, b, out_dtype=dtype)
+        assert bool(torch.isfinite(y).all()) and torch.equal(y, ops.fp8_matmul(a0, b0, out_dtype=dtype))
