@@ -6,6 +6,7 @@ Sub-modules
   layers        MyConv2d / MyLinear / Residual / PreResidual / ResNet / model_loss drop-ins
   adp_qtz_fan, adp_qtz_fix, adp_qtz_hint
                 per-variant modules with the reference scripts' names and signatures
+  fp8           linear layers in 8-bit floating point, row norm (imported on demand)
   train         training step, HIP-graph capture and data-parallel wrapper
 """
 __all__ = ["_lib", "ops", "layers", "adp_qtz_fan", "adp_qtz_fix", "adp_qtz_hint", "train"]
