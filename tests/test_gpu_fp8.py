@@ -872,3 +872,26 @@ def test_larger_products_ignore_what_lies_behind_their_rows(m, n, k, pow2):
     for dtype in TYPES:
         y = ops.fp8_matmul(a, b, out_dtype=dtype)
         assert bool(torch.isfinite(y).all()) and torch.equal(y, ops.fp8_matmul(a0, b0, out_dtype=dtype))
+
+
+def test_the_largest_products():
+    """Past 2^38 multiplications: rows of the result against float64, odd sizes, and the same product by its halves of K."""
+    m, n, k = 8190, 8130, 4210
+    a, b = operand(m, k, 1, True, 1, False), operand(n, k, 128, True, 2, False)
+    y = ops.fp8_matmul(a, b)
+    for rows in (slice(0, 40), slice(4000, 4040), slice(m - 40, m)):
+        part = ops.Fp8Blocks(a.data[rows].clone(), a.scale[rows].clone())
+        small = check_product(part, b, None, torch.bfloat16)
+        va, vb = ops.fp8_dequantize(part, torch.float32).double(), ops.fp8_dequantize(b, torch.float32).double()
+        mag, want = va.abs() @ vb.abs().t(), va @ vb.t()
+        tol = 2.0 ** -10 * mag + (k + 4 * -(-k // 128)) * 2 * U * mag  # (7 * 2^-13 of a group's largest product is less than 2^-10 of its sum)
+        tol = tol + half_step(torch.bfloat16) * (want.abs() + tol)
+        assert bool(((y[rows].double() - want).abs() <= tol).all())
+        assert np.isfinite(small).all()
+    assert torch.equal(y, ops.fp8_matmul(a, b))
+    a.data[5, k - 1] = float("nan")
+    b.scale[63, 2] = float("nan")  # rows 8064 .. 8129 of b
+    z = ops.fp8_matmul(a, b)
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[5], bad[:, 8064:] = True, True
+    assert torch.equal(torch.isnan(z), bad) and torch.equal(z[~bad], y[~bad])
