@@ -501,7 +501,8 @@ int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldr
                     long long cols, double eps, void *y, long long ldy, uint8_t *q, long long ldq, void *qs, long long ldqs, int scale_type,
                     void *h, long long ldh, float *rstd, void *stream);
 /* dx = rstd * (dy * w - h * rstd^2 * mean(dy * w * h)) + dh (dh: the gradient that arrives at h, NULL: none), dw = sum over rows of
- * dy * h * rstd (dx or dw may be NULL).  dx is the gradient of x and of res alike.  workspace:
+ * dy * h * rstd (dx or dw may be NULL).  dx is the gradient of x and of res alike; it may be dh itself, but
+ * not share memory with dy or h.  workspace:
  * aq_rms_norm_bwd_workspace_bytes(rows, cols) bytes, 16-byte aligned. */
 size_t aq_rms_norm_bwd_workspace_bytes(long long rows, long long cols);
 int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long lddh, const void *h, long long ldh, int type, const float *w,

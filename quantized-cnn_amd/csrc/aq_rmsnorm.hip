@@ -245,6 +245,72 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_kernel(const NormBwdArgs a)
     }
 }
 
+// Few rows: one launch.  The first workgroups have a row of dx each; the others 128 columns of dw each, for which they read all rows
+// again (rstd is known, so dw needs nothing of dx).  dw's terms are summed in double.  A call of 256 x 4096 takes 11.6 us, 15.3 us with a second
+// launch for dw and a workspace for its parts; 512 x 8192 bf16 13 against 21 us; at 1000 x 200, where a workgroup has 32 rows in turn
+// for each of its lanes, 19 against 15 us.
+constexpr int NORM_SMALL_ROWS = 512;
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_bwd_small_kernel(const NormBwdArgs a, float *__restrict__ dw)
+{
+    __shared__ float sh[16];
+    __shared__ double sums[16][16][8];
+    const int rows = (int)a.rows, dx_groups = a.dx ? rows : 0;
+    const bool whole = a.cols >= 8;
+    auto load = [&](const void *p, long long row, long long ld, int c) {
+        const T *at = static_cast<const T *>(p) + row * ld;
+        return whole ? load_row_chunk<false>(at, c, a.cols) : load_raw_n(at + c, (int)max(0LL, min(8LL, a.cols - c)));
+    };
+    auto placed = [&](const raw8<T> &v, int c) { return whole ? row_chunk(v, c, a.cols) : v; };
+    if ((int)blockIdx.x < dx_groups) {
+        const int r = blockIdx.x, c = threadIdx.x * 8, k = (int)max(0LL, min(8LL, a.cols - c));
+        raw8<T> dy = load(a.dy, r, a.lddy, c), h = load(a.h, r, a.ldh, c), dh = {};
+        if (a.dh) dh = load(a.dh, r, a.lddh, c);
+        float wv[8];
+        load_n(a.w + c, k, wv);
+        const float rs = a.rstd[r];
+        dy = placed(dy, c), h = placed(h, c);
+        if (a.dh) dh = placed(dh, c);
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = __builtin_fmaf(value(dy, j) * wv[j], value(h, j) * rs, s);
+        const float m = group_sum(s, sh) * (1.0f / (float)a.cols);
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = rs * __builtin_fmaf(-(value(h, j) * rs), m, value(dy, j) * wv[j]);
+            o[j] = a.dh ? d + value(dh, j) : d;
+        }
+        store_n(static_cast<T *>(a.dx) + r * a.lddx + c, k, o);
+        return;
+    }
+    // 16 lanes along a row, blockDim / 16 rows at a time
+    const int lane = threadIdx.x & 15, c = ((int)blockIdx.x - dx_groups) * 128 + lane * 8, step = (int)blockDim.x / 16;
+    double acc[8] = {};
+#pragma unroll 4
+    for (int r = (int)threadIdx.x >> 4; r < rows; r += step) {
+        const raw8<T> dy = placed(load(a.dy, r, a.lddy, c), c), h = placed(load(a.h, r, a.ldh, c), c);
+        const float rs = a.rstd[r];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = __builtin_fma((double)value(dy, j), (double)(value(h, j) * rs), acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        acc[j] += __shfl_xor(acc[j], 16, 64);
+        acc[j] += __shfl_xor(acc[j], 32, 64);
+    }
+    if ((threadIdx.x & 63) < 16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[threadIdx.x >> 6][lane][j] = acc[j];
+    }
+    __syncthreads();
+    const long long col = ((long long)blockIdx.x - dx_groups) * 128 + threadIdx.x;
+    if (threadIdx.x >= 128 || col >= a.cols) return;
+    double s = 0.0;
+    for (int i = 0; i < (int)blockDim.x / 64; ++i) s += sums[i][threadIdx.x >> 3][threadIdx.x & 7];
+    dw[col] = (float)s;
+}
+
 // rows too long for the registers: dx reads its row twice, dw is a sum over a slice of rows for 256 columns a workgroup
 template <typename T>
 __global__ __launch_bounds__(1024) void rms_norm_dx_long_kernel(const NormBwdArgs a)
@@ -298,6 +364,7 @@ constexpr long long NORM_LONG = 1024 * 4 * 8, NORM_BWD_LONG = 1024 * 2 * 8;  // 
 // threads for `cols` columns in chunks of 8, v of them a thread: whole wavefronts
 static unsigned norm_threads(long long cols, int v) { return (unsigned)((cols + 8 * v - 1) / (8 * v) + 63) / 64 * 64; }
 
+static bool norm_small(long long rows, long long cols) { return rows > 0 && rows <= NORM_SMALL_ROWS && cols <= 1024 * 8; }
 // workgroups of the backward kernel (= rows of partial dw)
 static int norm_parts(long long rows, long long cols) { return (int)std::min<long long>(rows, cols > NORM_BWD_LONG ? 64 : cols <= 1024 ? 2048 : 512); }
 
@@ -346,7 +413,7 @@ int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldr
 
 size_t aq_rms_norm_bwd_workspace_bytes(long long rows, long long cols)
 {
-    return rows > 0 && cols > 0 ? (size_t)aq::norm_parts(rows, cols) * (size_t)cols * sizeof(float) : 0;
+    return rows > 0 && cols > 0 && !aq::norm_small(rows, cols) ? (size_t)aq::norm_parts(rows, cols) * (size_t)cols * sizeof(float) : 0;
 }
 
 int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long lddh, const void *h, long long ldh, int type, const float *w,
@@ -363,11 +430,20 @@ int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long ld
     const int parts = norm_parts(rows, cols);
     if (dw && rows) {
         const size_t need = aq_rms_norm_bwd_workspace_bytes(rows, cols);
-        AQ_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, -ENOSPC,
+        AQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), -ENOSPC,
                    "aq_rms_norm_bwd: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
     }
     const NormBwdArgs a = {dy, dh, h, w, rstd, dx, dw ? static_cast<float *>(workspace) : nullptr, lddy, lddh, ldh, lddx, rows, cols};
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (norm_small(rows, cols)) {
+        const unsigned groups = (unsigned)((dx ? rows : 0) + (dw ? (cols + 127) / 128 : 0));
+        const dim3 b(std::max(512u, norm_threads(cols, 1)));
+        by_type(type, [&](auto *t) {
+            hipLaunchKernelGGL((rms_norm_bwd_small_kernel<std::remove_pointer_t<decltype(t)>>), dim3(groups), b, 0, st, a, dw);
+            return 0;
+        });
+        return check_launch("aq_rms_norm_bwd");
+    }
     if (rows > 0) {
         by_type(type, [&](auto *t) {
             using T = std::remove_pointer_t<decltype(t)>;

@@ -75,7 +75,7 @@ def test_norm_and_clip_refusals():
     assert rc < 0 and "pitch" in err
     rc, err = _rc("aq_rms_norm_bwd", P, 64, None, 0, P, 64, 0, P, P, 4, 64, None, 0, None, None, 0, None)
     assert rc < 0 and "no output" in err
-    rc, err = _rc("aq_rms_norm_bwd", P, 64, None, 0, P, 64, 0, P, P, 4, 64, P, 64, P, None, 0, None)
+    rc, err = _rc("aq_rms_norm_bwd", P, 64, None, 0, P, 64, 0, P, P, 2000, 64, P, 64, P, None, 0, None)  # (few rows need none)
     assert rc < 0 and "workspace" in err
     one = lambda t, v: (t * 1)(v)  # noqa: E731
     p, n, t = one(C.c_void_p, P), one(C.c_longlong, 10), one(C.c_int, 0)

@@ -895,3 +895,27 @@ def test_the_largest_products():
     bad = torch.zeros_like(y, dtype=torch.bool)
     bad[5], bad[:, 8064:] = True, True
     assert torch.equal(torch.isnan(z), bad) and torch.equal(z[~bad], y[~bad])
+
+
+@pytest.mark.parametrize("rows,cols", [(511, 130), (512, 129), (513, 128), (512, 8192), (513, 8191), (512, 8193), (64, 8185), (33, 6)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_backward_around_the_border_of_one_launch(rows, cols, dtype):
+    test_norm_backward(rows, cols, dtype)
+
+
+def test_norm_backward_of_few_rows_in_place_and_between_others():
+    """Strided operands, dx over dh, rows behind the last left as they were."""
+    from quantized_cnn_amd import _lib
+    rows, cols, ld = 37, 203, 260
+    g = torch.Generator(device=DEV).manual_seed(1)
+    dy, h, dh = (torch.randn(rows + 1, ld, device=DEV, generator=g).bfloat16() for _ in range(3))
+    w = torch.randn(cols, device=DEV, generator=g)
+    _, _, rstd = ops.rms_norm_forward(h[:rows, 3:3 + cols], w)
+    dx, dw = ops.rms_norm_backward(dy[:rows, 1:1 + cols], h[:rows, 3:3 + cols], w, rstd, dh=dh[:rows, 5:5 + cols])
+    keep, dw2 = dh.clone(), torch.full((cols + 1,), 7.0, device=DEV)
+    at = dh[0, 5:].data_ptr()
+    _lib.check(_lib.lib().aq_rms_norm_bwd(dy[0, 1:].data_ptr(), ld, at, ld, h[0, 3:].data_ptr(), ld, 1, w.data_ptr(), rstd.data_ptr(), rows, cols, at, ld,
+                                          dw2.data_ptr(), None, 0, _lib.stream()))
+    assert torch.equal(dh[:rows, 5:5 + cols], dx) and torch.equal(dw2[:cols], dw) and float(dw2[cols]) == 7.0
+    dh[:rows, 5:5 + cols] = keep[:rows, 5:5 + cols]
+    assert torch.equal(dh, keep)
