@@ -604,7 +604,7 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_scaled_kernel(const MatA
         for (int i = 0; i < LOADS; ++i) fetch(i, min(s, nkb - 1), s);
         fetch_scales(s);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * (LOADS + 1)) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 1) * (LOADS + 1)) : "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     auto begin = [&](int stage) {
