@@ -1,5 +1,5 @@
 """The 8-bit floating point format, the root-mean-square norm and gradient clipping in float64 numpy, from their definitions (the
-checker of the HIP kernels; no reference implementation exists: parity unpinned)."""
+oracle of the HIP kernels; no reference implementation exists: parity unpinned)."""
 import numpy as np
 
 BLK = 128

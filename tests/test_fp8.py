@@ -1,4 +1,4 @@
-"""Host side of the 8-bit floating point operators, the row norm and gradient clipping: the checker's own format against
+"""Host side of the 8-bit floating point operators, the row norm and gradient clipping: the oracle's own format against
 torch's e4m3 type, refusals of the C ABI before any launch, refusals of the wrappers (no GPU)."""
 import numpy as np
 import pytest
