@@ -211,6 +211,10 @@ class Fp8Linear(nn.Module):
         self._packed = None
         return super()._load_from_state_dict(*args, **kw)
 
+    def buffers_changed(self):
+        """Called where a data-parallel wrapper has written the parameters in place."""
+        self._packed = None
+
     def forward(self, x):
         if self._packed is not None and not self.training and not torch.is_grad_enabled():
             return linear(x, self._packed, self.bias)

@@ -141,7 +141,8 @@ class DataParallel:
 def _clip(opts, max_norm):
     """Clips the gradients of all parameters of the optimizers by their common norm, on the device -> the norm."""
     from . import ops
-    return ops.clip_grad_norm([p.grad for o in opts for g in o.param_groups for p in g["params"] if p.grad is not None], max_norm)
+    params = dict.fromkeys(p for o in opts for g in o.param_groups for p in g["params"] if p.grad is not None)  # (once each, if two optimizers share one)
+    return ops.clip_grad_norm([p.grad for p in params], max_norm)
 
 
 def _checked_max_norm(max_norm):

@@ -919,3 +919,30 @@ def test_norm_backward_of_few_rows_in_place_and_between_others():
     assert torch.equal(dh[:rows, 5:5 + cols], dx) and torch.equal(dw2[:cols], dw) and float(dw2[cols]) == 7.0
     dh[:rows, 5:5 + cols] = keep[:rows, 5:5 + cols]
     assert torch.equal(dh, keep)
+
+
+def test_optimizers_that_share_a_parameter_clip_it_once():
+    torch.manual_seed(0)
+    lin = fp8.Fp8Linear(64, 8).to(DEV)
+    x, y = torch.randn(40, 64, device=DEV), torch.randn(40, 8, device=DEV)
+    opts = [torch.optim.SGD(lin.parameters(), 0.0), torch.optim.SGD([lin.weight], 0.0)]
+    step = train.CapturedStep(lin, opts, torch.nn.functional.mse_loss, warmup=1, max_norm=1e-3)
+    step(x, y)
+    want = torch.autograd.grad(torch.nn.functional.mse_loss(lin(x), y), list(lin.parameters()))
+    norm = F8.grad_norm([f64(t) for t in want])
+    assert abs(float(step.grad_norm) - norm) <= 2 * U * norm
+    assert abs(F8.grad_norm([f64(p.grad) for p in lin.parameters()]) - 1e-3) <= 1e-3 * 1e-5 + 1e-6 * 1e-3 / norm
+
+
+def test_packed_codes_go_with_the_parameters_they_are_of():
+    import copy
+    layer = fp8.Fp8Linear(130, 40).to(DEV).eval().pack()
+    x = torch.randn(3, 130, device=DEV)
+    with torch.no_grad():
+        want = layer(x)
+        twin = copy.deepcopy(layer)
+        layer.weight.mul_(2.0)
+        layer.buffers_changed()
+        assert layer._packed is None and twin._packed is not None
+        assert torch.equal(twin(x), want) and not torch.equal(layer(x), want)
+        assert layer.pack().half()._packed is None and layer(x.half()).dtype == torch.float16
