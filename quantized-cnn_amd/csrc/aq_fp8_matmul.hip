@@ -974,10 +974,7 @@ static int matmul_splits(long long M, long long N, long long K)
 //   8192 x 8192 x 2048: 120 against 117.5 us, 5000^3: 145 against 141 us);
 //   128 x 128 with two stages, two workgroups on a unit, for more than a round (1500 x 5000 x 2560: 25 us against 30 us with four stages);
 //   128 x 128 with four stages for up to a round (1024 x 4096: 22 against 28 us with two);
-//   64 x 128 for fewer (512 x 4096: 17 us; 1000 x 1000 x 1000: 8 against 11 us), K in parts for very few;
-//   32 x 32 from streamed fragments where that is one round and K one round of the wavefronts' loads (256 x 1024: 11.5 us, in 64 x 128 and
-//   parts of K 14 us; 100 x 1000 x 2048: 7.4 against 10.1 us; at K = 8192 the parts win, 512 x 512: 15.6 against 19 us, and so they do
-//   for half a round, 256 x 256: 9.6 against 11.2 us).
+//   64 x 128 for fewer (512 x 4096: 17 us; 1000 x 1000 x 1000: 8 against 11 us), K in parts for very few.
 template <typename T> static void launch_pow2(MatArgs p, hipStream_t st)
 {
     if (p.N < 128) return launch_rows<4, 2, 2, POW2, T>(p, st);
@@ -986,8 +983,6 @@ template <typename T> static void launch_pow2(MatArgs p, hipStream_t st)
     if (p.M >= 128 && tiles_of(p.M, p.N, 128, 128) > 256) return launch_large<128, 128, 2, 2, 2, T>(p, st);
     if (p.M >= 128 && tiles_of(p.M, p.N, 64, 128) > 256) return launch_large<128, 128, 2, 2, 4, T>(p, st);
     const int splits = matmul_splits(p.M, p.N, p.K), nkb = (p.K + FP8_BLK - 1) / FP8_BLK;
-    const long long small = tiles_of(p.M, p.N, 32, 32);
-    if (small <= 256 && nkb <= 32 && (splits == 1 || small > 128)) return launch_rows<2, 2, 4, POW2, T>(p, st);
     if (splits == 1) return launch_large<64, 128, 1, 4, 4, T>(p, st);
     p.split_blocks = (nkb + splits - 1) / splits;
     p.splits = (nkb + p.split_blocks - 1) / p.split_blocks;
@@ -1021,18 +1016,32 @@ template <int MODE, typename T> static void launch_block(MatArgs p, hipStream_t 
     }
 }
 
+// Streamed fragments: the smallest tiles whose workgroups fit the 256 compute units once, since a workgroup's time goes with the rows of A and
+// B that it reads (128 x 1024 x 4096: 9.1 us in 16 x 32, 11.2 in 32 x 32, 16 in 64 x 32, 10.8 in 64 x 128 and parts of K; 64 x 1000 x 2048: 5.8 us
+// in 16 x 16, 8.6 in 64 x 16; 64 x 8192 x 4096: 17 us in 64 x 32, 19 in 32 x 32, 26 in 64 x 16).  Up to 16 rows the reading of B is all, which
+// two rounds of narrow tiles do as fast (1 x 8192 x 8192: 14.8 us, 17.8 in 16 x 32).  With more than 64 rows, power-of-two scales and long rows
+// the parts of K win (512 x 512 x 8192: 15.6 against 19 us).  False: there are more, and other kernels for them.
+template <int MODE, typename T> static bool launch_streamed(const MatArgs &p, hipStream_t st)
+{
+    const int nkb = (p.K + FP8_BLK - 1) / FP8_BLK;
+    const bool parts = MODE == POW2 && p.M > 64;
+    auto once = [&](int bm, int bn, int most) { return tiles_of(p.M, p.N, bm, bn) <= 256 && (!parts || nkb <= most); };
+    if (once(16, 16, 64) || (p.M <= 16 && tiles_of(p.M, p.N, 16, 16) <= 512)) launch_rows<1, 1, 4, MODE, T>(p, st);
+    else if (once(16, 32, 64) || p.M <= 16) launch_rows<1, 2, 4, MODE, T>(p, st);
+    else if (once(32, 32, 32) || p.M <= 32) launch_rows<2, 2, MODE == POW2 ? 4 : 2, MODE, T>(p, st);
+    else if (p.M <= 64) launch_rows<4, 2, 2, MODE, T>(p, st);
+    else return false;
+    return true;
+}
+
 template <int MODE, typename T> static void launch_matmul(MatArgs p, hipStream_t st)
 {
-    if (p.M <= 16) return launch_rows<1, 1, 4, MODE, T>(p, st);
-    if (p.M <= 32) return launch_rows<2, 1, 4, MODE, T>(p, st);
-    if (p.M <= 64) return launch_rows<4, 1, 2, MODE, T>(p, st);
+    if (launch_streamed<MODE, T>(p, st)) return;
     if constexpr (MODE == POW2) {
         launch_pow2<T>(p, st);
     } else {
-        // Streamed fragments while their workgroups fit the compute units once, in 32 x 32 (256 x 1024 x 4096: 13 us, in 64 x 32 19 us), then in
-        // 64 x 32 (512 x 1024 x 4096: 19 us, in 32 x 32 23 us, on tiles 28 us; 512 x 2048 x 4096: 35 us, on tiles 28 us); fp32 outputs with any
-        // scales, whose tiles are the slowest, for twice as many (36 against 48 us).
-        if (tiles_of(p.M, p.N, 32, 32) <= 256) return launch_rows<2, 2, 2, MODE, T>(p, st);
+        // Tiles of 64 x 32 that fit once are still streamed (512 x 1024 x 4096: 19 us, in 32 x 32 23 us, through LDS 28 us; 512 x 2048 x 4096: 35 us,
+        // through LDS 28 us); fp32 outputs with any scales, whose LDS kernel is the slowest, for twice as many (36 against 48 us).
         const long long few = MODE == EXACT && p.scale_f32 ? 512 : 256;
         if (p.M < 128 || p.N < 128 || tiles_of(p.M, p.N, 64, 32) <= few) return launch_rows<4, 2, 2, MODE, T>(p, st);
         launch_block<MODE, T>(p, st);

@@ -946,3 +946,18 @@ def test_packed_codes_go_with_the_parameters_they_are_of():
         assert layer._packed is None and twin._packed is not None
         assert torch.equal(twin(x), want) and not torch.equal(layer(x), want)
         assert layer.pack().half()._packed is None and layer(x.half()).dtype == torch.float16
+
+
+@pytest.mark.parametrize("m,n,k", [(250, 256, 1030), (256, 257, 8200), (16, 4097, 300), (17, 8192, 260), (33, 8100, 200), (49, 4000, 390), (64, 8300, 257), (130, 900, 8190)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pow2", [True, False])
+def test_product_of_streamed_fragments(m, n, k, dtype, pow2):
+    """Around the borders between their tiles."""
+    check_product(operand(m, k, 1, pow2, m), operand(n, k, 1 if n % 2 else 128, pow2, k), torch.randn(n, device=DEV) if m % 2 else None, dtype)
+
+
+@pytest.mark.parametrize("m,n", [(16, 200), (100, 1000), (64, 5000), (20, 9000)])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_special_values_in_streamed_fragments(m, n, pow2):
+    for dtype in TYPES:
+        test_product_special_values(m, n, dtype, pow2)
