@@ -482,6 +482,9 @@ int aq_fp8_transpose(const uint8_t *a, long long lda, const void *as, long long 
 /* y[i, j] = code * scale, rounded to y's type. */
 int aq_fp8_dequantize(const uint8_t *q, long long ldq, const void *qs, long long ldqs, long long rows, long long cols, int block_rows,
                       int scale_type, void *y, int ytype, long long ldy, void *stream);
+/* The codes alone, [rows, cols] from pitch ldq to pitch ldp: rows that start at multiples of 16 bytes and are zero from cols to the next multiple of
+ * 16, as aq_fp8_matmul reads them (p 16-byte aligned, ldp a multiple of 16; q anywhere). */
+int aq_fp8_repitch(const uint8_t *q, long long ldq, long long rows, long long cols, uint8_t *p, long long ldp, void *stream);
 /* y [M, N] = A [M, K] . B [N, K]^T + bias[N] (NULL: none).  A, B and their pitches 16-byte aligned, every row readable up to
  * the next multiple of 16 bytes (what lies behind K does not matter).  Sums in fp32.  bf16 / fp16 outputs: the 8-bit matrix
  * instructions, which align the products of a group of 8 to the largest of them and drop what lies 2^-14 below it; fp32

@@ -29,7 +29,7 @@ EXPORTS = (
     "aq_bn_relu_bwd_shortcut", "aq_bn_relu_fwd_shortcut", "aq_conv_dgrad_add", "aq_synth_fwd_static",
     "aq_tern_workspace_bytes", "aq_tern_fwd", "aq_tern_bwd", "aq_inq_partition", "aq_tern_bwd_adam", "aq_inq_effective", "aq_inq_effective_sumsq", "aq_bn_add_relu_fwd", "aq_bn_add_relu_bwd",
     "aq_pkt_workspace_bytes", "aq_pkt_loss", "aq_pkt_kernel_matrix", "aq_maxpool3s2_fwd", "aq_maxpool3s2_bwd",
-    "aq_fp8_quantize_workspace_bytes", "aq_fp8_quantize", "aq_fp8_transpose", "aq_fp8_dequantize", "aq_fp8_matmul_workspace_bytes", "aq_fp8_matmul",
+    "aq_fp8_quantize_workspace_bytes", "aq_fp8_quantize", "aq_fp8_transpose", "aq_fp8_dequantize", "aq_fp8_repitch", "aq_fp8_matmul_workspace_bytes", "aq_fp8_matmul",
     "aq_rms_norm_fwd", "aq_rms_norm_bwd_workspace_bytes", "aq_rms_norm_bwd", "aq_clip_grad_norm_workspace_bytes", "aq_clip_grad_norm",
 )
 TERN_TWN, TERN_TTQ, TERN_INQ = 0, 1, 2
@@ -181,6 +181,7 @@ def lib():
         L.aq_fp8_quantize.argtypes = [vp, i, ll, ll, ll, vp, ll, vp, ll, vp, ll, vp, ll, i, i, vp, vp, sz, vp]
         L.aq_fp8_transpose.argtypes = [vp, ll, vp, ll, ll, ll, vp, ll, vp, ll, i, i, vp]
         L.aq_fp8_dequantize.argtypes = [vp, ll, vp, ll, ll, ll, i, i, vp, i, ll, vp]
+        L.aq_fp8_repitch.argtypes = [vp, ll, ll, ll, vp, ll, vp]
         L.aq_fp8_matmul_workspace_bytes.argtypes = [ll, ll, ll]
         L.aq_fp8_matmul.argtypes = [vp, ll, vp, ll, i, vp, ll, vp, ll, i, ll, ll, ll, i, vp, vp, i, ll, vp, sz, vp]
         L.aq_rms_norm_fwd.argtypes = [vp, ll, vp, ll, i, vp, ll, ll, C.c_double, vp, ll, vp, ll, vp, ll, i, vp, ll, vp, vp]
@@ -191,7 +192,7 @@ def lib():
         for name in ("aq_fp8_quantize_workspace_bytes", "aq_fp8_matmul_workspace_bytes", "aq_rms_norm_bwd_workspace_bytes",
                      "aq_clip_grad_norm_workspace_bytes"):
             getattr(L, name).restype = sz
-        for name in ("aq_fp8_quantize", "aq_fp8_transpose", "aq_fp8_dequantize", "aq_fp8_matmul", "aq_rms_norm_fwd", "aq_rms_norm_bwd",
+        for name in ("aq_fp8_quantize", "aq_fp8_transpose", "aq_fp8_dequantize", "aq_fp8_repitch", "aq_fp8_matmul", "aq_rms_norm_fwd", "aq_rms_norm_bwd",
                      "aq_clip_grad_norm"):
             getattr(L, name).restype = i
         if L.aq_abi_version() != ABI_VERSION:

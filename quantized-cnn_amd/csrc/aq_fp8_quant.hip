@@ -243,6 +243,24 @@ __global__ __launch_bounds__(256) void fp8_values_kernel(const uint8_t *__restri
     for (int i = 0; c + i < cols; ++i) o[i] = from_f32<T>(to_f32(p[i]) * s);
 }
 
+// 16 codes per thread (8192 x 8191: 23 us, 5.8 TB/s)
+__global__ __launch_bounds__(256) void fp8_repitch_kernel(const uint8_t *__restrict__ q, long long ldq, uint32_t rows, int cols, uint32_t chunks,
+                                                          uint8_t *__restrict__ p, long long ldp)
+{
+    const uint32_t t = blockIdx.x * 256 + threadIdx.x, r = t / chunks;
+    const int c = (int)(t - r * chunks) * 16;
+    if (r >= rows) return;
+    const e4m3_el *row = reinterpret_cast<const e4m3_el *>(q) + (long long)r * ldq;
+    raw8<e4m3_el> lo, hi;
+    if (cols >= 8) {
+        lo = load_row_chunk<false>(row, c, cols), hi = load_row_chunk<false>(row, c + 8, cols);
+        lo = row_chunk(lo, c, cols), hi = row_chunk(hi, c + 8, cols);
+    } else {
+        lo = load_raw_n(row + c, cols - c), hi = {};
+    }
+    *reinterpret_cast<u4_t *>(p + (long long)r * ldp + c) = u4_t{lo.a[0], lo.a[1], hi.a[0], hi.a[1]};
+}
+
 static long long blocks_of(long long n, int b) { return (n + b - 1) / b; }
 
 template <typename T> static void launch_tiles(const TileArgs &a, long long tiles, bool square, hipStream_t st)
@@ -365,6 +383,21 @@ int aq_fp8_dequantize(const uint8_t *q, long long ldq, const void *qs, long long
         return 0;
     });
     return check_launch("aq_fp8_dequantize");
+}
+
+int aq_fp8_repitch(const uint8_t *q, long long ldq, long long rows, long long cols, uint8_t *p, long long ldp, void *stream)
+{
+    using namespace aq;
+    AQ_REQUIRE(rows >= 0 && cols >= 0 && cols < (1LL << 31) - 256, -EINVAL, "aq_fp8_repitch: bad sizes %lld x %lld", rows, cols);
+    if (rows == 0 || cols == 0) return 0;
+    const long long chunks = blocks_of(cols, 16);
+    AQ_REQUIRE(rows < (1LL << 32) / chunks - 256, -E2BIG, "aq_fp8_repitch: %lld x %lld is too large for one call", rows, cols);
+    AQ_REQUIRE(q && p, -EFAULT, "aq_fp8_repitch: NULL pointer");
+    AQ_REQUIRE(ldq >= cols && ldp >= chunks * 16, -EINVAL, "aq_fp8_repitch: a pitch is smaller than its row");
+    AQ_REQUIRE(((uintptr_t)p & 15) == 0 && ldp % 16 == 0, -EINVAL, "aq_fp8_repitch: rows of the output have to start at multiples of 16 bytes");
+    hipLaunchKernelGGL(fp8_repitch_kernel, dim3((unsigned)blocks_of(rows * chunks, 256)), dim3(256), 0, static_cast<hipStream_t>(stream), q, ldq, (uint32_t)rows,
+                       (int)cols, (uint32_t)chunks, p, ldp);
+    return check_launch("aq_fp8_repitch");
 }
 
 } // extern "C"

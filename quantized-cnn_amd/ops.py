@@ -1009,9 +1009,11 @@ class Fp8Blocks:
         if self._ld % 16 == 0 and p % 16 == 0 and (cols % 16 == 0 or d.storage_offset() + (self.shape[0] - 1) * self._ld + _up(cols, 16)
                                                    <= d.untyped_storage().nbytes()):
             return d, p, self._ld
-        c = torch.empty((self.shape[0], _up(cols, 16)), dtype=torch.float8_e4m3fn, device=self.device)
-        c[:, :cols].copy_(d)
-        return c, c.data_ptr(), c.shape[1]
+        ld = _up(cols, 16)
+        c = torch.empty(self.shape[0] * ld, dtype=torch.uint8, device=self.device)
+        at = c.data_ptr()
+        _lib.check(_lib.lib().aq_fp8_repitch(p, self._ld, self.shape[0], cols, at, ld, _current_stream(self.device.index)))
+        return c, at, ld
 
 
 def _up(n, m):

@@ -127,3 +127,12 @@ def test_matmul_refuses_scales_too_far_apart(ldas, ldbs):
     """(the offsets of a tile's scales have 32 bits)"""
     rc, err = _rc("aq_fp8_matmul", P, 128, P, ldas, 1, P, 128, P, ldbs, 1, 256, 256, 128, 0, None, P, 1, 256, None, 0, None)
     assert rc < 0 and "pitch" in err and "scales" in err
+
+
+@pytest.mark.parametrize("args,word", [
+    ((P, 100, -1, 100, P, 112, None), "bad sizes"), ((P, 99, 4, 100, P, 112, None), "pitch"), ((P, 100, 4, 100, P, 100, None), "pitch"),
+    ((P, 100, 4, 100, P + 8, 112, None), "multiples of 16"), ((P, 100, 4, 100, P, 120, None), "multiples of 16"), ((None, 100, 4, 100, P, 112, None), "NULL"),
+    ((P, 100, 1 << 40, 100, P, 112, None), "too large")])
+def test_repitch_refusals(args, word):
+    rc, err = _rc("aq_fp8_repitch", *args)
+    assert rc < 0 and word in err, err

@@ -962,3 +962,36 @@ def test_product_of_streamed_fragments(m, n, k, dtype, pow2):
 def test_special_values_in_streamed_fragments(m, n, pow2):
     for dtype in TYPES:
         test_product_special_values(m, n, dtype, pow2)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 8), (4, 15), (7, 16), (33, 17), (20, 1001), (129, 4091)])
+def test_codes_to_rows_at_multiples_of_16_bytes(rows, cols):
+    from quantized_cnn_amd import _lib
+    src = torch.randint(0, 256, (rows + 2, cols + 5), device=DEV, dtype=torch.uint8)
+    ld = -(-cols // 16) * 16 + 32
+    for q, ldq in ((src[1:, 3:], cols + 5), (src.view(-1)[:rows * cols].view(rows, cols), cols)):
+        out = torch.full((rows + 1, ld), 0x55, dtype=torch.uint8, device=DEV)
+        _lib.check(_lib.lib().aq_fp8_repitch(q.data_ptr(), ldq, rows, cols, out.data_ptr(), ld, _lib.stream()))
+        want = torch.full_like(out, 0x55)
+        want[:rows, :-(-cols // 16) * 16] = 0
+        want[:rows, :cols] = q[:rows, :cols]
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 1000), (37, 500, 2041), (300, 700, 999), (1030, 1100, 651)])
+def test_product_of_codes_packed_without_gaps(m, n, k):
+    """Operands of other origin: rows of k codes behind each other, k no multiple of 16; captured as well."""
+    a0, b0 = operand(m, k, 1, True, 1), operand(n, k, 128, True, 2)
+    a = ops.Fp8Blocks(a0.data.contiguous(), a0.scale.contiguous())
+    b = ops.Fp8Blocks(b0.data.contiguous(), b0.scale.contiguous(), 128)
+    want = ops.fp8_matmul(a0, b0)
+    assert b.data.stride(0) == k and torch.equal(ops.fp8_matmul(a, b), want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ops.fp8_matmul(a, b)
+    for _ in range(3):
+        y.zero_()
+        g.replay()
+        ops.fp8_matmul(a0, b0)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
