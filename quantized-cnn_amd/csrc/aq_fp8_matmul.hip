@@ -971,14 +971,16 @@ static int matmul_splits(long long M, long long N, long long K)
 //   256 x 256 from three quarters of a round on (4096 x 4096: 57 us against 75 us in 128 x 128; 2048 x 4096, half a round: 47 against 38).
 //   Products so large that they run at the power limit (2^38 multiplications and more) with four wavefronts of 128 x 128, which read a third less
 //   from LDS, smaller ones with eight of 64 x 128, whose waits overlap (8192^3: 429 against 462 us, 16384 x 8192 x 2048: 270 against 285 us;
-//   8192 x 8192 x 2048: 120 against 117.5 us, 5000^3: 145 against 141 us);
+//   8192 x 8192 x 2048: 120 against 117.5 us, 5000^3: 145 against 141 us).
+//   Not for a round and a few tiles more (2316 x 6403 x 1632, 260 tiles: 58 us, 44 us in 128 x 128; 4352 x 4096 x 1024, 272: 33 against 29 us);
 //   128 x 128 with two stages, two workgroups on a unit, for more than a round (1500 x 5000 x 2560: 25 us against 30 us with four stages);
 //   128 x 128 with four stages for up to a round (1024 x 4096: 22 against 28 us with two);
 //   64 x 128 for fewer (512 x 4096: 17 us; 1000 x 1000 x 1000: 8 against 11 us), K in parts for very few.
 template <typename T> static void launch_pow2(MatArgs p, hipStream_t st)
 {
     if (p.N < 128) return launch_rows<4, 2, 2, POW2, T>(p, st);
-    if (p.M >= 256 && p.N >= 256 && tiles_of(p.M, p.N, 256, 256) >= 192)
+    const long long big = tiles_of(p.M, p.N, 256, 256);
+    if (p.M >= 256 && p.N >= 256 && big >= 192 && (big <= 256 || big > 320))
         return (double)p.M * p.N * p.K >= 0x1p38 ? launch_large<256, 256, 2, 2, 2, T>(p, st) : launch_large<256, 256, 4, 2, 2, T>(p, st);
     if (p.M >= 128 && tiles_of(p.M, p.N, 128, 128) > 256) return launch_large<128, 128, 2, 2, 2, T>(p, st);
     if (p.M >= 128 && tiles_of(p.M, p.N, 64, 128) > 256) return launch_large<128, 128, 2, 2, 4, T>(p, st);
