@@ -499,7 +499,8 @@ int aq_fp8_matmul(const uint8_t *a, long long lda, const void *as, long long lda
 /* ---- root-mean-square norm over rows, with the residual's addition ---------------------------------------------------
  * h = round(x + res) (h = x without res), rstd = 1 / sqrt(mean(h^2) + eps), y = (h * rstd) * w; x, res, h, y of one type, w and
  * rstd fp32.  Outputs that are not wanted are NULL.  q / qs: y in blocks of 1 x 128 as aq_fp8_quantize makes them, instead
- * of or beside y.  h may be x or res itself (in place).  One call takes fewer than 2^22 rows, here and below. */
+ * of or beside y.  h may be x or res itself (in place).  One call takes fewer than 2^22 rows (2^28 of up to
+ * 256 columns), here and below. */
 int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldres, int type, const float *w, long long rows,
                     long long cols, double eps, void *y, long long ldy, uint8_t *q, long long ldq, void *qs, long long ldqs, int scale_type,
                     void *h, long long ldh, float *rstd, void *stream);

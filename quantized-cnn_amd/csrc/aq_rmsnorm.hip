@@ -111,6 +111,48 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_kernel(const NormArgs a)
     }
 }
 
+// Short rows (of a head, of a small layer): LPR lanes per row, four rows for each with all their loads in flight, and sums that need no LDS
+// (2^20 rows of 128 bf16: 94 us for 537 MB, 404 us with a workgroup a row; 2^20 rows of 64, half of whose lanes idle: 102 us).
+template <typename T, int LPR, bool NT>
+__global__ __launch_bounds__(256) void rms_norm_fwd_short_kernel(const NormArgs a)
+{
+    constexpr int U = 4, G = 256 / LPR;
+    const int c = (int)(threadIdx.x % LPR) * 8, k = (int)max(0LL, min(8LL, a.cols - c));
+    const long long r0 = (long long)blockIdx.x * (G * U) + threadIdx.x / LPR;
+    const bool whole = a.cols >= 8;
+    auto load = [&](const void *p, long long r, long long ld) {
+        const T *row = static_cast<const T *>(p) + min(r, a.rows - 1) * ld;
+        return whole ? load_row_chunk<NT>(row, c, a.cols) : load_raw_n(row + c, k);
+    };
+    raw8<T> xv[U], rv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) xv[u] = load(a.x, r0 + u * G, a.ldx);
+    if (a.res)
+#pragma unroll
+        for (int u = 0; u < U; ++u) rv[u] = load(a.res, r0 + u * G, a.ldres);
+    const raw8<float> w = load_raw_n(a.w + c, k);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long r = r0 + u * G;
+        if (whole) xv[u] = row_chunk(xv[u], c, a.cols);
+        if (whole && a.res) rv[u] = row_chunk(rv[u], c, a.cols);
+        float hv[8];
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            hv[j] = a.res ? to_f32(from_f32<T>(value(xv[u], j) + value(rv[u], j))) : value(xv[u], j);
+            s = __builtin_fma((double)hv[j], (double)hv[j], s);
+        }
+#pragma unroll
+        for (int m = LPR / 2; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+        const float rs = (float)(1.0 / sqrt(s / (double)a.cols + a.eps));
+        const int n = r < a.rows ? k : 0;
+        if (a.h) store_n<NT>(static_cast<T *>(a.h) + r * a.ldh + c, n, hv);
+        if (a.rstd && c == 0 && r < a.rows) a.rstd[r] = rs;
+        norm_outputs<NT, T>(a, r, c, n, hv, w, rs);
+    }
+}
+
 // rows too long for the registers: read twice
 template <typename T>
 __global__ __launch_bounds__(1024) void rms_norm_fwd_long_kernel(const NormArgs a)
@@ -311,6 +353,70 @@ __global__ __launch_bounds__(1024) void rms_norm_bwd_small_kernel(const NormBwdA
     dw[col] = (float)s;
 }
 
+// Short rows: LPR lanes per row, the row behind on its way, as above; the workgroup's groups of lanes join their dw at the end, in double
+// (2^20 rows of 128 bf16: 147 us for 805 MB, 651 us with a workgroup a row).
+template <typename T, int LPR, bool NT>
+__global__ __launch_bounds__(256) void rms_norm_bwd_short_kernel(const NormBwdArgs a)
+{
+    constexpr int G = 256 / LPR;
+    __shared__ float sums[G][LPR * 8];
+    const int c = (int)(threadIdx.x % LPR) * 8, k = (int)max(0LL, min(8LL, a.cols - c)), g = threadIdx.x / LPR;
+    const bool whole = a.cols >= 8;
+    float wv[8], acc[8] = {};
+    load_n(a.w + c, k, wv);
+    auto load1 = [&](const void *p, long long r, long long ld) {
+        const T *row = static_cast<const T *>(p) + r * ld;
+        return whole ? load_row_chunk<NT>(row, c, a.cols) : load_raw_n(row + c, k);
+    };
+    raw8<T> dyn = {}, hn = {}, dhn = {};
+    float rsn = 0.0f;
+    auto load = [&](long long r) {
+        rsn = a.rstd[r];
+        dyn = load1(a.dy, r, a.lddy);
+        hn = load1(a.h, r, a.ldh);
+        if (a.dh && a.dx) dhn = load1(a.dh, r, a.lddh);
+    };
+    const float inv = 1.0f / (float)a.cols;
+    const long long step = (long long)gridDim.x * G;
+    long long r = (long long)blockIdx.x * G + g;
+    if (r < a.rows) load(r);
+    for (; r < a.rows; r += step) {  // (the lanes of a row end together)
+        const raw8<T> dy = whole ? row_chunk(dyn, c, a.cols) : dyn, h = whole ? row_chunk(hn, c, a.cols) : hn;
+        raw8<T> dh = {};
+        if (a.dh && a.dx) dh = whole ? row_chunk(dhn, c, a.cols) : dhn;
+        const float rs = rsn;
+        if (r + step < a.rows) load(r + step);
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = value(dy, j), n = value(h, j) * rs;
+            acc[j] = __builtin_fmaf(d, n, acc[j]);
+            s = __builtin_fmaf(d * wv[j], n, s);
+        }
+        if (!a.dx) continue;
+#pragma unroll
+        for (int m = LPR / 2; m >= 1; m >>= 1) s += __shfl_xor(s, m, 64);
+        const float m = s * inv;
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = rs * __builtin_fmaf(-(value(h, j) * rs), m, value(dy, j) * wv[j]);
+            o[j] = a.dh ? d + value(dh, j) : d;
+        }
+        store_n<NT>(static_cast<T *>(a.dx) + r * a.lddx + c, k, o);
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[g][c + j] = acc[j];
+    __syncthreads();
+    for (int col = threadIdx.x; col < (int)a.cols; col += 256) {
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < G; ++i) s += (double)sums[i][col];
+        a.part[(long long)blockIdx.x * a.cols + col] = (float)s;
+    }
+}
+
 // rows too long for the registers: dx reads its row twice, dw is a sum over a slice of rows for 256 columns a workgroup
 template <typename T>
 __global__ __launch_bounds__(1024) void rms_norm_dx_long_kernel(const NormBwdArgs a)
@@ -360,13 +466,18 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float *__restri
     if (run == 0 && c < cols) dw[c] = (float)sh[0][lane];
 }
 
+constexpr long long NORM_SHORT = 256;
 constexpr long long NORM_LONG = 1024 * 4 * 8, NORM_BWD_LONG = 1024 * 2 * 8;  // columns that fit the registers of a workgroup
 // threads for `cols` columns in chunks of 8, v of them a thread: whole wavefronts
 static unsigned norm_threads(long long cols, int v) { return (unsigned)((cols + 8 * v - 1) / (8 * v) + 63) / 64 * 64; }
 
 static bool norm_small(long long rows, long long cols) { return rows > 0 && rows <= NORM_SMALL_ROWS && cols <= 1024 * 8; }
 // workgroups of the backward kernel (= rows of partial dw)
-static int norm_parts(long long rows, long long cols) { return (int)std::min<long long>(rows, cols > NORM_BWD_LONG ? 64 : cols <= 1024 ? 2048 : 512); }
+static int norm_parts(long long rows, long long cols)
+{
+    if (cols <= NORM_SHORT) return (int)std::min<long long>((rows + 7) / 8, 2048);  // (eight or sixteen rows a workgroup at a time)
+    return (int)std::min<long long>(rows, cols > NORM_BWD_LONG ? 64 : cols <= 1024 ? 2048 : 512);
+}
 
 } // namespace aq
 
@@ -379,7 +490,8 @@ int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldr
     using namespace aq;
     AQ_REQUIRE(type == AQ_F32 || type == AQ_BF16 || type == AQ_F16, -EINVAL, "aq_rms_norm_fwd: unknown element type %d", type);
     AQ_REQUIRE(scale_type == AQ_SCALE_POW2 || scale_type == AQ_SCALE_F32, -EINVAL, "aq_rms_norm_fwd: unknown scale type %d", scale_type);
-    AQ_REQUIRE(rows >= 0 && rows < (1LL << 22) && cols >= 1 && cols < (1LL << 31) - 16384, -EINVAL, "aq_rms_norm_fwd: bad sizes %lld x %lld", rows, cols);
+    AQ_REQUIRE(rows >= 0 && cols >= 1 && cols < (1LL << 31) - 16384, -EINVAL, "aq_rms_norm_fwd: bad sizes %lld x %lld", rows, cols);
+    AQ_REQUIRE(rows < (cols <= NORM_SHORT ? 1LL << 28 : 1LL << 22), -E2BIG, "aq_rms_norm_fwd: %lld rows of %lld are too many for one call", rows, cols);
     AQ_REQUIRE(eps >= 0, -EDOM, "aq_rms_norm_fwd: eps=%g is negative", eps);
     if (rows == 0) return 0;
     AQ_REQUIRE(x && w && (y || q || h || rstd) && (!q || qs), -EFAULT, "aq_rms_norm_fwd: NULL pointer");
@@ -403,7 +515,15 @@ int aq_rms_norm_fwd(const void *x, long long ldx, const void *res, long long ldr
             if (stream) hipLaunchKernelGGL((rms_norm_fwd_kernel<T, V, true>), g, dim3(norm_threads(cols, V)), 0, st, a);
             else hipLaunchKernelGGL((rms_norm_fwd_kernel<T, V, false>), g, dim3(norm_threads(cols, V)), 0, st, a);
         };
-        if (cols <= 256 * 8) launch(std::integral_constant<int, 1>{});
+        auto launch_short = [&](auto lanes) {
+            constexpr int LPR = decltype(lanes)::value, ROWS = 4 * 256 / LPR;
+            const dim3 gs((unsigned)((rows + ROWS - 1) / ROWS)), b(256);
+            if (stream) hipLaunchKernelGGL((rms_norm_fwd_short_kernel<T, LPR, true>), gs, b, 0, st, a);
+            else hipLaunchKernelGGL((rms_norm_fwd_short_kernel<T, LPR, false>), gs, b, 0, st, a);
+        };
+        if (cols <= 128) launch_short(std::integral_constant<int, 16>{});
+        else if (cols <= NORM_SHORT) launch_short(std::integral_constant<int, 32>{});
+        else if (cols <= 256 * 8) launch(std::integral_constant<int, 1>{});
         else if (cols <= 512 * 2 * 8) launch(std::integral_constant<int, 2>{});
         else launch(std::integral_constant<int, 4>{});
         return 0;
@@ -422,7 +542,8 @@ int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long ld
 {
     using namespace aq;
     AQ_REQUIRE(type == AQ_F32 || type == AQ_BF16 || type == AQ_F16, -EINVAL, "aq_rms_norm_bwd: unknown element type %d", type);
-    AQ_REQUIRE(rows >= 0 && rows < (1LL << 22) && cols >= 1 && cols < (1LL << 31) - 16384, -EINVAL, "aq_rms_norm_bwd: bad sizes %lld x %lld", rows, cols);
+    AQ_REQUIRE(rows >= 0 && cols >= 1 && cols < (1LL << 31) - 16384, -EINVAL, "aq_rms_norm_bwd: bad sizes %lld x %lld", rows, cols);
+    AQ_REQUIRE(rows < (cols <= NORM_SHORT ? 1LL << 28 : 1LL << 22), -E2BIG, "aq_rms_norm_bwd: %lld rows of %lld are too many for one call", rows, cols);
     AQ_REQUIRE(dx || dw, -EINVAL, "aq_rms_norm_bwd: no output is wanted");
     AQ_REQUIRE(rows == 0 || (dy && h && w && rstd), -EFAULT, "aq_rms_norm_bwd: NULL pointer");
     AQ_REQUIRE(rows == 0 || (lddy >= cols && ldh >= cols && (!dh || lddh >= cols) && (!dx || lddx >= cols)), -EINVAL,
@@ -460,7 +581,14 @@ int aq_rms_norm_bwd(const void *dy, long long lddy, const void *dh, long long ld
                 if (stream) hipLaunchKernelGGL((rms_norm_bwd_kernel<T, V, true>), dim3((unsigned)parts), dim3(norm_threads(cols, V)), 0, st, a);
                 else hipLaunchKernelGGL((rms_norm_bwd_kernel<T, V, false>), dim3((unsigned)parts), dim3(norm_threads(cols, V)), 0, st, a);
             };
-            if (cols <= 1024 * 8) launch(std::integral_constant<int, 1>{});
+            auto launch_short = [&](auto lanes) {
+                constexpr int LPR = decltype(lanes)::value;
+                if (stream) hipLaunchKernelGGL((rms_norm_bwd_short_kernel<T, LPR, true>), dim3((unsigned)parts), dim3(256), 0, st, a);
+                else hipLaunchKernelGGL((rms_norm_bwd_short_kernel<T, LPR, false>), dim3((unsigned)parts), dim3(256), 0, st, a);
+            };
+            if (cols <= 128) launch_short(std::integral_constant<int, 16>{});
+            else if (cols <= NORM_SHORT) launch_short(std::integral_constant<int, 32>{});
+            else if (cols <= 1024 * 8) launch(std::integral_constant<int, 1>{});
             else launch(std::integral_constant<int, 2>{});
             return 0;
         });

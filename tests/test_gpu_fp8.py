@@ -995,3 +995,43 @@ def test_product_of_codes_packed_without_gaps(m, n, k):
         ops.fp8_matmul(a0, b0)
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+SHORT = [(513, 1), (600, 7), (700, 8), (515, 64), (4100, 100), (40001, 128), (520, 129), (3001, 200), (9000, 256), (513, 257)]
+
+
+@pytest.mark.parametrize("rows,cols", SHORT)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_many_short_rows(rows, cols, dtype):
+    test_norm_forward(rows, cols, dtype, True)
+    test_norm_forward(rows, cols, dtype, False)
+    test_norm_backward(rows, cols, dtype)
+
+
+def test_norm_of_short_rows_in_place_and_between_others():
+    from quantized_cnn_amd import _lib
+    rows, cols, ld = 1001, 100, 130
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, r, dy, dh = (torch.randn(rows + 1, ld, device=DEV, generator=g).bfloat16() for _ in range(4))
+    w = torch.randn(cols, device=DEV, generator=g)
+    y, h, rstd = ops.rms_norm_forward(x[:rows, 3:103], w, residual=r[:rows, 5:105])
+    q, _, _ = ops.rms_norm_forward(x[:rows, 3:103], w, residual=r[:rows, 5:105], quantize=True)
+    dx, dw = ops.rms_norm_backward(dy[:rows, 1:101], h, w, rstd, dh=dh[:rows, 7:107])
+    # h over x, y between other values, dx over dh
+    keep_x, keep_dh = x.clone(), dh.clone()
+    out, qc, qs, rs = torch.full_like(x, 3.0), torch.full((rows + 1, 112), 0x55, device=DEV, dtype=torch.uint8), torch.full((rows + 1,), 0x55, device=DEV, dtype=torch.uint8), torch.empty_like(rstd)
+    at = x[0, 3:].data_ptr()
+    _lib.check(_lib.lib().aq_rms_norm_fwd(at, ld, r[0, 5:].data_ptr(), ld, 1, w.data_ptr(), rows, cols, 1e-6, out[0, 2:].data_ptr(), ld, qc.data_ptr(), 112,
+                                          qs.data_ptr(), 1, 0, at, ld, rs.data_ptr(), _lib.stream()))
+    assert torch.equal(x[:rows, 3:103], h) and torch.equal(out[:rows, 2:102], y) and torch.equal(rs, rstd)
+    assert np.array_equal(qc[:rows, :100].cpu().numpy(), codes_of(q)) and np.array_equal(qs[:rows].cpu().numpy() - 127.0, exps_of(q)[:, 0])
+    x[:rows, 3:103] = keep_x[:rows, 3:103]
+    out[:rows, 2:102] = 3.0
+    assert torch.equal(x, keep_x) and bool((out == 3.0).all()) and bool((qc[:, 100:] == 0x55).all()) and bool((qc[rows] == 0x55).all()) and int(qs[rows]) == 0x55
+    ws = torch.empty(_lib.lib().aq_rms_norm_bwd_workspace_bytes(rows, cols), dtype=torch.uint8, device=DEV)
+    at, dw2 = dh[0, 7:].data_ptr(), torch.empty_like(dw)
+    _lib.check(_lib.lib().aq_rms_norm_bwd(dy[0, 1:].data_ptr(), ld, at, ld, h.data_ptr(), cols, 1, w.data_ptr(), rstd.data_ptr(), rows, cols, at, ld, dw2.data_ptr(),
+                                          ws.data_ptr(), ws.numel(), _lib.stream()))
+    assert torch.equal(dh[:rows, 7:107], dx) and torch.equal(dw2, dw)
+    dh[:rows, 7:107] = keep_dh[:rows, 7:107]
+    assert torch.equal(dh, keep_dh)
