@@ -5,13 +5,14 @@
 // The matrix instruction takes B's rows as its first operand and A's as its second: a lane then holds four neighbouring
 // columns n of one row m.  Three ways to the sum over a block:
 //   POW2:  power-of-two scales go into the scaled 16x16x128 instruction itself; one instruction per block, fp32 accumulator.
-//   FP32S: scales of any value: the block's sum from a zero accumulator, then acc += sum * (sA * sB) in fp32.
+//   FP32S: scales of any value: the block's sum from a zero accumulator, then acc += sum * (sA * sB) in fp32 (add_scaled() where
+//          sA * sB leaves fp32's normal numbers).
 //   EXACT: fp32 outputs.  The 8-bit instruction aligns the products of 8 neighbouring k to the largest of them and drops what
 //          lies 2^-14 below it (measured; 1.5e-5 of a sum of 128 normally distributed products): nothing beside the rounding of
 //          a 16-bit output, too much for an fp32 one.  The codes, which are exact in fp16, go through the 16x16x32 fp16
 //          instruction instead (measured 1e-8), then as FP32S.
-//   WIDE:  the same for large products with power-of-two scales: code * scale is exact in bf16 (for scales of 2^-117 and more; below,
-//          a code's last bits fall under bf16's smallest step), so the scales go into the conversion, the blocks' sums into
+//   WIDE:  the same for large products with power-of-two scales: code * scale is exact in bf16 (for scales of 2^-124 to 2^119; what has
+//          others is computed as EXACT at the end), so the scales go into the conversion, the blocks' sums into
 //          one accumulator through the bf16 instruction, and the fp32 multiplications per block are saved.
 //
 // What bounds them, measured: 8192^3 to bf16 0.43 ms, 2.56 PFLOP/s (a library product of fp8 matrices with one scale: 2.64): the power
@@ -82,6 +83,19 @@ template <int MODE> __device__ inline f4_t block_product(const i8_t &b, const i8
 #pragma unroll
     for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_to_fp16(b[2 * i], b[2 * i + 1]), codes_to_fp16(a[2 * i], a[2 * i + 1]), s, 0, 0, 0);
     return s;
+}
+
+// |scale| may be multiplied with another such one: 2^-63 .. 2^63, whose products are normal fp32 numbers (0, infinities and NaN are
+// outside as well)
+__device__ inline bool outside(uint32_t bits) { return (bits & 0x7fffffffu) - 0x20000000u > 0x3f000000u; }
+// acc + sum * sa * sb for scales of any value.  Where sa * sb is no normal number, the mantissas are multiplied and the exponents added:
+// a sum of zeros stays zero, and what the scales bring back to an ordinary size is kept.
+__device__ inline float add_scaled(float acc, float sum, float sa, float sb)
+{
+    const float s = sa * sb, a = fabsf(s);
+    if (a >= 0x1p-126f && a < __builtin_inff()) return __builtin_fmaf(sum, s, acc);
+    const float m = __builtin_amdgcn_frexp_mantf(sa) * __builtin_amdgcn_frexp_mantf(sb);
+    return acc + __builtin_ldexpf(sum * m, __builtin_amdgcn_frexp_expf(sa) + __builtin_amdgcn_frexp_expf(sb));
 }
 
 template <typename T> __device__ inline void store4(T *p, int n, const f4_t &v)
@@ -358,14 +372,69 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
     }
 }
 
+// The kernels below multiply the scales of a block in fp32, or put them into bf16 values: wavefronts that meet scales so far from 1 that
+// this loses something compute their 64 x 64 outputs again at the end, block by block from memory with add_scaled().
+// Where there are none the watch costs 1 to 2 % (any scales, 4096^3: 16-bit output 82 -> 84 us, fp32 150 -> 152 us).
+// power-of-two scales with which all codes are bf16 numbers: the smallest code is 2^-9 and bf16's smallest step 2^-133, the largest code 448
+constexpr uint32_t BF16_LOW = 127 - 124, BF16_HIGH = 127 + 119;
+__device__ inline bool far_scales(const MatArgs &p, int m0, int n0, int lane)
+{
+    const long long a = (long long)((m0 + lane) >> p.ashift) * p.ldas, b = (long long)(min(n0 + lane, p.N - 1) >> p.bshift) * p.ldbs;
+    auto far = [&](const void *s, long long i) {
+        if (p.scale_f32) {
+            const uint32_t u = static_cast<const uint32_t *>(s)[i], v = u & 0x7fffffffu;
+            return outside(u) && v != 0 && v < 0x7f800000u;
+        }
+        const uint32_t e = static_cast<const uint8_t *>(s)[i];
+        return e < BF16_LOW || (e > BF16_HIGH && e != 255);
+    };
+    bool any = false;
+    for (int kb = 0; kb * FP8_BLK < p.K; ++kb) any |= far(p.as, a + kb) || far(p.bs, b + kb);
+    return __any(any);
+}
+template <typename T> __device__ inline void careful_part(const MatArgs &p, int m0, int n0, int lane)
+{
+    asm volatile("" : "+v"(lane));  // (nothing of this is worked out ahead, in registers that the kernel's own loop needs)
+    const int r = lane & 15, g = lane >> 4, kround = (p.K + 15) & ~15;
+    auto piece = [&](const uint8_t *row, int k) {
+        i4_t v = {0, 0, 0, 0};
+        if (k < kround) v = *reinterpret_cast<const i4_t *>(row + k);
+        return mask16(v, k, p.K);
+    };
+    auto fragment = [&](const uint8_t *row, int k) {
+        const i4_t lo = piece(row, k + 16 * g), hi = piece(row, k + 16 * g + 64);
+        return i8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+#pragma unroll 1
+    for (int f = 0; f < 16; ++f) {  // 16 x 16 outputs: four columns n of row m in every lane
+        const int m = m0 + 16 * (f & 3) + r, nf = n0 + 16 * (f >> 2), n = nf + 4 * g;
+        const uint8_t *ar = p.a + (long long)m * p.lda, *br = p.b + (long long)min(nf + r, p.N - 1) * p.ldb;
+        f4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int kb = 0; kb * FP8_BLK < p.K; ++kb) {
+            const f4_t sum = block_product<EXACT>(fragment(br, kb * FP8_BLK), fragment(ar, kb * FP8_BLK), acc, 0, 0);
+            const float sa = load_scale(p.as, (long long)(m >> p.ashift) * p.ldas + kb, p.scale_f32);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                acc[e] = add_scaled(acc[e], sum[e], sa, load_scale(p.bs, (long long)(min(n + e, p.N - 1) >> p.bshift) * p.ldbs + kb, p.scale_f32));
+        }
+        if (p.bias)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) acc[e] += p.bias[n + e];
+        store4(static_cast<T *>(p.y) + (long long)m * p.ldy + n, p.N - n, acc);
+    }
+}
+
 // Large products with scales of any value and fp32 outputs: the tile's blocks of K in two stages of LDS as above; per block and pair of
 // fragments the block's sum from zero, through fp16, then acc += sum * (sA * sB).
 template <int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kernel(const MatArgs p)
+__global__ __launch_bounds__(WM *WN * 64, 2) void fp8_matmul_block_kernel(const MatArgs p)
 {
     constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr int LOADS = (BM + BN) / 8 / WAVES, STAGE = (BM + BN) * FP8_BLK;
     static_assert((BM + BN) % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && BM + BN <= WAVES * 64, "");
+    static_assert(TM == 2 && TN == 2, "careful_part() has 64 x 64 outputs");
     __shared__ __attribute__((aligned(128))) uint8_t tile[2 * STAGE];
     __shared__ __attribute__((aligned(16))) float scale[2][BM + BN];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -393,7 +462,8 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
     long long sfirst = 0;
     if (tid < BM) ssrc = p.as, sfirst = (long long)((m0 + tid) >> p.ashift) * p.ldas;
     else if (tid < BM + BN) ssrc = p.bs, sfirst = (long long)((n0 + tid - BM) >> p.bshift) * p.ldbs;
-    auto read_scale = [&](int kb) { return tid < BM + BN ? static_cast<const float *>(ssrc)[sfirst + kb] : 0.0f; };
+    auto read_scale = [&](int kb) { return tid < BM + BN ? static_cast<const float *>(ssrc)[sfirst + kb] : 1.0f; };
+    bool far = false;  // one of the scales that passed through this thread is outside()
 
     f16_t acc[TM][TN];
 #pragma unroll
@@ -456,21 +526,24 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_block_kern
     fetch(0, 0);
     const float first = read_scale(0);
     if (tid < BM + BN) scale[0][tid] = first;
+    far |= outside(__float_as_uint(first));
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     for (int kb = 0; kb < nkb; ++kb) {
         const int stage = kb & 1;
         // the next block's scale is asked for before its codes, so that the wait for the one is not a wait for the other
-        const float next = kb + 1 < nkb ? read_scale(kb + 1) : 0.0f;
+        const float next = kb + 1 < nkb ? read_scale(kb + 1) : 1.0f;
         if (kb + 1 < nkb) fetch(kb + 1, stage ^ 1);
         if ((kb + 1) * FP8_BLK <= p.K) block(kb, stage, false);
         else block(kb, stage, true);
         if (tid < BM + BN) scale[stage ^ 1][tid] = next;
+        far |= outside(__float_as_uint(next));
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
+    if (__syncthreads_or(far) && far_scales(p, m0 + wm, n0 + wn, lane)) return careful_part<float>(p, m0 + wm, n0 + wn, lane);
     float *y = static_cast<float *>(p.y);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -549,10 +622,15 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_scaled_kernel(const MatA
     // scales of the block whose sums wait: of this lane's rows m, and (BTILE) of the fragments' columns; before the first block zeros
     float sa[2] = {0.f, 0.f}, sb[2] = {0.f, 0.f};
     if (!BTILE) scale[3][tid] = 0.0f;
+    float least = 1.0f, most = 1.0f;  // magnitudes of this wavefront's scales
     auto read_scales = [&](int kb) {
         const float *sc = scale[kb & 3];
         sa[0] = sc[wm + row], sa[1] = sc[wm + 32 + row];
-        if (BTILE) sb[0] = sc[BM + wn], sb[1] = sc[BM + wn + 32];
+        float b0, b1;
+        if (BTILE) b0 = sb[0] = sc[BM + wn], b1 = sb[1] = sc[BM + wn + 32];
+        else b0 = b1 = sc[BM + wn + lane];
+        least = fminf(fminf(fminf(least, fabsf(sa[0])), fminf(fabsf(sa[1]), fabsf(b0))), fabsf(b1));
+        most = fmaxf(fmaxf(fmaxf(most, fabsf(sa[0])), fmaxf(fabsf(sa[1]), fabsf(b0))), fabsf(b1));
     };
     // sums of block kb into the accumulators
     auto scale_in = [&](int i, int j, int kb) {
@@ -640,6 +718,8 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_scaled_kernel(const MatA
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int t = 0; t < 4; ++t) scale_in(t & 1, t >> 1, nkb - 1);
+    if (__any(outside(__float_as_uint(least)) || outside(__float_as_uint(most))) && far_scales(p, m0 + wm, n0 + wn, lane))
+        return careful_part<T>(p, m0 + wm, n0 + wn, lane);
     T *y = static_cast<T *>(p.y);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -733,9 +813,12 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_wide_kernel(const MatArg
         raw[f][0] = *(lds_i4)(p0 + stage * STAGE + (f & 1) * 4096);
         raw[f][1] = *(lds_i4)(p1 + stage * STAGE + (f & 1) * 4096);
     };
+    uint32_t least = 127, most = 127;
     auto read_scales = [&](int stage) {
 #pragma unroll
         for (int f = 0; f < 4; ++f) sc[stage][f] = *(lds_u1)((f < 2 ? asread : bsread) + stage * WAVES * 256 + (f & 1) * 128);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) least = min(least, sc[stage][f]), most = max(most, sc[stage][f]);
     };
     auto convert = [&](b8_t(&to)[4][4], int f, int w, uint32_t s) {  // (the conversion takes the exponent field alone: 2^(b - 127) for b = 0 too)
         to[f][w] = codes_to_bf16(raw[f][w >> 1][2 * (w & 1)], raw[f][w >> 1][2 * (w & 1) + 1], __uint_as_float(s << 23));
@@ -786,6 +869,7 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_wide_kernel(const MatArg
             if (kb + s < nkb) block(kb + s, s);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (__any(least < BF16_LOW || most > BF16_HIGH) && far_scales(p, m0 + wm, n0 + wn, lane)) return careful_part<float>(p, m0 + wm, n0 + wn, lane);
     float *y = static_cast<float *>(p.y);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -840,6 +924,14 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_rows_kernel(const MatArgs p
         return MODE == POW2 ? static_cast<const uint8_t *>(s)[i] : __float_as_uint(load_scale(s, i, p.scale_f32));
     };
     auto multiply = [&](const i8_t(&af)[TM], const i8_t(&bf)[TN], const uint32_t(&sa)[TM], const uint32_t(&sb)[TN]) {
+        bool far = false;
+        if (MODE != POW2) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) far |= outside(sa[i]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) far |= outside(sb[j]);
+            far = __any(far);
+        }
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             if (MODE == POW2) {
@@ -852,6 +944,11 @@ __global__ __launch_bounds__(512, 2) void fp8_matmul_rows_kernel(const MatArgs p
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
                     const f4_t s = block_product<MODE>(bf[j], af[i], acc[i][j], 0, 0);
+                    if (far) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] = add_scaled(acc[i][j][e], s[e], __uint_as_float(sa[i]), sn[e]);
+                        continue;
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(s[e], sn[e] * __uint_as_float(sa[i]), acc[i][j][e]);
                 }

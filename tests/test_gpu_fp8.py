@@ -1035,3 +1035,53 @@ def test_norm_of_short_rows_in_place_and_between_others():
     assert torch.equal(dh[:rows, 7:107], dx) and torch.equal(dw2, dw)
     dh[:rows, 7:107] = keep_dh[:rows, 7:107]
     assert torch.equal(dh, keep_dh)
+
+
+FAR = [(1, 64, 400), (20, 130, 384), (40, 700, 1025), (300, 900, 500), (512, 700, 384), (1030, 1100, 389), (4200, 4300, 260)]
+
+
+@pytest.mark.parametrize("m,n,k", FAR)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_product_of_scales_far_from_one(m, n, k, dtype, pow2):
+    """Scales of one operand that those of the other bring back to an ordinary size, block by block; the tolerance is check_product's."""
+    nb, g = -(-k // 128), torch.Generator(device=DEV).manual_seed(k)
+    far = torch.tensor([124.0, -124.0, 0.0, -119.0, 70.0, 112.0, -90.0, 121.0, -121.0], device=DEV)[:nb]
+    for br in (1, 128):
+        ops_ = []
+        for rows, sign, blocks in ((m, 1, 1), (n, -1, br)):
+            q = operand(rows, k, blocks, True, rows, False)
+            e = sign * far + torch.randint(-2, 3, q.scale.shape, device=DEV, generator=g)
+            s = torch.exp2(e.double()) * (1 if pow2 else 1 + 0.9 * torch.rand(q.scale.shape, device=DEV, generator=g, dtype=torch.float64))
+            ops_.append(ops.Fp8Blocks(q.data, s.float().to(E8) if pow2 else s.float(), blocks))
+        assert np.isfinite(check_product(*ops_, torch.randn(n, device=DEV, generator=g), dtype)).all()
+
+
+@pytest.mark.parametrize("m,n,k", FAR)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_product_of_scales_whose_product_leaves_the_range(m, n, k, dtype, pow2):
+    def filled(rows, v, e):
+        s = torch.full((rows, -(-k // 128)), 2.0 ** e, device=DEV)
+        return ops.Fp8Blocks(torch.full((rows, k + -k % 16), v, device=DEV).to(torch.float8_e4m3fn)[:, :k], s.to(E8) if pow2 else s)
+    # 2^200 times nothing is nothing
+    a, b = filled(m, 0.0, 100), filled(n, 1.0, 100)
+    assert bool((ops.fp8_matmul(a, b, out_dtype=dtype) == 0).all())
+    # one product of the smallest codes: 2^-18 * 2^140
+    a, b = filled(m, 0.0, 70), filled(n, 0.0, 70)
+    a.data[m - 1, k - 1], b.data[:, k - 1] = 2.0 ** -9, 2.0 ** -9
+    y = ops.fp8_matmul(a, b, out_dtype=dtype)
+    assert bool((y[m - 1] == 2.0 ** 122).all()) and bool((y[:m - 1] == 0).all())
+    # 2^-150 times sums that reach a normal number; all sums are multiples of 2^-138 below 2^-120: exact in fp32
+    y = ops.fp8_matmul(filled(m, 448.0, -75), filled(n, 448.0, -75), out_dtype=dtype)
+    assert bool((y == torch.tensor(k * 448.0 ** 2 * 2.0 ** -150, dtype=torch.float64).to(dtype).to(DEV)).all())
+
+
+@pytest.mark.parametrize("e", [-124, -123, -117, 112, 119])
+def test_large_product_between_the_borders_of_its_scales(e):
+    """Scales of one operand, 2^e, and of the other, 2^f, up to the last ones that 16-bit values hold: the same sums bit for bit."""
+    one = lambda q, v: ops.Fp8Blocks(q.data, torch.full(q.scale.shape, 2.0 ** v, device=DEV).to(E8), q.block_rows)  # noqa: E731
+    a, b = operand(1100, 300, 1, True, 1), operand(900, 300, 128, True, 2)  # (codes of all magnitudes)
+    want = ops.fp8_matmul(one(a, 0), one(b, 0), out_dtype=torch.float32)
+    f = min(-e, 119)
+    assert torch.equal(ops.fp8_matmul(one(a, e), one(b, f), out_dtype=torch.float32), want * 2.0 ** (e + f))
