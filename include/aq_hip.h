@@ -474,9 +474,10 @@ size_t aq_fp8_quantize_workspace_bytes(long long rows, long long cols);
 int aq_fp8_quantize(const void *x, int xtype, long long rows, long long cols, long long ldx, uint8_t *q, long long ldq, void *qs,
                     long long ldqs, uint8_t *qt, long long ldqt, void *qts, long long ldqts, int block_rows, int scale_type,
                     float *colsum, void *workspace, size_t workspace_bytes, void *stream);
-/* Codes and scales of the transpose of a matrix that is in the format already.  block_rows = 128: the same codes; block_rows =
- * 1: the values are quantised again in blocks along the other axis (exact but for values that fall below the new block's
- * smallest subnormal step). */
+/* Codes and scales of the transpose of a matrix that is in the format already.  block_rows = 128: the same codes and scales; block_rows =
+ * 1: the values code * scale, formed in fp32 (beyond its range: NaN), are quantised again in blocks along the other axis, as
+ * aq_fp8_quantize does it.  With power-of-two scales that is exact but for values that fall below the new block's smallest
+ * subnormal step; with others it is a second rounding, off by up to 2^-4 of a value. */
 int aq_fp8_transpose(const uint8_t *a, long long lda, const void *as, long long ldas, long long rows, long long cols, uint8_t *at,
                      long long ldat, void *ats, long long ldats, int block_rows, int scale_type, void *stream);
 /* y[i, j] = code * scale, rounded to y's type. */

@@ -1077,8 +1077,10 @@ def fp8_quantize(x, forms="rows", block_rows=1, scale_dtype=torch.float8_e8m0fnu
 
 
 def fp8_transpose(q):
-    """Fp8Blocks of the transposed matrix.  Tiles of 128 x 128 keep their codes; 1 x 128 blocks are formed anew along the other axis
-    (exact but for values below the new block's smallest subnormal step)."""
+    """Fp8Blocks of the transposed matrix.  Tiles of 128 x 128 keep their codes and scales; 1 x 128 blocks are formed anew along the other axis,
+    with power-of-two scales, from the values code * scale in fp32 (beyond its range: NaN).  Where the scales are powers of two
+    already, that is exact but for values below the new block's smallest subnormal step; where they are not, it is a second rounding, off
+    by up to 2^-4 of a value."""
     if q.device.index != _current_device():
         with torch.cuda.device(q.device):
             return fp8_transpose(q)

@@ -1085,3 +1085,23 @@ def test_large_product_between_the_borders_of_its_scales(e):
     want = ops.fp8_matmul(one(a, 0), one(b, 0), out_dtype=torch.float32)
     f = min(-e, 119)
     assert torch.equal(ops.fp8_matmul(one(a, e), one(b, f), out_dtype=torch.float32), want * 2.0 ** (e + f))
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 129), (130, 257), (64, 1000)])
+def test_transpose_of_rows_with_scales_of_any_value(rows, cols):
+    """A second rounding: the codes are those of the fp32 values code * scale, off by up to half a step of 2^-3, 2^-4 of a value (or half a
+    subnormal step of the new block)."""
+    q = ops.fp8_quantize(features(rows, cols, torch.float32, 4), scale_dtype=torch.float32)
+    q = ops.Fp8Blocks(q.data, q.scale * (0.5 + torch.rand(q.scale.shape, device=DEV)))
+    v = F8.VALUES[codes_of(q)].astype(np.float32) * np.repeat(q.scale.cpu().numpy(), 128, 1)[:, :cols]
+    t = ops.fp8_transpose(q)
+    c, e = F8.quantize(v.T)
+    same_codes(codes_of(t), c)
+    assert t.scale.dtype == torch.float32 and np.array_equal(exps_of(t), e)
+    got, step = f64(ops.fp8_dequantize(t, torch.float32)).T, np.repeat(2.0 ** (e - 9.0), 128, 1)[:, :rows].T
+    assert np.all(np.abs(got - v) <= np.maximum(2.0 ** -4 * np.abs(v), step / 2))
+    # values that fp32 does not hold
+    q.scale[1, 0] = 2.0 ** 127
+    q.data[1, 0], q.data[1, 1] = 448.0, 1.0
+    t = ops.fp8_transpose(q)
+    assert bool(torch.isnan(t.data[0, 1].float())) and float(ops.fp8_dequantize(t, torch.float32)[1, 1]) == 2.0 ** 127
