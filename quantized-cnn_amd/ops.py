@@ -1111,7 +1111,8 @@ def fp8_dequantize(q, dtype=torch.bfloat16):
 
 def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     """a (M, K) @ b (N, K)^T + bias (N,) of two Fp8Blocks with scales of one type -> (M, N).  fp32 outputs keep fp32 sums; bf16 and
-    fp16 outputs run on the 8-bit matrix instructions (error of a sum up to 2^-13 of the sum of its terms' magnitudes)."""
+    fp16 outputs run on the 8-bit matrix instructions: the sum of a group of 8 neighbouring k is off by less than 7 * 2^-13 of the group's
+    largest product (of 8 times that where a subnormal code has part in it)."""
     if not isinstance(a, Fp8Blocks) or not isinstance(b, Fp8Blocks):
         raise ValueError("fp8_matmul: both operands have to be Fp8Blocks")
     M, K = a.shape
