@@ -10,6 +10,7 @@ product's contraction, weights in 128 x 128 tiles.  The weight gradient of fp32 
 roundings unchanged (straight through).  The reference has no such layer: parity unpinned.
 """
 import math
+import weakref
 
 import torch
 import torch.nn as nn
@@ -189,14 +190,35 @@ class Fp8Linear(nn.Module):
         bound = 1 / math.sqrt(in_feature)
         nn.init.uniform_(self.weight, -bound, bound)
         self.bias = nn.Parameter(torch.empty(out_feature).uniform_(-bound, bound)) if bias else None
-        self._packed = None
+        self._packed = self._packed_of = None
 
     def pack(self):
-        """Quantises the weight once, for serving: forward() under no_grad in eval mode then reads the codes.  They are of the weight as
-        it is now; train(), load_state_dict() and moving the module drop them."""
+        """Quantises the weight once, for serving: forward() under no_grad in eval mode then reads the codes.  train(), load_state_dict(),
+        moving the module, another parameter in the weight's place, the training steps and torch's writes to it drop them; only a write
+        through `weight.data` or from outside torch (a graph of one's own) goes unnoticed: call pack() again after it."""
         with torch.no_grad():
-            self._packed = _weight_forms(self.weight, False)[0]
+            self._packed, self._packed_of = _weight_forms(self.weight, False)[0], self._weight_state()
         return self
+
+    def _weight_state(self):
+        """The weight's storage and how often it has been written (a tensor made in inference mode does not count that)."""
+        w = self.weight
+        return weakref.ref(w), None if w.is_inference() else w._version
+
+    def _packed_codes(self):
+        """The kept codes; None, for good, if the weight is not the one that they were made of any more."""
+        if self._packed is not None and self._packed_of != self._weight_state():
+            self._packed = None
+        return self._packed
+
+    def __getstate__(self):  # (copies and pickles: the codes go along if they are the weight's)
+        self._packed_codes()
+        return dict(self.__dict__, _packed_of=None)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if self._packed is not None:
+            self._packed_of = self._weight_state()
 
     def train(self, mode=True):
         if mode:
@@ -212,11 +234,11 @@ class Fp8Linear(nn.Module):
         return super()._load_from_state_dict(*args, **kw)
 
     def buffers_changed(self):
-        """Called where a data-parallel wrapper has written the parameters in place."""
+        """Called where a data-parallel wrapper or a captured or fused step has written the parameters in place."""
         self._packed = None
 
     def forward(self, x):
-        if self._packed is not None and not self.training and not torch.is_grad_enabled():
+        if self._packed is not None and not self.training and not torch.is_grad_enabled() and self._packed_codes() is not None:
             return linear(x, self._packed, self.bias)
         return linear(x, self.weight, self.bias)
 

@@ -138,6 +138,17 @@ class DataParallel:
         layers.set_dW_reduce_hook(None)
 
 
+def _layers_with_codes(model):
+    """Layers that may keep codes of their weights: replayed graphs and the update kernels write the weights without torch's notice."""
+    from .fp8 import Fp8Linear
+    return [m for m in model.modules() if isinstance(m, Fp8Linear)]
+
+
+def _drop_codes(layers_with_codes):
+    for m in layers_with_codes:
+        m.buffers_changed()
+
+
 def _clip(opts, max_norm):
     """Clips the gradients of all parameters of the optimizers by their common norm, on the device -> the norm."""
     from . import ops
@@ -160,6 +171,7 @@ class TrainStep:
     def __init__(self, model, config, module, dp=None, use_graph=False, max_norm=None):
         self.model, self.config, self.module, self.dp = model, config, module, dp
         self.max_norm, self.grad_norm = _checked_max_norm(max_norm), None
+        self._coded = _layers_with_codes(model)
         self.criterion = nn.CrossEntropyLoss()
         self.use_graph = use_graph
         self.opts = make_optimizers(model, config, capturable=use_graph)
@@ -197,6 +209,7 @@ class TrainStep:
         self._sx.copy_(x)
         self._sy.copy_(y)
         self._graph.replay()
+        _drop_codes(self._coded)
         self.logits = self._slogits
         return self._sloss
 
@@ -251,6 +264,7 @@ class CapturedStep:
         self.model, self.loss_fn, self.warmup = model, loss_fn, warmup
         self.opts = list(optimizers) if isinstance(optimizers, (list, tuple)) else [optimizers]
         self.max_norm, self.grad_norm = _checked_max_norm(max_norm), None
+        self._coded = _layers_with_codes(model)
         self._graph = None
 
     def _body(self):
@@ -290,6 +304,7 @@ class CapturedStep:
         self._sx.copy_(x)
         self._sy.copy_(y)
         self._graph.replay()
+        _drop_codes(self._coded)
         return self.loss
 
 
@@ -357,6 +372,7 @@ class FusedTrainStep:
         self.criterion = nn.CrossEntropyLoss()
         self.opts = make_optimizers(model, config, capturable=use_graph, fused=True)
         self.qlayers = model.quant_layers()
+        self._coded = _layers_with_codes(model)
         dev = next(model.parameters()).device
         named = list(model.named_parameters())
         self.dense = [p for n, p in named if "p_c" not in n and "q_level" not in n and p.requires_grad]
@@ -501,6 +517,7 @@ class FusedTrainStep:
             self._phase_a(x, y)
             self._comm()
             self._phase_b()
+            _drop_codes(self._coded)
             return self.loss
         key = (tuple(x.shape), float(self.module.beta), tuple(g["lr"] for o in self.opts for g in o.param_groups), self._exchange)
         if self._graphs is None or key != self._key:
@@ -514,6 +531,7 @@ class FusedTrainStep:
         if self._graphs[1] is not None:
             self._comm()
             self._graphs[1].replay()
+        _drop_codes(self._coded)
         return self.loss
 
     def invalidate(self):
@@ -621,6 +639,7 @@ class FusedTernaryStep:
         if any(isinstance(m, layers._QuantBase) for m in model.modules()):
             raise ValueError("FusedTernaryStep: adaptive (p_c / q_level) layers belong to FusedTrainStep")
         self.qlayers = self.tern or self.inq
+        self._coded = _layers_with_codes(model)
         if self.tern:
             keys = {(l.mode_q, l.factor, l.threshold_from_max) for l in self.tern}
             if len(keys) != 1:
@@ -773,6 +792,7 @@ class FusedTernaryStep:
             self._phase_a(x, y)
             self._comm()
             self._phase_b()
+            _drop_codes(self._coded)
             return self.loss
         key = (tuple(x.shape), tuple(g["lr"] for g in self.opts[0].param_groups), self._exchange)
         if self._graphs is None or key != self._key:
@@ -786,6 +806,7 @@ class FusedTernaryStep:
         if self._graphs[1] is not None:
             self._comm()
             self._graphs[1].replay()
+        _drop_codes(self._coded)
         return self.loss
 
     def invalidate(self):

@@ -1158,3 +1158,56 @@ def test_product_cuts_what_is_stated(m, n, dtype, pow2, kind):
     assert bool(((y - total).abs() <= tol)[fits].all())
     assert bool(((y - want).abs() <= cut + tol)[fits].all())
     assert kind != "border" or bool(((total - want).abs() > 2 * tol).any())  # (the large ones cancel: the cut shows)
+
+
+def test_packed_codes_do_not_outlive_a_write_to_the_weight():
+    import copy
+    import pickle
+    x = torch.randn(3, 130, device=DEV)
+    layer = fp8.Fp8Linear(130, 40).to(DEV).eval().pack()
+
+    def check(kept):
+        with torch.no_grad():
+            assert torch.equal(layer(x), fp8.linear(x, layer.weight, layer.bias))
+        assert (layer._packed is not None) == kept
+    check(True)
+    with torch.no_grad():
+        layer.weight.mul_(2.0)  # an averaged or a rescaled weight, in evaluation mode
+    check(False)
+    layer.pack().weight = torch.nn.Parameter(torch.randn(130, 40, device=DEV))
+    check(False)
+    layer.pack()
+    opt = torch.optim.SGD([layer.weight], 0.1)  # a step in evaluation mode
+    layer(x).sum().backward()
+    check(True)
+    opt.step()
+    check(False)
+    layer.pack()
+    with torch.no_grad():
+        torch._foreach_add_([layer.weight], 1.0)
+    check(False)
+    # copies take the codes along, if they are the weight's, and drop them in their own time
+    for twin in (copy.deepcopy(layer.pack()), pickle.loads(pickle.dumps(layer))):
+        with torch.no_grad():
+            assert twin._packed is not None and torch.equal(twin(x), layer(x)) and twin._packed is not None
+            twin.weight.add_(1.0)
+            assert torch.equal(twin(x), fp8.linear(x, twin.weight, twin.bias)) and twin._packed is None
+    check(True)
+    with torch.no_grad():
+        layer.weight.add_(1.0)
+    assert copy.deepcopy(layer)._packed is None
+    with torch.inference_mode():  # (tensors that do not count their writes)
+        served = fp8.Fp8Linear(130, 40).to(DEV).eval().pack()
+        assert torch.equal(served(x), fp8.linear(x, served.weight, served.bias)) and served._packed is not None
+
+
+def test_packed_codes_do_not_outlive_a_captured_step():
+    layer = fp8.Fp8Linear(64, 8).to(DEV)
+    x, y = torch.randn(40, 64, device=DEV), torch.randn(40, 8, device=DEV)
+    step = train.CapturedStep(layer, torch.optim.SGD(layer.parameters(), 0.1), torch.nn.functional.mse_loss, warmup=1)
+    for _ in range(3):
+        step(x, y)
+        layer.eval().pack()  # (the replays go on: the mode is of no account to a graph)
+        step(x, y)
+        with torch.no_grad():
+            assert torch.equal(layer(x), fp8.linear(x, layer.weight, layer.bias)) and layer._packed is None
