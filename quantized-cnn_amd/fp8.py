@@ -64,12 +64,25 @@ def _grad_forms(dy, need_dx, need_dw, need_db):
     return ops.fp8_quantize(dy) if need_dx else None, None, None
 
 
+def _save(ctx, blocks, *tensors):
+    """The buffers of codes (None: not needed) and tensors as saved tensors, which are freed with the graph, seen by hooks and
+    recomputed under checkpointing."""
+    ctx.blocks = tuple(q and q._on(None) for q in blocks)
+    ctx.save_for_backward(*(q and q._buf for q in blocks), *tensors)
+
+
+def _saved(ctx):
+    got, n = ctx.saved_tensors, len(ctx.blocks)
+    return tuple(q and q._on(buf) for q, buf in zip(ctx.blocks, got)) + got[n:]
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, out_dtype):
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        xq, ctx.xt = ops.fp8_quantize(x, forms="both") if need_dw else (ops.fp8_quantize(x), None)
-        wt, ctx.w = _weight_forms(weight, need_dx)
+        xq, xt = ops.fp8_quantize(x, forms="both") if need_dw else (ops.fp8_quantize(x), None)
+        wt, w = _weight_forms(weight, need_dx)
+        _save(ctx, (xt, w))
         ctx.types = x.dtype, weight.dtype, bias.dtype if bias is not None else None
         return ops.fp8_matmul(xq, wt, bias=bias.float() if bias is not None else None, out_dtype=out_dtype)
 
@@ -77,10 +90,11 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        xt, w = _saved(ctx)
         xtype, wtype, btype = ctx.types
         dq, dt, db = _grad_forms(_flat(dy), need_dx, need_dw, need_db)
-        dx = ops.fp8_matmul(dq, ctx.w, out_dtype=xtype) if need_dx else None
-        dw = ops.fp8_matmul(ctx.xt, dt, out_dtype=wtype) if need_dw else None
+        dx = ops.fp8_matmul(dq, w, out_dtype=xtype) if need_dx else None
+        dw = ops.fp8_matmul(xt, dt, out_dtype=wtype) if need_dw else None
         return dx, dw, db.to(btype) if need_db else None, None
 
 
@@ -109,11 +123,10 @@ class _NormLinear(torch.autograd.Function):
     def forward(ctx, x, norm_weight, weight, bias, residual, eps, out_dtype):
         need_dn = ctx.needs_input_grad[0] or ctx.needs_input_grad[1] or ctx.needs_input_grad[4]
         xq, h, rstd = ops.rms_norm_forward(x, norm_weight, residual=residual, eps=eps, quantize=True)
-        wt, ctx.w = _weight_forms(weight, need_dn)
-        ctx.xq = xq if ctx.needs_input_grad[2] else None
+        wt, w = _weight_forms(weight, need_dn)
         ctx.types = x.dtype, weight.dtype, bias.dtype if bias is not None else None
         ctx.both = residual is not None
-        ctx.save_for_backward(h, norm_weight, rstd)
+        _save(ctx, (xq if ctx.needs_input_grad[2] else None, w), h, norm_weight, rstd)
         ctx.set_materialize_grads(False)
         y = ops.fp8_matmul(xq, wt, bias=bias.float() if bias is not None else None, out_dtype=out_dtype)
         return (y, h) if ctx.both else y
@@ -121,17 +134,17 @@ class _NormLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, norm_weight, rstd = ctx.saved_tensors
+        xq, w, h, norm_weight, rstd = _saved(ctx)
         need_x, need_nw, need_dw, need_db, need_r = ctx.needs_input_grad[:5]
         if dy is None:
             return dh, None, None, None, dh if ctx.both else None, None, None
         need_dn = need_x or need_nw or need_r
         xtype, wtype, btype = ctx.types
         dq, dt, db = _grad_forms(_flat(dy), need_dn, need_dw, need_db)
-        dw = ops.fp8_matmul(ops.fp8_transpose(ctx.xq), dt, out_dtype=wtype) if need_dw else None
+        dw = ops.fp8_matmul(ops.fp8_transpose(xq), dt, out_dtype=wtype) if need_dw else None
         dx = dnw = None
         if need_dn:
-            dn = ops.fp8_matmul(dq, ctx.w, out_dtype=xtype)
+            dn = ops.fp8_matmul(dq, w, out_dtype=xtype)
             dx, dnw = ops.rms_norm_backward(dn, h, norm_weight, rstd, dh=_flat(dh) if dh is not None else None, need_dx=need_x or need_r,
                                             need_dweight=need_nw)
         return dx, dnw, dw, db.to(btype) if need_db else None, dx if ctx.both else None, None, None

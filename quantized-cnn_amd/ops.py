@@ -1000,6 +1000,14 @@ class Fp8Blocks:
             return p, p + self._soff
         return self._data.data_ptr(), self._scale.data_ptr()
 
+    def _on(self, buf):
+        """The same matrix made here, its codes and scales in `buf` (None: without any)."""
+        b = Fp8Blocks.__new__(Fp8Blocks)
+        b._data = b._scale = None
+        b._buf, b._soff, b.block_rows, b.shape, b.device = buf, self._soff, self.block_rows, self.shape, self.device
+        b._ld, b._lds, b._scale_type = self._ld, self._lds, self._scale_type
+        return b
+
     def _by16(self):
         """Codes whose rows can be read 16 bytes at a time up to their last: (tensor to keep alive, address, pitch)."""
         if self._buf is not None:

@@ -1211,3 +1211,43 @@ def test_packed_codes_do_not_outlive_a_captured_step():
         step(x, y)
         with torch.no_grad():
             assert torch.equal(layer(x), fp8.linear(x, layer.weight, layer.bias)) and layer._packed is None
+
+
+@pytest.mark.parametrize("layer", ["linear", "norm_linear"])
+def test_codes_for_the_backward_pass_are_saved_tensors(layer):
+    """Freed by the backward pass though the loss is kept, seen by hooks, recomputed under checkpointing, gone for a second pass."""
+    from torch.utils.checkpoint import checkpoint
+    m, n = 2048, 1024
+    x, w = torch.randn(m, n, device=DEV, requires_grad=True), torch.randn(n, n, device=DEV, requires_grad=True)
+    nw = torch.rand(n, device=DEV, requires_grad=True)
+    leaves = (x, w) if layer == "linear" else (x, w, nw)
+
+    def call(t):
+        return fp8.linear(t, w) if layer == "linear" else fp8.norm_linear(t, nw, w)
+
+    def used():
+        torch.cuda.synchronize()
+        return torch.cuda.memory_allocated()
+    want = torch.autograd.grad(call(x).square().sum(), leaves)
+    loss = call(x).sum()  # (its graph holds no result: the codes of x and w and, with a norm, x's own statistics)
+    got = torch.autograd.grad(loss, leaves)
+    del got
+    before = used()
+    del loss
+    assert before - used() < n * n // 4
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (packed.append(t.numel() * t.element_size()), t.cpu())[1], lambda t: t.to(DEV)):
+        y = call(x)
+    assert sum(p >= n * n for p in packed) >= 2 and any(m * n <= p <= 1.1 * m * n for p in packed)
+    for a, c in zip(torch.autograd.grad(y.square().sum(), leaves), want):
+        assert torch.equal(a, c)
+    y = checkpoint(call, x, use_reentrant=False)
+    for a, c in zip(torch.autograd.grad(y.square().sum(), leaves), want):
+        assert torch.equal(a, c)
+    y = call(x)
+    for _ in range(2):
+        for a, c in zip(torch.autograd.grad(y, leaves, 2 * y.detach(), retain_graph=True), want):
+            assert torch.equal(a, c)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
