@@ -37,21 +37,40 @@ def _weight_forms(weight, need_dx):
     return ops.fp8_quantize(_flat(weight), forms="cols", block_rows=ops.FP8_BLOCK), None
 
 
-def _checked(out):
-    """out, the result of a Function's apply, after a check of the leaves among its arguments.  A leaf's gradient is accumulated on the stream
-    that was current when its first graph was made.  If that graph lives on and was made on the default stream, a backward pass in a
-    capture would make that stream wait for the capture, which ends the process: it is refused here, where nothing is lost yet."""
-    fn = (out[0] if isinstance(out, tuple) else out).grad_fn
+def _leaf_nodes(fn, weights):
+    """The AccumulateGrad nodes of the leaves behind fn's operands: through views, casts and other operators of one operand, behind the operands
+    at the places `weights` through any operators; not through nodes of this module, whose own call has looked behind them."""
+    found = []
+    for i, (node, _) in enumerate(fn.next_functions):
+        stack = [node]
+        while stack:
+            node = stack.pop()
+            name = type(node).__name__
+            if name == "AccumulateGrad":
+                found.append(node)
+            elif node is not None and name not in ("_LinearBackward", "_RmsNormBackward", "_NormLinearBackward"):
+                behind = [n for n, _ in node.next_functions if n is not None]
+                if len(behind) == 1 or i in weights:
+                    stack += behind
+    return found
+
+
+def _checked(out, weights):
+    """out, the result of a Function's apply, after a check of the leaves behind its operands (`weights`: places of the weights among them).  A leaf's
+    gradient is accumulated on the stream that was current when its first graph was made.  If that graph lives on and was made on the
+    default stream, a backward pass in a capture would make that stream wait for the capture, which ends the process: it is refused here,
+    where nothing is lost yet."""
+    first = out[0] if isinstance(out, tuple) else out
+    fn = first.grad_fn
     if fn is not None:
         capturing = torch.cuda.is_current_stream_capturing()
-        eager = not capturing and torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()) == 0
-        for node, _ in fn.next_functions:
-            if node is not None and type(node).__name__ == "AccumulateGrad":
-                if capturing and node.metadata.get("fp8_default_stream"):
+        if capturing or ops._current_stream(first.device.index) == 0:
+            for node in _leaf_nodes(fn, weights):
+                if not capturing:
+                    node.metadata.setdefault("fp8_default_stream", True)
+                elif node.metadata.get("fp8_default_stream"):
                     raise RuntimeError("fp8: a graph of the same parameters, made on the default stream, is still alive (a loss or an output is kept): "
                                        "its gradients cannot be captured; delete or detach it before the capture")
-                if eager:
-                    node.metadata.setdefault("fp8_default_stream", True)
     return out
 
 
@@ -167,14 +186,14 @@ def linear(x, weight, bias=None, out_dtype=None):
     else:
         if weight.dim() != 2 or weight.shape[0] != x.shape[-1]:
             raise ValueError("fp8.linear: x %s / weight %s: need (..., in) and (in, out)" % (tuple(x.shape), tuple(weight.shape)))
-        y = _checked(_Linear.apply(x2, weight, bias, out_dtype))
+        y = _checked(_Linear.apply(x2, weight, bias, out_dtype), (1, 2))
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (y.shape[1],))
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight over the last axis -> (y, h), or y alone without residual."""
     _check_residual("rms_norm", x, residual)
-    out = _checked(_RmsNorm.apply(_flat(x), weight.float(), _flat(residual) if residual is not None else None, eps))
+    out = _checked(_RmsNorm.apply(_flat(x), weight.float(), _flat(residual) if residual is not None else None, eps), (1,))
     if residual is None:
         return out.view(x.shape)
     return out[0].view(x.shape), out[1].view(x.shape)
@@ -188,7 +207,7 @@ def norm_linear(x, norm_weight, weight, bias=None, residual=None, eps=1e-6, out_
         raise ValueError("fp8.norm_linear: x %s / weight %s: need (..., in) and (in, out)" % (tuple(x.shape), tuple(weight.shape)))
     _check_residual("norm_linear", x, residual)
     out = _checked(_NormLinear.apply(_flat(x), norm_weight.float(), weight, bias, _flat(residual) if residual is not None else None, eps,
-                                     out_dtype or x.dtype))
+                                     out_dtype or x.dtype), (1, 2, 3) if bias is not None else (1, 2))
     y, h = out if residual is not None else (out, None)
     y = y.view(x.shape[:-1] + (y.shape[1],))
     return y if residual is None else (y, h.view(x.shape))

@@ -136,3 +136,32 @@ def test_matmul_refuses_scales_too_far_apart(ldas, ldbs):
 def test_repitch_refusals(args, word):
     rc, err = _rc("aq_fp8_repitch", *args)
     assert rc < 0 and word in err, err
+
+
+def test_leaves_behind_operands_are_found():
+    """(the check before a capture looks at them)"""
+    from quantized_cnn_amd import fp8
+
+    class _Linear(torch.autograd.Function):  # (any node of that name)
+        @staticmethod
+        def forward(ctx, x, w, b):
+            return x @ w.float() + (0 if b is None else b)
+
+        @staticmethod
+        def backward(ctx, g):
+            return g, g, g
+    leaf = lambda *s, t=torch.float32: torch.randn(*s).to(t).requires_grad_(True)  # noqa: E731
+
+    def names(out, weights):
+        return sorted(id(n.variable) for n in fp8._leaf_nodes(out.grad_fn, weights))
+    ids = lambda *ts: sorted(map(id, ts))  # noqa: E731
+    x, w, b = leaf(2, 3, 4), leaf(5, 4, t=torch.bfloat16), leaf(5)
+    y = _Linear.apply(x.view(6, 4), w.t(), b)
+    assert names(y, (1, 2)) == ids(x, w, b)
+    lo, hi = leaf(4, 2), leaf(2, 5)
+    y = _Linear.apply(x.view(6, 4).relu(), torch.randn(4, 5) + lo @ hi, None)  # a weight of several leaves
+    assert names(y, (1, 2)) == ids(x, lo, hi)
+    z = _Linear.apply(y, torch.randn(5, 5), b)  # behind a node of this kind its own call has looked
+    assert names(z, (1, 2)) == ids(b)
+    u, v = leaf(6, 4), leaf(6, 4)
+    assert names(_Linear.apply(u + v, w.float().t(), None), (1, 2)) == ids(w)  # (what other operators join is theirs)

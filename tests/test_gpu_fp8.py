@@ -1251,3 +1251,34 @@ def test_codes_for_the_backward_pass_are_saved_tensors(layer):
     y.sum().backward()
     with pytest.raises(RuntimeError, match="second time"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("case", ["16-bit norm", "transposed weight", "input of three dimensions"])
+def test_capture_beside_a_live_eager_graph_is_refused_behind_views_and_casts(case):
+    """The leaf is marked on the host, before anything is captured."""
+    x = torch.randn(4, 8, 256, device=DEV, dtype=torch.bfloat16 if case == "16-bit norm" else torch.float32, requires_grad=case.startswith("input"))
+    nw = torch.ones(256, device=DEV, dtype=x.dtype, requires_grad=case == "16-bit norm")
+    w = torch.randn(64, 256, device=DEV, requires_grad=case == "transposed weight")
+    (leaf,) = [t for t in (x, nw, w) if t.requires_grad]
+    calls = [lambda: fp8.norm_linear(x, nw, w.t())]
+    calls += [lambda: fp8.rms_norm(x, nw)] if leaf is not w else []
+    calls += [lambda: fp8.linear(x, w.t())] if leaf is not nw else []
+    for call in calls:
+        kept = call().float().square().sum()
+        node = torch.autograd.graph.get_gradient_edge(leaf).node
+        assert node.metadata.get("fp8_default_stream")
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        torch.cuda.synchronize()
+        want = torch.autograd.grad(kept, leaf)[0]
+        del kept, node
+        s = torch.cuda.Stream()  # nothing is alive: the same call is captured
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+            got = torch.autograd.grad(call().float().square().sum(), leaf)[0]
+        for _ in range(3):
+            got.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
