@@ -1220,6 +1220,17 @@ def rms_norm_backward(dy, h, weight, rstd, dh=None, need_dx=True, need_dweight=T
 
 # ------------------------------------------------------------------- gradient norm over all tensors
 
+def in_memory_order(t):
+    """A contiguous view of a dense tensor, its axes in the order in which they lie in memory: what `grad_norm` and `clip_grad_norm` take of a
+    gradient whose parameter is transposed or channels_last (a gradient has its parameter's strides)."""
+    if t.is_contiguous():
+        return t
+    v = t.permute(sorted(range(t.dim()), key=lambda d: (t.shape[d] == 1, -t.stride(d))))
+    if not v.is_contiguous():
+        raise ValueError("in_memory_order: strides %s of shape %s leave gaps or overlap" % (t.stride(), tuple(t.shape)))
+    return v
+
+
 def _grad_lists(tensors):
     """(addresses, sizes, types) of a list of gradients as arrays, and their device; checked in bulk, a training step has many."""
     T = torch.Tensor
@@ -1231,7 +1242,8 @@ def _grad_lists(tensors):
         for i, t in enumerate(tensors):
             _hip(t, "tensor[%d]" % i)
             if t.device != dev or t.dtype not in _lib.ELEMENT_TYPES or not t.is_contiguous():
-                raise ValueError("tensor[%d]: %s on %s, strides %s: contiguous float32, bfloat16 or float16 tensors of one device are expected" % (
+                raise ValueError("tensor[%d]: %s on %s, strides %s: contiguous float32, bfloat16 or float16 tensors of one device are expected (in_memory_order() makes a "
+                                 "contiguous view of one that is dense in another order)" % (
                     i, t.dtype, t.device, t.stride()))
     if len(kinds) == 1:
         types = array.array("i", [_lib.ELEMENT_TYPES[kinds.pop()]]) * len(ptrs)

@@ -153,7 +153,7 @@ def _clip(opts, max_norm):
     """Clips the gradients of all parameters of the optimizers by their common norm, on the device -> the norm."""
     from . import ops
     params = dict.fromkeys(p for o in opts for g in o.param_groups for p in g["params"] if p.grad is not None)  # (once each, if two optimizers share one)
-    return ops.clip_grad_norm([p.grad for p in params], max_norm)
+    return ops.clip_grad_norm([ops.in_memory_order(p.grad) for p in params], max_norm)
 
 
 def _checked_max_norm(max_norm):

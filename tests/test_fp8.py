@@ -165,3 +165,15 @@ def test_leaves_behind_operands_are_found():
     assert names(z, (1, 2)) == ids(b)
     u, v = leaf(6, 4), leaf(6, 4)
     assert names(_Linear.apply(u + v, w.float().t(), None), (1, 2)) == ids(w)  # (what other operators join is theirs)
+
+
+def test_dense_gradients_in_memory_order():
+    from quantized_cnn_amd import ops
+    for t in (torch.randn(4, 6).t(), torch.randn(2, 3, 4, 5).to(memory_format=torch.channels_last), torch.randn(3, 1, 5).permute(2, 1, 0), torch.randn(7),
+              torch.tensor(2.0), torch.empty(0, 3).t(), torch.randn(1, 5).t(), torch.randn(2, 3, 4).permute(1, 2, 0)):
+        v = ops.in_memory_order(t)
+        assert v.is_contiguous() and v.data_ptr() == t.data_ptr() and v.numel() == t.numel()
+        assert torch.equal(v.flatten().sort()[0], t.flatten().sort()[0])
+    for t in (torch.randn(4, 6)[:, :5], torch.randn(1, 5).expand(3, 5), torch.randn(9).as_strided((3, 3), (2, 1)), torch.randn(6, 4)[::2].t()):
+        with pytest.raises(ValueError, match="gaps or overlap"):
+            ops.in_memory_order(t)

@@ -1282,3 +1282,33 @@ def test_capture_beside_a_live_eager_graph_is_refused_behind_views_and_casts(cas
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+
+
+def test_steps_clip_gradients_in_any_dense_order():
+    """A transposed and a channels_last parameter, whose gradients have their strides."""
+    torch.manual_seed(0)
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.conv = torch.nn.Conv2d(3, 8, 3).to(memory_format=torch.channels_last)
+            self.lin = fp8.Fp8Linear(8, 5)
+            self.lin.weight = torch.nn.Parameter(torch.randn(5, 8).t())
+
+        def forward(self, x):
+            return self.lin(self.conv(x).mean((2, 3)))
+    net = Net().to(DEV)
+    x, y = torch.randn(6, 3, 9, 9, device=DEV), torch.randn(6, 5, device=DEV)
+    step = train.CapturedStep(net, torch.optim.SGD(net.parameters(), 0.0), torch.nn.functional.mse_loss, warmup=1, max_norm=1e-3)
+    for _ in range(3):
+        step(x, y)
+        torch.cuda.synchronize()
+        gs = [p.grad for p in net.parameters()]
+        assert sum(not g.is_contiguous() for g in gs) == 2
+        assert abs(F8.grad_norm([f64(g) for g in gs]) - 1e-3) <= 1e-3 * 1e-5
+        want = torch.autograd.grad(torch.nn.functional.mse_loss(net(x), y), list(net.parameters()))
+        norm = F8.grad_norm([f64(t) for t in want])
+        assert norm > 0.1 and abs(float(step.grad_norm) - norm) <= 1e-5 * norm  # (the stock convolution may sum in another order)
+        k = 1e-3 / (norm + 1e-6)
+        for g, t in zip(gs, want):
+            assert torch.allclose(g, t * k, rtol=1e-4, atol=1e-7)
