@@ -156,21 +156,34 @@ def _clip(opts, max_norm):
     return ops.clip_grad_norm([ops.in_memory_order(p.grad) for p in params], max_norm)
 
 
-def _checked_max_norm(max_norm):
-    if max_norm is not None and not max_norm > 0:
-        raise ValueError("max_norm %r: a positive number, or None for no clipping" % (max_norm,))
-    return max_norm
+class _Clipping:
+    """max_norm of a step, which may change between calls (a captured step is then captured again), and the norm of the last one."""
+    _max_norm = grad_norm = None
+
+    @property
+    def max_norm(self):
+        return self._max_norm
+
+    @max_norm.setter
+    def max_norm(self, value):
+        if value is not None and not value > 0:
+            raise ValueError("max_norm %r: a positive number, or None for no clipping" % (value,))
+        self._max_norm = None if value is None else float(value)
+
+    def _clip(self):
+        self.grad_norm = None if self._max_norm is None else _clip(self.opts, self._max_norm)
 
 
-class TrainStep:
+class TrainStep(_Clipping):
     """One optimisation step with the reference's order of operations: forward, CrossEntropy +
     model_loss, backward, optimizer_prim / optimizer_q / optimizer .step(), three zero_grad().
     max_norm: the gradients of all parameters together are clipped to this norm before the optimizers' steps (behind the
-    data-parallel exchange, so all ranks scale alike); the norm before clipping is left in `grad_norm`, a device scalar."""
+    data-parallel exchange, so all ranks scale alike); the norm before clipping is left in `grad_norm`, a device scalar.  It may be changed
+    from step to step."""
 
     def __init__(self, model, config, module, dp=None, use_graph=False, max_norm=None):
         self.model, self.config, self.module, self.dp = model, config, module, dp
-        self.max_norm, self.grad_norm = _checked_max_norm(max_norm), None
+        self.max_norm = max_norm
         self._coded = _layers_with_codes(model)
         self.criterion = nn.CrossEntropyLoss()
         self.use_graph = use_graph
@@ -185,8 +198,7 @@ class TrainStep:
         loss.backward()
         if self.dp is not None:
             self.dp.reduce_dense()
-        if self.max_norm is not None:
-            self.grad_norm = _clip(self.opts, self.max_norm)
+        self._clip()
         for o in self.opts:
             o.step()
         return loss, logits
@@ -202,7 +214,7 @@ class TrainStep:
 
     # -- whole step captured in one HIP graph ----------------------------------------------------
     def _graph_step(self, x, y):
-        key = (tuple(x.shape), float(self.module.beta), tuple(g["lr"] for o in self.opts for g in o.param_groups))
+        key = (tuple(x.shape), float(self.module.beta), tuple(g["lr"] for o in self.opts for g in o.param_groups), self.max_norm)
         if self._graph is None or key != self._key:
             self._capture(x, y)
             self._key = key
@@ -246,7 +258,7 @@ class TrainStep:
         self._graph = g
 
 
-class CapturedStep:
+class CapturedStep(_Clipping):
     """A training step of any model on torch autograd with torch optimizers - forward, loss_fn(model(x), y), backward,
     optimizer.step() - captured once and replayed as ONE HIP graph (the library's kernels are launched on torch's current
     stream, so they are captured like stock operators).  For the models outside the reference's three-optimizer loop
@@ -255,7 +267,7 @@ class CapturedStep:
     the capture; every call
     copies (x, y) into the graph's input buffers and replays.  Shapes must stay fixed; SyncBatchNorm is refused.
     max_norm: the gradients of all parameters of the optimizers together are clipped to this norm before their steps; the norm
-    before clipping is left in `grad_norm`, a device scalar."""
+    before clipping is left in `grad_norm`, a device scalar.  Assigning another one captures the step again at the next call."""
 
     def __init__(self, model, optimizers, loss_fn, warmup=2, max_norm=None):
         if warmup < 1:  # optimizers create their state (momentum, Adam's averages) in their first step: a capture of THAT
@@ -263,7 +275,7 @@ class CapturedStep:
             raise ValueError("CapturedStep: at least one eager warm-up step is needed before the capture")
         self.model, self.loss_fn, self.warmup = model, loss_fn, warmup
         self.opts = list(optimizers) if isinstance(optimizers, (list, tuple)) else [optimizers]
-        self.max_norm, self.grad_norm = _checked_max_norm(max_norm), None
+        self.max_norm = max_norm
         self._coded = _layers_with_codes(model)
         self._graph = None
 
@@ -271,8 +283,7 @@ class CapturedStep:
         out = self.model(self._sx)
         loss = self.loss_fn(out, self._sy)
         loss.backward()
-        if self.max_norm is not None:
-            self.grad_norm = _clip(self.opts, self.max_norm)
+        self._clip()
         for o in self.opts:
             o.step()
         self.loss, self.output = loss.detach(), out.detach()
@@ -289,18 +300,24 @@ class CapturedStep:
                     o.zero_grad(set_to_none=True)
                 self._body()
         torch.cuda.current_stream().wait_stream(s)
+        self._record()
+
+    def _record(self):
+        self._graph = None
         for o in self.opts:
             o.zero_grad(set_to_none=True)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self._body()
-        self._graph = g
+        self._graph, self._recorded_norm = g, self.max_norm
 
     def __call__(self, x, y):
         if self._graph is None:
             self._capture(x, y)  # (the capture itself does not execute: the replay below is this call's step)
         elif tuple(x.shape) != tuple(self._sx.shape) or tuple(y.shape) != tuple(self._sy.shape):
             raise ValueError("CapturedStep: batch shape changed (%s -> %s); build a new step" % (tuple(self._sx.shape), tuple(x.shape)))
+        elif self.max_norm != self._recorded_norm:
+            self._record()
         self._sx.copy_(x)
         self._sy.copy_(y)
         self._graph.replay()

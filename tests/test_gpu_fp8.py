@@ -1312,3 +1312,46 @@ def test_steps_clip_gradients_in_any_dense_order():
         k = 1e-3 / (norm + 1e-6)
         for g, t in zip(gs, want):
             assert torch.allclose(g, t * k, rtol=1e-4, atol=1e-7)
+
+
+def test_max_norm_of_captured_steps_may_change():
+    import argparse
+    import quantized_cnn_amd.adp_qtz_fan as fan
+    torch.manual_seed(0)
+    a, b = fp8.Fp8Linear(64, 8).to(DEV), fp8.Fp8Linear(64, 8).to(DEV)
+    b.load_state_dict(a.state_dict())
+    loss = torch.nn.functional.mse_loss
+    opt = torch.optim.SGD(a.parameters(), 0.1, momentum=0.9)
+    step = train.CapturedStep(b, torch.optim.SGD(b.parameters(), 0.1, momentum=0.9), loss, warmup=1, max_norm=1e-2)
+
+    def eager(x, y, max_norm):
+        opt.zero_grad(set_to_none=True)
+        loss(a(x), y).backward()
+        norm = ops.clip_grad_norm([p.grad for p in a.parameters()], max_norm) if max_norm else None
+        opt.step()
+        return norm
+    for i, max_norm in enumerate((1e-2, 1e-2, 3e-3, None, None, 0.5, 1e-2)):
+        x, y = torch.randn(40, 64, device=DEV), torch.randn(40, 8, device=DEV)
+        step.max_norm = max_norm
+        if i == 0:
+            eager(x, y, max_norm)  # (the warm-up step)
+        norm = eager(x, y, max_norm)
+        step(x, y)
+        torch.cuda.synchronize()
+        assert (step.grad_norm is None) == (norm is None) and (norm is None or torch.equal(step.grad_norm, norm))
+        assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters())), i
+    for bad in (0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            step.max_norm = bad
+    c = argparse.Namespace(mode="train", prim_init="uniform", num_level_conv=32, num_level_fc=32, l2_reg=5e-4, liar=True, prim_lr=1e-2, q_lr=1e-3, lr=1e-2)
+    fan.beta = 1
+    net = fan.ResNet(c, 3).to(DEV).train()
+    x, y = torch.randn(8, 3, 32, 32, device=DEV), torch.randint(0, 10, (8,), device=DEV)
+    step = train.TrainStep(net, c, fan, use_graph=True, max_norm=0.1)
+    graphs = []
+    for max_norm in (0.1, 0.1, 0.2, None, None):
+        step.max_norm = max_norm
+        step(x, y)
+        graphs.append(step._graph)
+        assert (step.grad_norm is None) == (max_norm is None)
+    assert graphs[0] is graphs[1] is not graphs[2] and graphs[2] is not graphs[3] is graphs[4]
