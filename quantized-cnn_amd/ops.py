@@ -908,8 +908,9 @@ FP8_BLOCK = 128
 _SCALE_TYPES = {torch.float8_e8m0fnu: _lib.SCALE_POW2, torch.float32: _lib.SCALE_F32}
 
 
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# (short ways to torch.cuda.current_device() and current_stream(i).cuda_stream; a torch without a GPU back end has them not)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _hip(t, name, device=None):

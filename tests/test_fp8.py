@@ -177,3 +177,18 @@ def test_dense_gradients_in_memory_order():
     for t in (torch.randn(4, 6)[:, :5], torch.randn(1, 5).expand(3, 5), torch.randn(9).as_strided((3, 3), (2, 1)), torch.randn(6, 4)[::2].t()):
         with pytest.raises(ValueError, match="gaps or overlap"):
             ops.in_memory_order(t)
+
+
+def test_package_imports_on_a_torch_without_a_gpu_back_end():
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for name in [n for n in dir(torch._C) if n.startswith('_cuda')]: delattr(torch._C, name)\n"
+            "import quantized_cnn_amd.layers, quantized_cnn_amd.checkpoint, quantized_cnn_amd.fp8, quantized_cnn_amd.train\n"
+            "from quantized_cnn_amd import ops\n"
+            "try: ops.fp8_quantize(torch.zeros(2, 2))\n"
+            "except RuntimeError as e: print('refused:', e)\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "HIP device only" in r.stdout, r.stderr[-2000:]
