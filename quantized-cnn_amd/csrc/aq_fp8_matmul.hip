@@ -24,6 +24,7 @@
 #include "aq_fp8.h"
 
 #pragma clang diagnostic ignored "-Wint-to-pointer-cast"  // LDS addresses have 32 bits; the host pass does not know
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 among the clobbers: no register for the allocator, but instruction selection writes it too
 
 namespace aq {
 
@@ -118,15 +119,15 @@ typedef float f16_t __attribute__((ext_vector_type(16)));
 // pipeline needs it.
 __device__ inline void load_to_lds(uint32_t lds, uint32_t off, const uint8_t *base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
 }
 __device__ inline void load_byte_to_lds(uint32_t lds, uint32_t off, const uint8_t *base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
 }
 __device__ inline void load_word_to_lds(uint32_t lds, uint32_t off, const uint8_t *base)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0", "memory");
 }
 template <typename P> __device__ inline uint32_t lds_address(P *p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) P *)p; }
 

@@ -192,3 +192,15 @@ def test_package_imports_on_a_torch_without_a_gpu_back_end():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "HIP device only" in r.stdout, r.stderr[-2000:]
+
+
+def test_inline_assembly_names_what_it_writes():
+    """m0 is the compiler's too: assembly that writes it has to say so."""
+    import os
+    import re
+    src = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "quantized-cnn_amd", "csrc")
+    for name in sorted(os.listdir(src)):
+        if name.endswith((".hip", ".h")):
+            with open(os.path.join(src, name)) as f:
+                for stmt in re.findall(r"asm volatile\(.*?\);", f.read(), re.S):
+                    assert "m0," not in stmt or '"m0"' in stmt, (name, stmt)
