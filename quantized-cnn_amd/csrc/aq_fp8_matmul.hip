@@ -1071,7 +1071,8 @@ static int matmul_splits(long long M, long long N, long long K)
 //   Products so large that they run at the power limit (2^38 multiplications and more) with four wavefronts of 128 x 128, which read a third less
 //   from LDS, smaller ones with eight of 64 x 128, whose waits overlap (8192^3: 429 against 462 us, 16384 x 8192 x 2048: 270 against 285 us;
 //   8192 x 8192 x 2048: 120 against 117.5 us, 5000^3: 145 against 141 us).
-//   Not for a round and a few tiles more (2316 x 6403 x 1632, 260 tiles: 58 us, 44 us in 128 x 128; 4352 x 4096 x 1024, 272: 33 against 29 us);
+//   Not for a round and a few tiles more (2316 x 6403 x 1632, 260 tiles: 58 us, 44 us in 128 x 128; 4352 x 4096 x 1024, 272: 33.5 against 30 us;
+//   from 321 on again: 5120 x 4352 x 1024, 340: 34.6 against 35.2 us, 4608 x 4864 x 2048, 342: 53.5 against 54, 4096 x 6144 x 4096, 384: 95 against 101 us);
 //   128 x 128 with two stages, two workgroups on a unit, for more than a round (1500 x 5000 x 2560: 25 us against 30 us with four stages);
 //   128 x 128 with four stages for up to a round (1024 x 4096: 22 against 28 us with two);
 //   64 x 128 for fewer (512 x 4096: 17 us; 1000 x 1000 x 1000: 8 against 11 us), K in parts for very few.
@@ -1099,7 +1100,9 @@ template <int MODE, typename T> static void launch_block(MatArgs p, hipStream_t 
 {
     // Two workgroups of 128 x 128 on a compute unit run past each other's barriers (fp32 output 512 x 4096 x 4096: 30 us against 46 us for one
     // of 128 x 256, any scales 28 against 34 us); with scales in fp32 arithmetic the larger tile wins once there are two
-    // rounds of it (4096^3: 16-bit output 82 against 86 us, fp32 output 147 against 191 us).
+    // rounds of it (4096^3: 16-bit output 84 against 86 us, fp32 output 152 against 191 us).  In one nearly full round it gains where the
+    // round is full and loses where it is not (16-bit output, 1500 x 5000 x 2560, 240 tiles: 34.4 against 31.5 us; 2048 x 4096 x 4096, 256: 43
+    // against 45.5 us), and is not taken.
     const bool wide = p.scale_f32 && p.N >= 256 && tiles_of(p.M, p.N, 128, 256) >= 512;
     p.tiles_m = (p.M + 127) / 128;
     p.tiles_n = wide ? (p.N + 255) / 256 : (p.N + 127) / 128;

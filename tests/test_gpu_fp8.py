@@ -1355,3 +1355,38 @@ def test_max_norm_of_captured_steps_may_change():
         graphs.append(step._graph)
         assert (step.grad_norm is None) == (max_norm is None)
     assert graphs[0] is graphs[1] is not graphs[2] and graphs[2] is not graphs[3] is graphs[4]
+
+
+@pytest.mark.parametrize("m,c,n", [(60, 520, 200), (150, 130, 260)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_linear_against_the_oracle(m, c, n, dtype):
+    """Every quantisation by the oracle, products and norm in float64.  The weight gradient reads the norm's codes, quantised anew along the
+    rows.  dx: an error e of the product's gradient dn comes through as rstd (|w| e + |n| mean(|w n| e))."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    mk = lambda *s: torch.randn(*s, device=DEV, generator=g)  # noqa: E731
+    x, r = mk(m, c).to(dtype).requires_grad_(True), mk(m, c).to(dtype).requires_grad_(True)
+    nw, w, b = (1 + 0.1 * mk(c)).requires_grad_(True), (mk(c, n) / 20).requires_grad_(True), mk(n).requires_grad_(True)
+    dy, dh = mk(m, n).to(dtype), mk(m, c).to(dtype)
+    y, h = fp8.norm_linear(x, nw, w, b, residual=r)
+    dx, dr, dnw, dw, db = torch.autograd.grad((y, h), (x, r, nw, w, b), (dy, dh))
+    hv = (x.detach().float() + r.detach().float()).to(dtype)
+    rstd = F8.rms_norm(f64(hv), f64(nw), 1e-6)[1].astype(np.float32)
+    codes, e = F8.quantize((hv.float().cpu().numpy() * rstd[:, None]) * nw.detach().cpu().numpy())
+    xv, wv, dv, dt = F8.values(codes, 2.0 ** e.astype(np.float64)), rounded(w, 128), rounded(dy), rounded(dy, turn=True)
+    assert torch.equal(h, hv) and torch.equal(dx, dr)
+    near(y, xv @ wv + f64(b), np.abs(xv) @ np.abs(wv) + np.abs(f64(b)), dtype, c)
+    ct, et = F8.quantize(xv.T)
+    xt = F8.values(ct, 2.0 ** et.astype(np.float64))
+    near(dw, xt @ dt.T, np.abs(xt) @ np.abs(dt.T), torch.float32, m)
+    assert np.all(np.abs(f64(db) - f64(dy).sum(0)) <= U * np.abs(f64(dy).sum(0)) * 1.01 + 1e-12 * np.abs(f64(dy)).sum(0))
+    dn, mag = dv @ wv.T, np.abs(dv) @ np.abs(wv.T)
+    cut = 2.0 ** -10 if dtype != torch.float32 else 0.0
+    err = (cut + (n + 4 * -(-n // 128)) * 2 * U) * mag
+    err = err + half_step(dtype) * (np.abs(dn) + err)
+    want, want_nw = F8.rms_norm_grad(dn, f64(hv), f64(nw), 1e-6, f64(dh))
+    rs, nv, wn = rstd[:, None].astype(np.float64), f64(hv) * rstd[:, None], np.abs(f64(nw))
+    gn = np.abs(dn) * wn
+    tol = rs * (wn * err + np.abs(nv) * (wn * err * np.abs(nv)).mean(1, keepdims=True) + 66 * U * (gn + np.abs(nv) * (gn * np.abs(nv)).mean(1, keepdims=True)))
+    tol = tol + 2 * U * np.abs(f64(dh))
+    assert np.all(np.abs(f64(dx) - want) <= tol + half_step(dtype) * (np.abs(want) + tol))
+    assert np.all(np.abs(f64(dnw) - want_nw) <= (err * np.abs(nv)).sum(0) + 8 * U * (np.abs(dn * nv)).sum(0))
