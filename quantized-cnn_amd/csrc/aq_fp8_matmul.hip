@@ -374,14 +374,16 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN / 4) void fp8_matmul_large_kern
     }
 }
 
-// The kernels below multiply the scales of a block in fp32, or put them into bf16 values: wavefronts that meet scales so far from 1 that
-// this loses something compute their 64 x 64 outputs again at the end, block by block from memory with add_scaled().
-// Where there are none the watch costs 1 to 2 % (any scales, 4096^3: 16-bit output 82 -> 84 us, fp32 150 -> 152 us).
+// The kernels below multiply the scales of a block in fp32, or put them into bf16 values.  Wavefronts that meet scales so far from 1 that
+// this loses something compute, behind their stores, the outputs of these rows and columns again, block by block from memory with
+// add_scaled().  Which outputs that are depends on the scales of their own row and column alone, so that tiles that overlap leave the
+// same values.
+// Where there are no such scales the watch costs 1 to 2 % (any scales, 4096^3: 16-bit output 82 -> 84 us, fp32 150 -> 152 us).
 // power-of-two scales with which all codes are bf16 numbers: the smallest code is 2^-9 and bf16's smallest step 2^-133, the largest code 448
 constexpr uint32_t BF16_LOW = 127 - 124, BF16_HIGH = 127 + 119;
-__device__ inline bool far_scales(const MatArgs &p, int m0, int n0, int lane)
+template <typename T> __device__ inline void careful_part(const MatArgs &p, int m0, int n0, int lane)
 {
-    const long long a = (long long)((m0 + lane) >> p.ashift) * p.ldas, b = (long long)(min(n0 + lane, p.N - 1) >> p.bshift) * p.ldbs;
+    asm volatile("" : "+v"(lane));  // (nothing of this is worked out ahead, in registers that the kernel's own loop needs)
     auto far = [&](const void *s, long long i) {
         if (p.scale_f32) {
             const uint32_t u = static_cast<const uint32_t *>(s)[i], v = u & 0x7fffffffu;
@@ -390,13 +392,12 @@ __device__ inline bool far_scales(const MatArgs &p, int m0, int n0, int lane)
         const uint32_t e = static_cast<const uint8_t *>(s)[i];
         return e < BF16_LOW || (e > BF16_HIGH && e != 255);
     };
-    bool any = false;
-    for (int kb = 0; kb * FP8_BLK < p.K; ++kb) any |= far(p.as, a + kb) || far(p.bs, b + kb);
-    return __any(any);
-}
-template <typename T> __device__ inline void careful_part(const MatArgs &p, int m0, int n0, int lane)
-{
-    asm volatile("" : "+v"(lane));  // (nothing of this is worked out ahead, in registers that the kernel's own loop needs)
+    const long long as = (long long)((m0 + lane) >> p.ashift) * p.ldas, bs = (long long)(min(n0 + lane, p.N - 1) >> p.bshift) * p.ldbs;
+    bool row_far = false, col_far = false;
+    for (int kb = 0; kb * FP8_BLK < p.K; ++kb) row_far |= far(p.as, as + kb), col_far |= far(p.bs, bs + kb);
+    const uint64_t rows = __ballot(row_far), cols = __ballot(col_far);
+    if (!(rows | cols)) return;  // (zeros, infinities or NaN)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores of the same outputs
     const int r = lane & 15, g = lane >> 4, kround = (p.K + 15) & ~15;
     auto piece = [&](const uint8_t *row, int k) {
         i4_t v = {0, 0, 0, 0};
@@ -409,6 +410,8 @@ template <typename T> __device__ inline void careful_part(const MatArgs &p, int 
     };
 #pragma unroll 1
     for (int f = 0; f < 16; ++f) {  // 16 x 16 outputs: four columns n of row m in every lane
+        const uint32_t fr = (uint32_t)(rows >> 16 * (f & 3)) & 0xffff, fc = (uint32_t)(cols >> 16 * (f >> 2)) & 0xffff;
+        if (!(fr | fc)) continue;
         const int m = m0 + 16 * (f & 3) + r, nf = n0 + 16 * (f >> 2), n = nf + 4 * g;
         const uint8_t *ar = p.a + (long long)m * p.lda, *br = p.b + (long long)min(nf + r, p.N - 1) * p.ldb;
         f4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -420,11 +423,10 @@ template <typename T> __device__ inline void careful_part(const MatArgs &p, int 
             for (int e = 0; e < 4; ++e)
                 acc[e] = add_scaled(acc[e], sum[e], sa, load_scale(p.bs, (long long)(min(n + e, p.N - 1) >> p.bshift) * p.ldbs + kb, p.scale_f32));
         }
-        if (p.bias)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < p.N) acc[e] += p.bias[n + e];
-        store4(static_cast<T *>(p.y) + (long long)m * p.ldy + n, p.N - n, acc);
+        for (int e = 0; e < 4; ++e)
+            if (n + e < p.N && ((fr >> r | fc >> (4 * g + e)) & 1))
+                static_cast<T *>(p.y)[(long long)m * p.ldy + n + e] = from_f32<T>(p.bias ? acc[e] + p.bias[n + e] : acc[e]);
     }
 }
 
@@ -545,7 +547,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_matmul_block_kernel(const 
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
-    if (__syncthreads_or(far) && far_scales(p, m0 + wm, n0 + wn, lane)) return careful_part<float>(p, m0 + wm, n0 + wn, lane);
+    const bool watch = __syncthreads_or(far);
     float *y = static_cast<float *>(p.y);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -562,6 +564,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_matmul_block_kernel(const 
                 store4(y + (long long)(m0 + wm + 32 * i + row) * p.ldy + n, 4, v + bias);
             }
         }
+    if (watch) careful_part<float>(p, m0 + wm, n0 + wn, lane);
 }
 
 // Large products with scales of any value and 16-bit outputs: tiles of 128 x BN, wavefronts with 64 x 64 each, loads and reads
@@ -720,8 +723,7 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_scaled_kernel(const MatA
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int t = 0; t < 4; ++t) scale_in(t & 1, t >> 1, nkb - 1);
-    if (__any(outside(__float_as_uint(least)) || outside(__float_as_uint(most))) && far_scales(p, m0 + wm, n0 + wn, lane))
-        return careful_part<T>(p, m0 + wm, n0 + wn, lane);
+    const bool watch = __any(outside(__float_as_uint(least)) || outside(__float_as_uint(most)));
     T *y = static_cast<T *>(p.y);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -738,6 +740,7 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_scaled_kernel(const MatA
                 store4(y + (long long)(m0 + wm + 32 * i + row) * p.ldy + n, p.N - n,
                        f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]} + bias);
         }
+    if (watch) careful_part<T>(p, m0 + wm, n0 + wn, lane);
 }
 
 // Large products with power-of-two scales and fp32 outputs: tiles of 128 x BN, wavefronts with 64 x 64 each.  K in half blocks of 64;
@@ -871,7 +874,7 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_wide_kernel(const MatArg
             if (kb + s < nkb) block(kb + s, s);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (__any(least < BF16_LOW || most > BF16_HIGH) && far_scales(p, m0 + wm, n0 + wn, lane)) return careful_part<float>(p, m0 + wm, n0 + wn, lane);
+    const bool watch = __any(least < BF16_LOW || most > BF16_HIGH);
     float *y = static_cast<float *>(p.y);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -887,6 +890,7 @@ __global__ __launch_bounds__(BN * 2, 2) void fp8_matmul_wide_kernel(const MatArg
                 *reinterpret_cast<f4_any *>(y + (long long)(m0 + wm + 32 * i + row) * p.ldy + n) =
                     f4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]} + bias;
         }
+    if (watch) careful_part<float>(p, m0 + wm, n0 + wn, lane);
 }
 
 // Few rows: bound by the reading of B.  A workgroup has 16 TN columns and 16 TM rows, its wavefronts share out the blocks of K, U

@@ -1390,3 +1390,22 @@ def test_norm_linear_against_the_oracle(m, c, n, dtype):
     tol = tol + 2 * U * np.abs(f64(dh))
     assert np.all(np.abs(f64(dx) - want) <= tol + half_step(dtype) * (np.abs(want) + tol))
     assert np.all(np.abs(f64(dnw) - want_nw) <= (err * np.abs(nv)).sum(0) + 8 * U * (np.abs(dn * nv)).sum(0))
+
+
+@pytest.mark.parametrize("m,n,k", [(333, 701, 384), (1030, 1100, 389), (4190, 4300, 260)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pow2", [True, False])
+def test_scales_far_from_one_are_their_rows_own_affair(m, n, k, dtype, pow2):
+    """Other rows and columns keep their bits, and a call repeats bit for bit where the last tiles overlap the ones before."""
+    a, b = operand(m, k, 1, pow2, 1, False), operand(n, k, 1, pow2, 2, False)
+    clean = ops.fp8_matmul(a, b, out_dtype=dtype)
+    rows, cols = torch.tensor([3, m - 100, m - 1], device=DEV), torch.tensor([0, n - 120, n - 30], device=DEV)
+    for q, at in ((a, rows), (b, cols)):
+        q.scale.view(torch.uint8 if pow2 else torch.float32)[at, 1] = 1 if pow2 else 1e-37
+    y = check_product(a, b, None, dtype)
+    keep = torch.ones_like(clean, dtype=torch.bool)
+    keep[rows], keep[:, cols] = False, False
+    y = ops.fp8_matmul(a, b, out_dtype=dtype)
+    assert torch.equal(y[keep], clean[keep])
+    for _ in range(5):
+        assert torch.equal(ops.fp8_matmul(a, b, out_dtype=dtype), y)
