@@ -229,17 +229,16 @@ class Fp8Linear(nn.Module):
         moving the module, another parameter in the weight's place, the training steps and torch's writes to it drop them; only a write
         through `weight.data` or from outside torch (a graph of one's own) goes unnoticed: call pack() again after it."""
         with torch.no_grad():
-            self._packed, self._packed_of = _weight_forms(self.weight, False)[0], self._weight_state()
+            self._packed, self._packed_of = _weight_forms(self.weight, False)[0], (weakref.ref(self.weight), self._writes())
         return self
 
-    def _weight_state(self):
-        """The weight's storage and how often it has been written (a tensor made in inference mode does not count that)."""
-        w = self.weight
-        return weakref.ref(w), None if w.is_inference() else w._version
+    def _writes(self):
+        """How often the weight has been written (tensors made in inference mode do not count that)."""
+        return None if self.weight.is_inference() else self.weight._version
 
     def _packed_codes(self):
         """The kept codes; None, for good, if the weight is not the one that they were made of any more."""
-        if self._packed is not None and self._packed_of != self._weight_state():
+        if self._packed is not None and (self._packed_of[0]() is not self.weight or self._packed_of[1] != self._writes()):
             self._packed = None
         return self._packed
 
@@ -250,7 +249,7 @@ class Fp8Linear(nn.Module):
     def __setstate__(self, state):
         super().__setstate__(state)
         if self._packed is not None:
-            self._packed_of = self._weight_state()
+            self._packed_of = weakref.ref(self.weight), self._writes()
 
     def train(self, mode=True):
         if mode:

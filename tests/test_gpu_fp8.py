@@ -1409,3 +1409,13 @@ def test_scales_far_from_one_are_their_rows_own_affair(m, n, k, dtype, pow2):
     assert torch.equal(y[keep], clean[keep])
     for _ in range(5):
         assert torch.equal(ops.fp8_matmul(a, b, out_dtype=dtype), y)
+
+
+def test_packed_codes_beside_a_parameter_that_lives_on():
+    layer = fp8.Fp8Linear(130, 40).to(DEV).eval().pack()
+    old, x = layer.weight, torch.randn(3, 130, device=DEV)
+    layer.weight = torch.nn.Parameter(torch.randn(130, 40, device=DEV))
+    with torch.no_grad():
+        assert torch.equal(layer(x), fp8.linear(x, layer.weight, layer.bias)) and layer._packed is None
+        layer.weight = old
+        assert torch.equal(layer.pack()(x), fp8.linear(x, old, layer.bias)) and layer._packed is not None
