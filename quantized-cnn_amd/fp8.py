@@ -45,10 +45,9 @@ def _leaf_nodes(fn, weights):
         stack = [node]
         while stack:
             node = stack.pop()
-            name = type(node).__name__
-            if name == "AccumulateGrad":
+            if type(node).__name__ == "AccumulateGrad":
                 found.append(node)
-            elif node is not None and name not in ("_LinearBackward", "_RmsNormBackward", "_NormLinearBackward"):
+            elif node is not None and "fp8_checked" not in node.metadata:
                 behind = [n for n, _ in node.next_functions if n is not None]
                 if len(behind) == 1 or i in weights:
                     stack += behind
@@ -63,6 +62,7 @@ def _checked(out, weights):
     first = out[0] if isinstance(out, tuple) else out
     fn = first.grad_fn
     if fn is not None:
+        fn.metadata["fp8_checked"] = True
         capturing = torch.cuda.is_current_stream_capturing()
         if capturing or ops._current_stream(first.device.index) == 0:
             for node in _leaf_nodes(fn, weights):

@@ -142,7 +142,7 @@ def test_leaves_behind_operands_are_found():
     """(the check before a capture looks at them)"""
     from quantized_cnn_amd import fp8
 
-    class _Linear(torch.autograd.Function):  # (any node of that name)
+    class Product(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, w, b):
             return x @ w.float() + (0 if b is None else b)
@@ -156,15 +156,19 @@ def test_leaves_behind_operands_are_found():
         return sorted(id(n.variable) for n in fp8._leaf_nodes(out.grad_fn, weights))
     ids = lambda *ts: sorted(map(id, ts))  # noqa: E731
     x, w, b = leaf(2, 3, 4), leaf(5, 4, t=torch.bfloat16), leaf(5)
-    y = _Linear.apply(x.view(6, 4), w.t(), b)
+    y = Product.apply(x.view(6, 4), w.t(), b)
     assert names(y, (1, 2)) == ids(x, w, b)
     lo, hi = leaf(4, 2), leaf(2, 5)
-    y = _Linear.apply(x.view(6, 4).relu(), torch.randn(4, 5) + lo @ hi, None)  # a weight of several leaves
+    y = Product.apply(x.view(6, 4).relu(), torch.randn(4, 5) + lo @ hi, None)  # a weight of several leaves
     assert names(y, (1, 2)) == ids(x, lo, hi)
-    z = _Linear.apply(y, torch.randn(5, 5), b)  # behind a node of this kind its own call has looked
+    z = Product.apply(y.relu(), torch.randn(5, 5), None)
+    assert names(z, (1, 2)) == []  # (several operands: theirs are not this call's)
+    z = Product.apply(Product.apply(x.view(6, 4), torch.randn(4, 5), None).relu(), torch.randn(5, 5), b)
+    assert names(z, (1, 2)) == ids(x, b)
+    z.grad_fn.next_functions[0][0].next_functions[0][0].metadata["fp8_checked"] = True  # a node of the module: its own call has looked
     assert names(z, (1, 2)) == ids(b)
     u, v = leaf(6, 4), leaf(6, 4)
-    assert names(_Linear.apply(u + v, w.float().t(), None), (1, 2)) == ids(w)  # (what other operators join is theirs)
+    assert names(Product.apply(u + v, w.float().t(), None), (1, 2)) == ids(w)  # (what other operators join is theirs)
 
 
 def test_dense_gradients_in_memory_order():
