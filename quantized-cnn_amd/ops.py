@@ -1001,8 +1001,14 @@ class Fp8Blocks:
             return p, p + self._soff
         return self._data.data_ptr(), self._scale.data_ptr()
 
+    def _nbytes(self):
+        rows = self.shape[0] if self.block_rows == 1 else (self.shape[0] + 127) // 128
+        return self._soff + rows * self._lds * (4 if self._scale_type else 1)
+
     def _on(self, buf):
-        """The same matrix made here, its codes and scales in `buf` (None: without any)."""
+        """The same matrix made here, its codes and scales in `buf` (None: without any), as a hook of saved tensors may have moved it."""
+        if buf is not None and (buf.device != self.device or buf.dtype != torch.uint8 or buf.shape != (self._nbytes(),) or not buf.is_contiguous()):
+            raise ValueError("Fp8Blocks: storage of %s %s on %s, expected %d bytes on %s" % (tuple(buf.shape), buf.dtype, buf.device, self._nbytes(), self.device))
         b = Fp8Blocks.__new__(Fp8Blocks)
         b._data = b._scale = None
         b._buf, b._soff, b.block_rows, b.shape, b.device = buf, self._soff, self.block_rows, self.shape, self.device

@@ -1419,3 +1419,13 @@ def test_packed_codes_beside_a_parameter_that_lives_on():
         assert torch.equal(layer(x), fp8.linear(x, layer.weight, layer.bias)) and layer._packed is None
         layer.weight = old
         assert torch.equal(layer.pack()(x), fp8.linear(x, old, layer.bias)) and layer._packed is not None
+
+
+def test_codes_that_a_hook_has_moved_away_are_refused():
+    """(a kernel would read them where they are not)"""
+    w = torch.randn(64, 64, device=DEV, requires_grad=True)
+    for unpack in (lambda t: t.cpu(), lambda t: t[:-1], lambda t: t.float() if t.dtype == torch.uint8 else t):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = fp8.linear(torch.randn(5, 64, device=DEV), w)
+        with pytest.raises(ValueError, match="storage"):
+            y.sum().backward()
