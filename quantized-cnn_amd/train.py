@@ -277,7 +277,7 @@ class CapturedStep(_Clipping):
         self.opts = list(optimizers) if isinstance(optimizers, (list, tuple)) else [optimizers]
         self.max_norm = max_norm
         self._coded = _layers_with_codes(model)
-        self._graph = None
+        self._graph, self._warm = None, False
 
     def _body(self):
         out = self.model(self._sx)
@@ -300,6 +300,7 @@ class CapturedStep(_Clipping):
                     o.zero_grad(set_to_none=True)
                 self._body()
         torch.cuda.current_stream().wait_stream(s)
+        self._warm = True
         self._record()
 
     def _record(self):
@@ -312,11 +313,11 @@ class CapturedStep(_Clipping):
         self._graph, self._recorded_norm = g, self.max_norm
 
     def __call__(self, x, y):
-        if self._graph is None:
+        if not self._warm:
             self._capture(x, y)  # (the capture itself does not execute: the replay below is this call's step)
         elif tuple(x.shape) != tuple(self._sx.shape) or tuple(y.shape) != tuple(self._sy.shape):
             raise ValueError("CapturedStep: batch shape changed (%s -> %s); build a new step" % (tuple(self._sx.shape), tuple(x.shape)))
-        elif self.max_norm != self._recorded_norm:
+        elif self._graph is None or self.max_norm != self._recorded_norm:  # (None: a capture was refused; the warm-up steps are not run again)
             self._record()
         self._sx.copy_(x)
         self._sy.copy_(y)

@@ -1429,3 +1429,24 @@ def test_codes_that_a_hook_has_moved_away_are_refused():
             y = fp8.linear(torch.randn(5, 64, device=DEV), w)
         with pytest.raises(ValueError, match="storage"):
             y.sum().backward()
+
+
+def test_a_refused_capture_does_not_repeat_the_warm_up():
+    torch.manual_seed(0)
+    a, b = fp8.Fp8Linear(64, 8).to(DEV), fp8.Fp8Linear(64, 8).to(DEV)
+    b.load_state_dict(a.state_dict())
+    x, y = torch.randn(40, 64, device=DEV), torch.randn(40, 8, device=DEV)
+    loss = torch.nn.functional.mse_loss
+    step = train.CapturedStep(b, torch.optim.SGD(b.parameters(), 0.1), loss, warmup=1)
+    kept = loss(b(x), y)
+    with pytest.raises(RuntimeError, match="still alive"):
+        step(x, y)
+    del kept
+    step(x, y)
+    opt = torch.optim.SGD(a.parameters(), 0.1)
+    for _ in range(2):
+        opt.zero_grad()
+        loss(a(x), y).backward()
+        opt.step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
