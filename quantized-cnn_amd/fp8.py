@@ -42,6 +42,9 @@ def _leaf_nodes(fn, weights):
     at the places `weights` through any operators; not through nodes of this module, whose own call has looked behind them."""
     found = []
     for i, (node, _) in enumerate(fn.next_functions):
+        if type(node).__name__ == "AccumulateGrad":
+            found.append(node)
+            continue
         stack = [node]
         while stack:
             node = stack.pop()
@@ -84,15 +87,20 @@ def _grad_forms(dy, need_dx, need_dw, need_db):
 
 
 def _save(ctx, blocks, *tensors):
-    """The buffers of codes (None: not needed) and tensors as saved tensors, which are freed with the graph, seen by hooks and
-    recomputed under checkpointing."""
-    ctx.blocks = tuple(q and q._on(None) for q in blocks)
-    ctx.save_for_backward(*(q and q._buf for q in blocks), *tensors)
+    """The buffers of two matrices of codes (None: not needed) and tensors as saved tensors, which are freed with the graph, seen by hooks and
+    recomputed under checkpointing; the matrices themselves, not used any more, stay without them."""
+    a, b = ctx.blocks = blocks
+    ctx.save_for_backward(a and a._buf, b and b._buf, *tensors)
+    if a is not None:
+        a._buf = None
+    if b is not None:
+        b._buf = None
 
 
 def _saved(ctx):
-    got, n = ctx.saved_tensors, len(ctx.blocks)
-    return tuple(q and q._on(buf) for q, buf in zip(ctx.blocks, got)) + got[n:]
+    a, b = ctx.blocks
+    p, q, *tensors = ctx.saved_tensors
+    return a and a._on(p), b and b._on(q), *tensors
 
 
 class _Linear(torch.autograd.Function):
@@ -145,9 +153,9 @@ class _NormLinear(torch.autograd.Function):
         wt, w = _weight_forms(weight, need_dn)
         ctx.types = x.dtype, weight.dtype, bias.dtype if bias is not None else None
         ctx.both = residual is not None
-        _save(ctx, (xq if ctx.needs_input_grad[2] else None, w), h, norm_weight, rstd)
         ctx.set_materialize_grads(False)
         y = ops.fp8_matmul(xq, wt, bias=bias.float() if bias is not None else None, out_dtype=out_dtype)
+        _save(ctx, (xq if ctx.needs_input_grad[2] else None, w), h, norm_weight, rstd)
         return (y, h) if ctx.both else y
 
     @staticmethod
@@ -238,8 +246,10 @@ class Fp8Linear(nn.Module):
 
     def _packed_codes(self):
         """The kept codes; None, for good, if the weight is not the one that they were made of any more."""
-        if self._packed is not None and (self._packed_of[0]() is not self.weight or self._packed_of[1] != self._writes()):
-            self._packed = None
+        if self._packed is not None:
+            (of, writes), w = self._packed_of, self.weight
+            if of() is not w or (writes is not None and writes != w._version):
+                self._packed = None
         return self._packed
 
     def __getstate__(self):  # (copies and pickles: the codes go along if they are the weight's)

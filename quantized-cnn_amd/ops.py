@@ -1006,8 +1006,8 @@ class Fp8Blocks:
         return self._soff + rows * self._lds * (4 if self._scale_type else 1)
 
     def _on(self, buf):
-        """The same matrix made here, its codes and scales in `buf` (None: without any), as a hook of saved tensors may have moved it."""
-        if buf is not None and (buf.device != self.device or buf.dtype != torch.uint8 or buf.shape != (self._nbytes(),) or not buf.is_contiguous()):
+        """The same matrix with its codes and scales in `buf`, which a hook of saved tensors may have moved."""
+        if buf.dtype != torch.uint8 or buf.numel() != self._nbytes() or buf.device != self.device or not buf.is_contiguous():
             raise ValueError("Fp8Blocks: storage of %s %s on %s, expected %d bytes on %s" % (tuple(buf.shape), buf.dtype, buf.device, self._nbytes(), self.device))
         b = Fp8Blocks.__new__(Fp8Blocks)
         b._data = b._scale = None
