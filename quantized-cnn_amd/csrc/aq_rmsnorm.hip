@@ -5,7 +5,7 @@
 // The squares are summed in double: rstd is then the correctly rounded one whatever the order of the sum, and codes next to
 // a rounding border do not depend on the launch's shape.  One pass: a row stays in the registers of its workgroup between the
 // statistics and the outputs, so the traffic is what the operands hold and the kernels are bound by memory bandwidth: 16384 x 8192
-// bf16 with residual to codes 160 us (939 MB, 5.9 TB/s), 8192 x 5120 backward 64 us + 6 us for dw's second stage (335 MB, 5.2 TB/s).
+// bf16 with residual to codes 168 us (939 MB, 5.6 TB/s), 8192 x 5120 backward 64 us + 6 us for dw's second stage (335 MB, 5.2 TB/s).
 #include <algorithm>
 
 #include "aq_fp8.h"
